@@ -29,6 +29,7 @@ static_assert(kBlockN == B200FA_BLOCK_KEYS, "capture block size mismatch");
 static_assert(kFlagCapture == B200FA_FLAG_CAPTURE, "capture flag mismatch");
 static_assert(kFlagTestBounds == B200FA_FLAG_TEST_BOUNDS, "test flag mismatch");
 static_assert(kFlagCausal == B200FA_FLAG_CAUSAL, "causal flag mismatch");
+static_assert(kFlagWindow == B200FA_FLAG_WINDOW, "window flag mismatch");
 static_assert(kDevTimeout == B200FA_DEV_TIMEOUT && kDevBounds == B200FA_DEV_BOUNDS && kDevPhase == B200FA_DEV_PHASE,
               "device status codes mismatch");
 
@@ -57,6 +58,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // Causal-mask kernels, defined in b200fa_causal.cu (B200FA_FLAG_CAUSAL).
 __global__ void b200_fa_fp16_causal_kernel(const __grid_constant__ FwdParams p);
 __global__ void b200_fa_fp32_causal_kernel(const __grid_constant__ FwdParams p);
+// Sliding-window kernels, defined in b200fa_window.cu (B200FA_FLAG_WINDOW).
+__global__ void b200_fa_fp16_window_kernel(const __grid_constant__ FwdParams p);
+__global__ void b200_fa_fp32_window_kernel(const __grid_constant__ FwdParams p);
 
 // Test hook (b200fa_test_exp2): the softmax's two exponential forms on an
 // array, pairwise as the softmax evaluates them -- exp2_poly2 (FMA pipe) into
@@ -78,7 +82,8 @@ __global__ void __launch_bounds__(256) exp2_probe_kernel(const float* x, float* 
 
 using KernelFn = void (*)(FwdParams);
 
-KernelFn kernel_for(int variant, bool capture, bool causal) {
+KernelFn kernel_for(int variant, bool capture, bool causal, bool window = false) {
+  if (window) return variant == B200FA_VARIANT_FP16 ? b200_fa_fp16_window_kernel : b200_fa_fp32_window_kernel;
   if (capture) return variant == B200FA_VARIANT_FP16 ? b200_fa_fp16_capture_kernel : b200_fa_fp32_capture_kernel;
   if (causal) return variant == B200FA_VARIANT_FP16 ? b200_fa_fp16_causal_kernel : b200_fa_fp32_causal_kernel;
   return variant == B200FA_VARIANT_FP16 ? b200_fa_fp16_kernel : b200_fa_fp32_kernel;
@@ -131,9 +136,9 @@ int device_setup(int dev, int* pairs) {
   std::call_once(d.once, [&d] {
     cudaError_t e = cudaSuccess;
     for (int variant : {B200FA_VARIANT_FP16, B200FA_VARIANT_FP32})
-      for (int kind = 0; kind < 3; ++kind)  // product, capture, causal
+      for (int kind = 0; kind < 4; ++kind)  // product, capture, causal, window
         if (e == cudaSuccess)
-          e = cudaFuncSetAttribute(kernel_for(variant, kind == 1, kind == 2),
+          e = cudaFuncSetAttribute(kernel_for(variant, kind == 1, kind == 2, kind == 3),
                                    cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (e == cudaSuccess) {
       cudaLaunchConfig_t cfg = {};
@@ -198,18 +203,17 @@ int encode_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t planes, 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // The caller's options as a full struct: NULL means defaults, and the
-// 16-byte layout without the capture fields is accepted as well.
-constexpr uint32_t kOptionsV1Bytes = 16;
+// 16-byte layout without the capture fields and the 32-byte one without the
+// window fields are accepted as well.
+constexpr uint32_t kOptionsV1Bytes = 16, kOptionsV2Bytes = 32;
 int read_options(const b200fa_options* in, b200fa_options* out) {
-  *out = b200fa_options{sizeof(b200fa_options), 0u, 0u, 0, nullptr, 0};
+  *out = b200fa_options{sizeof(b200fa_options), 0u, 0u, 0, nullptr, 0, 0, 0};
   if (in == nullptr) return B200FA_OK;
   if (in->struct_size == sizeof(b200fa_options)) {
     *out = *in;
-  } else if (in->struct_size == kOptionsV1Bytes) {
-    std::memcpy(out, in, kOptionsV1Bytes);
+  } else if (in->struct_size == kOptionsV1Bytes || in->struct_size == kOptionsV2Bytes) {
+    std::memcpy(out, in, in->struct_size);
     out->struct_size = sizeof(b200fa_options);
-    out->capture = nullptr;
-    out->capture_bytes = 0;
   } else {
     return fail(B200FA_ERR_OPTIONS, "b200fa_options.struct_size mismatch");
   }
@@ -230,6 +234,16 @@ int check_capture(const b200fa_options& o, int64_t B, int64_t Hq, int64_t Nq, in
   if (o.capture == nullptr || (reinterpret_cast<uintptr_t>(o.capture) & 15u) != 0 || o.capture_bytes < need)
     return fail(B200FA_ERR_OPTIONS, "B200FA_FLAG_CAPTURE needs a 16-byte aligned buffer of at least %llu bytes",
                 (unsigned long long)need);
+  return B200FA_OK;
+}
+
+// Window checks (B200FA_FLAG_WINDOW).
+int check_window(const b200fa_options& o) {
+  if ((o.flags & B200FA_FLAG_WINDOW) == 0) return B200FA_OK;
+  if ((o.flags & B200FA_FLAG_CAUSAL) == 0 || (o.flags & B200FA_FLAG_CAPTURE) != 0)
+    return fail(B200FA_ERR_OPTIONS, "B200FA_FLAG_WINDOW needs B200FA_FLAG_CAUSAL and excludes B200FA_FLAG_CAPTURE");
+  if (o.window < 1 || o.sinks < 0)
+    return fail(B200FA_ERR_OPTIONS, "window must be at least 1 and sinks at least 0, got %d and %d", o.window, o.sinks);
   return B200FA_OK;
 }
 
@@ -261,6 +275,7 @@ int read_call_options(const b200fa_options* opts, int64_t B, int64_t Hq, int64_t
   int rc = read_options(opts, o_full);
   if (rc != B200FA_OK) return rc;
   if ((rc = check_capture(*o_full, B, Hq, Nq, Nk)) != B200FA_OK) return rc;
+  if ((rc = check_window(*o_full)) != B200FA_OK) return rc;
   *items = plan_count<int64_t>(ceil_div<int64_t>(Nq, kBlockM), unit_begin, unit_end);
   return B200FA_OK;
 }
@@ -292,12 +307,16 @@ int fill_params(const void* q, const void* k, const void* v, void* o, int64_t B,
   p->capture = (opts.flags & B200FA_FLAG_CAPTURE) ? opts.capture : nullptr;
   p->heads = int32_t(B * Hq);
   p->nq = int32_t(Nq);
+  if (opts.flags & B200FA_FLAG_WINDOW) {
+    p->window = opts.window;
+    p->sinks = opts.sinks < Nk ? opts.sinks : int32_t(Nk);
+  }
   return B200FA_OK;
 }
 
 int launch(int32_t variant, const FwdParams& p, int grid, void* stream, const char* where) {
-  kernel_for(variant, p.capture != nullptr, (p.flags & kFlagCausal) != 0)<<<grid, kThreads, kSmemBytes,
-                                                                          static_cast<cudaStream_t>(stream)>>>(p);
+  kernel_for(variant, p.capture != nullptr, (p.flags & kFlagCausal) != 0, (p.flags & kFlagWindow) != 0)
+      <<<grid, kThreads, kSmemBytes, static_cast<cudaStream_t>(stream)>>>(p);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, where);
   return B200FA_OK;

@@ -90,6 +90,14 @@
 #define B200FA_CAUSAL 0
 #endif
 
+// B200FA_WINDOW = 1 (with B200FA_CAUSAL = 1, b200fa_window.cu): row i attends
+// the causal keys of its window, i - window < j <= i, and the first `sinks`
+// keys.  A work item visits the key blocks that hold a sink, then those from
+// its first row's window to its last row's diagonal, and nothing between.
+#ifndef B200FA_WINDOW
+#define B200FA_WINDOW 0
+#endif
+
 namespace b200fa {
 
 constexpr int kBlockM = 128;    // query rows per unit (per CTA)
@@ -243,6 +251,7 @@ struct FwdParams {
   float* capture;           // capture kernels: [4][heads][n_kv][nq] + [heads][n_kv][nq][128] FP32
   int32_t heads;            // B * Hq
   int32_t nq;               // query rows per head
+  int32_t window, sinks;    // window kernels: keys behind a row that stay visible, first keys that always do
 };
 
 constexpr uint32_t kFlagTrace = 1u;
@@ -251,6 +260,7 @@ constexpr uint32_t kFlagTimeline = 4u;
 constexpr uint32_t kFlagCapture = 8u;
 constexpr uint32_t kFlagTestBounds = 16u;  // checking build: one planted out-of-range coordinate
 constexpr uint32_t kFlagCausal = 32u;      // causal mask (kernels of the causal translation unit)
+constexpr uint32_t kFlagWindow = 64u;      // sliding window and sinks (kernels of the window translation unit)
 
 // Checking build (B200FA_DEBUG): coordinates, indices and layout are
 // verified before use and the roles' block counts at exit; a violation is
@@ -357,7 +367,37 @@ __host__ __device__ inline void plan_decode(I nqb, I ub, I ue, I x, I& bh, I& qb
   cnt = left < G ? left : G;
 }
 
-#if B200FA_CAUSAL
+#if B200FA_WINDOW
+// The key blocks of a work item (query blocks qb .. qb+cnt-1) with a window:
+// block j of the item is key block j for j < sink, else j + skip.  At least
+// one, so that an item whose rows see no key (Nq > Nk, no sinks) still runs
+// the pipeline; its scores are then masked throughout.
+struct WindowBlocks {
+  int n, sink, skip;
+  __device__ __forceinline__ int key_block(int j) const { return j < sink ? j : j + skip; }
+};
+
+__device__ __forceinline__ WindowBlocks window_blocks(const FwdParams& p, int qb, int cnt) {
+  const int end = qb + cnt < p.n_kv ? qb + cnt : p.n_kv;  // past the last row's diagonal block
+  const int first_key = qb * kBlockM - p.window + 1;
+  const int first = first_key > 0 ? first_key / kBlockN : 0;
+  int sink = (p.sinks + kBlockN - 1) / kBlockN;
+  if (sink > end) sink = end;
+  if (sink > first) sink = first;
+  WindowBlocks b;
+  b.n = sink + (end > first ? end - first : 0);
+  b.sink = sink;
+  b.skip = first - sink;
+  if (b.n == 0) b = WindowBlocks{1, 1, 0};
+  return b;
+}
+
+__device__ __forceinline__ int item_blocks_causal(const FwdParams& p, int item) {
+  int bh, qb, cnt;
+  plan_decode<int>(p.nqb, p.unit_begin, p.unit_end, item, bh, qb, cnt);
+  return window_blocks(p, qb, cnt).n;
+}
+#elif B200FA_CAUSAL
 // Key blocks of work item `item` with the causal mask: up to the diagonal
 // block of the item's last unit.  Every role derives its block count, and
 // with it every barrier parity, from this function.
@@ -629,7 +669,10 @@ __device__ void load_role(const FwdParams& p, const Smem& sm, const Waiter& w, u
   for (int item = int(cluster_id_x()), it = 0; ok && item < p.num_items; item += int(num_clusters_x()), ++it) {
     int bh, qb, cnt;
     plan_decode<int>(p.nqb, p.unit_begin, p.unit_end, item, bh, qb, cnt);
-#if B200FA_CAUSAL
+#if B200FA_WINDOW
+    const WindowBlocks blocks = window_blocks(p, qb, cnt);
+    const int n = blocks.n;
+#elif B200FA_CAUSAL
     const int n = qb + cnt < p.n_kv ? qb + cnt : p.n_kv;  // this item's blocks (item_blocks_causal)
 #endif
     const int b = bh / p.Hq;
@@ -667,7 +710,12 @@ __device__ void load_role(const FwdParams& p, const Smem& sm, const Waiter& w, u
       tl.mark(9, j, 0);
       if (!w.wait(sm.bar(kBarKEmpty + int(e)), ph ^ 1u, site | (kBarKEmpty + e))) { ok = false; break; }
       tl.mark(9, j, 1);
-      const int krow = j * kBlockN + int(rank) * kKBoxRows;
+#if B200FA_WINDOW
+      const int kb = blocks.key_block(j);
+#else
+      const int kb = j;
+#endif
+      const int krow = kb * kBlockN + int(rank) * kKBoxRows;
       if (!w.check(krow >= 0 && krow + kKBoxRows <= key_end, site | (kCheckSite + 2u))) { ok = false; break; }
       mbar_arrive_expect_tx(sm.bar(kBarKFull + int(e)), kStageBytes);
       tma_load_3d(sm.k(e), &p.tm_k, sm.bar(kBarKFull + int(e)), 0, krow, kvh);
@@ -679,13 +727,13 @@ __device__ void load_role(const FwdParams& p, const Smem& sm, const Waiter& w, u
       tl.mark(9, j, 2);
       if (!w.wait(sm.bar(kBarVEmpty + int(e)), ph ^ 1u, site | (kBarVEmpty + e))) { ok = false; break; }
       tl.mark(9, j, 3);
-      if (!w.check(j * kBlockN + kBlockN <= key_end && int(rank) * kPairDims + kPairDims <= kHeadDim,
+      if (!w.check(kb * kBlockN + kBlockN <= key_end && int(rank) * kPairDims + kPairDims <= kHeadDim,
                    site | (kCheckSite + 3u))) {
         ok = false;
         break;
       }
       mbar_arrive_expect_tx(sm.bar(kBarVFull + int(e)), kStageBytes);
-      tma_load_3d(sm.v(e), &p.tm_v, sm.bar(kBarVFull + int(e)), int(rank) * kPairDims, j * kBlockN, kvh);
+      tma_load_3d(sm.v(e), &p.tm_v, sm.bar(kBarVFull + int(e)), int(rank) * kPairDims, kb * kBlockN, kvh);
       issued |= 1u << (kRing + e);
       last_par = (last_par & ~(1u << (kRing + e))) | (ph << (kRing + e));
     }
@@ -777,6 +825,36 @@ __device__ __forceinline__ void mask_keys64(uint32_t* r, int first, int valid) {
     if (first + i >= valid) r[i] = __float_as_uint(-INFINITY);
 }
 
+#if B200FA_WINDOW
+// Bits 0 .. x-1 of a word (none for x <= 0, all for x >= 32).
+__device__ __forceinline__ uint32_t bits_below(int x) {
+  return x <= 0 ? 0u : x >= 32 ? 0xffffffffu : (1u << x) - 1u;
+}
+
+// Masks this thread's row of a block's scores in tensor memory, before the
+// softmax loads it: key c stays when c < valid and (c >= lo or c < sink), the
+// others get -inf (one bit of a word per 32 keys rather than three comparisons
+// a key).  In place and ahead of the load, so that blocks no row of the warp
+// masks -- most -- run the same instructions as the kernel without a mask:
+// with the selects on the loaded registers a block took 1.6 us instead of 0.95
+// (B=4, Hq=32, N=8192), masked or not.
+__device__ __forceinline__ void mask_window(uint32_t tS, int valid, int lo, int sink) {
+#pragma unroll 1
+  for (int c0 = 0; c0 < kBlockN; c0 += 32) {
+    const uint32_t keep = bits_below(valid - c0) & (~bits_below(lo - c0) | bits_below(sink - c0));
+    if (__all_sync(0xffffffffu, keep == 0xffffffffu)) continue;
+    uint32_t s[32];
+    tmem_ld32(tS + uint32_t(c0), s);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if ((keep & (1u << i)) == 0u) s[i] = __float_as_uint(-INFINITY);
+    tmem_st32(tS + uint32_t(c0), s);
+  }
+  tmem_wait_st();
+}
+#endif
+
 // O row of this thread (128 FP32 columns in TMEM) times `f`, in place.
 __device__ __forceinline__ void scale_o_row(uint32_t tO, float f) {
 #pragma unroll 1
@@ -834,6 +912,14 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
 #if B200FA_CAUSAL
   uint32_t g_items = 0;      // the CTA's key blocks of all earlier items
 #endif
+#if B200FA_WINDOW
+  // A row may see no key of its item's first blocks: its reference starts at
+  // a finite floor (x = -inf - floor stays -inf, P = 0) and the first block
+  // with a visible key moves it, scaling the zeros gathered so far by 0.
+  constexpr float kFirstRef = -1e30f;
+#else
+  constexpr float kFirstRef = -INFINITY;
+#endif
 
   for (int item = int(cluster_id_x()), it = 0; ok && item < p.num_items; item += int(num_clusters_x()), ++it) {
 #if B200FA_CAUSAL
@@ -843,10 +929,16 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
     // This thread's query row (rank r holds unit r of the item; a one-unit
     // item repeats it in rank 1): the mask's bound.
     int qrow_g;
+#if B200FA_WINDOW
+    WindowBlocks blocks;
+#endif
     {
       int bh_i, qb_i, cnt_i;
       plan_decode<int>(p.nqb, p.unit_begin, p.unit_end, item, bh_i, qb_i, cnt_i);
       qrow_g = (qb_i + (int(rank) < cnt_i ? int(rank) : cnt_i - 1)) * kBlockM + row;
+#if B200FA_WINDOW
+      blocks = window_blocks(p, qb_i, cnt_i);
+#endif
     }
 #else
     const uint32_t g0 = uint32_t(it) * uint32_t(n);  // the CTA's block count before this item
@@ -898,7 +990,7 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
       const uint32_t b = buf(gb);
       const uint32_t tS = tmem_base + lane_off + kTmemS + 128u * b;
       const uint32_t tP = tmem_base + lane_off + kTmemP + 64u * b;
-      float m_prev = -INFINITY;
+      float m_prev = kFirstRef;
       tl.mark(int(warp), j, 0);
       if (!wait_warp(kBarSFull + int(b), buf_parity(gb))) {
         ok = false;
@@ -906,7 +998,17 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
       }
       tl.mark(int(warp), j, 7);
       tc_fence_after();
-#if B200FA_CAUSAL
+#if B200FA_WINDOW
+      // Keys of the block that this row sees: c < valid (the end of the keys,
+      // the diagonal) and c >= lo (its window) or c < sink.
+      const int kb = blocks.key_block(j);
+      const int ahead = qrow_g - kb * kBlockN;
+      int valid = kb == p.n_kv - 1 ? p.nk_tail : kBlockN;
+      if (ahead + 1 < valid) valid = ahead + 1;
+      const int lo = ahead - p.window + 1;
+      const int sink = p.sinks - kb * kBlockN;
+      if (__any_sync(0xffffffffu, valid < kBlockN || (lo > 0 && sink < lo))) mask_window(tS, valid, lo, sink);
+#elif B200FA_CAUSAL
       // Valid keys of the block for this row: the last block's key count
       // and the keys up to the row.
       int valid = j == p.n_kv - 1 ? p.nk_tail : kBlockN;
@@ -940,6 +1042,7 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
       }
       tl.mark(int(warp), j, 1);
       tmem_wait_ld();
+#if !B200FA_WINDOW
       if (tail) {
 #if B200FA_CAUSAL
         mask_keys64(r, 0, valid);
@@ -949,6 +1052,7 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
         mask_keys64(r + 64, 64, p.nk_tail);
 #endif
       }
+#endif
       arrive_rank0(kBarSFree + int(b));  // the S issuer may refill the buffer
       const float mx = fmaxf(row_max64(r), row_max64(r + 64)) * sl2;
       tl.mark(int(warp), j, 2);
@@ -1060,7 +1164,11 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
     arrive_local(kBarXchg);
     if (!wait_warp(kBarXchg, 1u)) { ok = false; break; }
     const float l = l_g + ld_shared_f32(sm.xchg(mine ^ 1u, row));
+#if B200FA_WINDOW
+    const float inv_l = l > 0.f ? 1.f / l : 0.f;  // a row that sees no key: zeros
+#else
     const float inv_l = 1.f / l;
+#endif
 #pragma unroll 1
     for (int c = 0; c < 2; ++c) {
       uint32_t o[32];

@@ -26,6 +26,7 @@ FLAG_TIMELINE = 4
 FLAG_CAPTURE = 8
 FLAG_TEST_BOUNDS = 16
 FLAG_CAUSAL = 32
+FLAG_WINDOW = 64
 BLOCK_KEYS = 128
 
 DEV_OK = 0
@@ -51,7 +52,8 @@ _i64, _i32, _u32, _u64, _p, _f = C.c_int64, C.c_int32, C.c_uint32, C.c_uint64, C
 class Options(C.Structure):
     _fields_ = [("struct_size", C.c_uint32), ("flags", C.c_uint32),
                 ("timeout_us", C.c_uint32), ("max_ctas", C.c_int32),
-                ("capture", C.c_void_p), ("capture_bytes", C.c_uint64)]
+                ("capture", C.c_void_p), ("capture_bytes", C.c_uint64),
+                ("window", C.c_int32), ("sinks", C.c_int32)]
 
 
 SIGNATURES = {
@@ -161,10 +163,10 @@ def kernel_name(variant: int) -> str:
 
 def fwd(q_ptr, k_ptr, v_ptr, o_ptr, B, Hq, Hkv, Nq, Nk, D, scale, variant,
         unit_begin, unit_end, ws_ptr, ws_bytes, stream, *, flags=0, timeout_us=0, max_ctas=0,
-        capture_ptr=None, capture_bytes=0, debug=False):
+        capture_ptr=None, capture_bytes=0, window=0, sinks=0, debug=False):
     """Raw pointer call of b200fa_fwd_ex (``debug``: of the checking build);
     raises B200FAError on a nonzero status."""
-    opts = Options(C.sizeof(Options), flags, timeout_us, max_ctas, capture_ptr, capture_bytes)
+    opts = Options(C.sizeof(Options), flags, timeout_us, max_ctas, capture_ptr, capture_bytes, window, sinks)
     status = load(debug=debug).b200fa_fwd_ex(q_ptr, k_ptr, v_ptr, o_ptr, B, Hq, Hkv, Nq, Nk, D, scale, variant,
                                              unit_begin, unit_end, ws_ptr, ws_bytes, stream, C.byref(opts))
     check(status, "b200fa_fwd", debug)

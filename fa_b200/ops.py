@@ -45,6 +45,17 @@ def _geometry(q, k, v):
     return b, h, k.shape[1], nq, nk
 
 
+def _window(window, sinks, causal) -> tuple[int, int]:
+    """Checked (window, sinks) of a call; window 0 = none."""
+    if window is None or sinks is None or int(window) < 0 or int(sinks) < 0:
+        raise ValueError("window and sinks must be at least 0")
+    if window and not causal:
+        raise ValueError("window needs causal=True")
+    if sinks and not window:
+        raise ValueError("sinks need a window")
+    return min(int(window), 2**31 - 1), min(int(sinks), 2**31 - 1)
+
+
 class Operator:
     """``op(q, k, v) -> O``: non-causal GQA attention forward, FP16 in/out.
 
@@ -83,14 +94,21 @@ class Operator:
 
     def __call__(self, q, k, v, *, scale: float | None = None, out: torch.Tensor | None = None,
                  unit_range: tuple[int, int] | None = None, flags: int = 0,
-                 capture: torch.Tensor | None = None, causal: bool = False) -> torch.Tensor:
+                 capture: torch.Tensor | None = None, causal: bool = False, window: int = 0,
+                 sinks: int = 0) -> torch.Tensor:
         """O = softmax(Q K^T * scale) V.  ``causal``: query row i attends keys
         0..i only (top-left aligned, as torch's ``is_causal``; an addition,
-        the reference's operator is non-causal).  ``capture`` (FP32, at least
+        the reference's operator is non-causal).  ``window`` > 0 (with
+        ``causal``): only keys i - window < j <= i of those, and the first
+        ``sinks`` keys; a row that sees no key (Nq > Nk) gets zeros, and key
+        blocks that no row of a work item sees are not read.  ``capture`` (FP32, at least
         ``capture_bytes(...)`` bytes, on Q's device) turns on the debug
         capture of the per-block online-softmax state (``capture_view``)."""
         if causal:
             flags |= lib.FLAG_CAUSAL
+        window, sinks = _window(window, sinks, causal)
+        if window:
+            flags |= lib.FLAG_WINDOW
         B, Hq, Hkv, Nq, Nk = _geometry(q, k, v)
         if out is None:
             out = torch.empty_like(q)
@@ -112,12 +130,13 @@ class Operator:
                     B, Hq, Hkv, Nq, Nk, HEAD_DIM, scale, self.variant_id, begin, end,
                     ws.data_ptr(), ws.numel(), stream,
                     flags=self.flags | flags | cap_flag, timeout_us=self.timeout_us, max_ctas=self.max_ctas,
-                    capture_ptr=cap_ptr, capture_bytes=cap_bytes, debug=self.debug)
+                    capture_ptr=cap_ptr, capture_bytes=cap_bytes, window=window, sinks=sinks, debug=self.debug)
         return out
 
     def forward_host(self, q_host, k_host, v_host, out_host, *, q_dev, k_dev, v_dev, o_dev,
                      scale: float | None = None, unit_range: tuple[int, int] | None = None,
-                     chunks: int = 3, causal: bool = False) -> tuple[int, int]:
+                     chunks: int = 3, causal: bool = False, window: int = 0,
+                     sinks: int = 0) -> tuple[int, int]:
         """O = attention(Q, K, V) from pinned host buffers into a pinned host
         buffer, with the copies overlapped with the kernel.
 
@@ -132,7 +151,7 @@ class Operator:
         ``out_host`` hold either the full Q/O or only the unit range's rows
         (flattened to [rows, 128]).  Work is enqueued on the current stream,
         which also waits for the last download: synchronize it to read
-        ``out_host``.  Returns the (host-to-device, device-to-host) bytes.
+        ``out_host``.  ``causal``, ``window`` and ``sinks`` as in the call.  Returns the (host-to-device, device-to-host) bytes.
         """
         B, Hq, Hkv, Nq, Nk = _geometry(q_dev, k_dev, v_dev)
         units = num_units(B, Hq, Nq)
@@ -184,7 +203,8 @@ class Operator:
                 ev_q.append(s_in.record_event())
         for c in range(n):
             cur.wait_event(ev_q[c])
-            self(q_dev, k_dev, v_dev, scale=scale, out=o_dev, unit_range=(bounds[c], bounds[c + 1]), causal=causal)
+            self(q_dev, k_dev, v_dev, scale=scale, out=o_dev, unit_range=(bounds[c], bounds[c + 1]),
+                 causal=causal, window=window, sinks=sinks)
             s_out.wait_stream(cur)
             r0, r1 = row_range(bounds[c], bounds[c + 1], Nq)
             with torch.cuda.stream(s_out):

@@ -123,11 +123,17 @@ extern "C" {
  * Runs separate kernels (b200_fa_fp{16,32}_causal_kernel); not combined
  * with B200FA_FLAG_CAPTURE (B200FA_ERR_OPTIONS). */
 #define B200FA_FLAG_CAUSAL        32u
+/* Sliding window with sinks, on top of B200FA_FLAG_CAUSAL (required): query
+ * row i attends keys i - window < j <= i and the first `sinks` keys j <= i
+ * (b200fa_options.window >= 1, .sinks >= 0).  A row that sees no key (Nq > Nk)
+ * gets zeros.  Key blocks that no row of a work item sees are not read.
+ * Runs separate kernels (b200_fa_fp{16,32}_window_kernel). */
+#define B200FA_FLAG_WINDOW        64u
 #define B200FA_BLOCK_KEYS        128
 
 typedef struct b200fa_options {
     uint32_t struct_size;   /* sizeof(b200fa_options); 16 (no capture fields)
-                               is accepted too                               */
+                               and 32 (no window fields) are accepted too    */
     uint32_t flags;         /* B200FA_FLAG_*                                  */
     uint32_t timeout_us;    /* bound of every device-side wait; 0 = 2 s       */
     int32_t  max_ctas;      /* cap on the persistent grid (CTAs; rounded down
@@ -135,6 +141,8 @@ typedef struct b200fa_options {
                                pair per TPC                                  */
     float*   capture;       /* B200FA_FLAG_CAPTURE: device buffer             */
     uint64_t capture_bytes; /* its size, >= b200fa_capture_bytes(...)        */
+    int32_t  window;        /* B200FA_FLAG_WINDOW: keys of the window, >= 1   */
+    int32_t  sinks;         /* B200FA_FLAG_WINDOW: first keys always visible  */
 } b200fa_options;
 
 /* Workspace layout (bytes, 256-B aligned, zeroed once by the owner):
