@@ -9,7 +9,6 @@
 //   * PartitionContiguous (cce_task.h:28-35) -> b200fa_partition.
 #include <cuda.h>
 #include <cuda_runtime.h>
-#include <cudaTypedefs.h>
 
 #include <cmath>
 #include <cstdarg>
@@ -19,6 +18,7 @@
 
 #include "b200fa.h"
 #include "fa_kernel.cuh"
+#include "host.h"
 
 using namespace b200fa;
 
@@ -93,6 +93,12 @@ namespace {
 
 thread_local char g_last_error[512] = "";
 
+}  // namespace
+
+namespace b200fa {
+
+void clear_error() { g_last_error[0] = '\0'; }
+
 int fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
@@ -104,8 +110,6 @@ int fail(int code, const char* fmt, ...) {
 int cuda_fail(cudaError_t e, const char* where) {
   return fail(static_cast<int>(e), "%s: %s (%s)", where, cudaGetErrorName(e), cudaGetErrorString(e));
 }
-
-constexpr int64_t kMax31 = (int64_t(1) << 31) - 1;
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static std::once_flag once;
@@ -120,6 +124,12 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   });
   return fn;
 }
+
+}  // namespace b200fa
+
+namespace {
+
+constexpr int64_t kMax31 = (int64_t(1) << 31) - 1;
 
 // Per-device facts read once: kernel attributes set, and how many CTA pairs
 // can be resident at once (one per TPC whose two SMs are both available).

@@ -1,0 +1,259 @@
+// paged.h -- attention over a paged cache: what its kernels share.  The
+// parameters, how the work is cut, and how partial results are joined.
+//
+// Rows.  The `group` query heads of one key/value head read the same keys, so
+// a work item takes them together: `tokens_per_tile` consecutive new tokens
+// of a request times the group, row = token * group + head in the tile.
+//
+// Work.  The key blocks (128 keys) of every item -- request, key/value head,
+// tile, in that order -- form one line, and worker w of n takes the stretch
+// [total w / n, total (w + 1) / n) of it: every worker has the same number of
+// blocks whatever the lengths, a long context is split over many workers when
+// there are few rows, and nothing but cu_q and kv_lens (on the device) is
+// needed to find one's place.  An item that a worker's end cuts leaves
+// partial results, per row the unnormalised output relative to its maximum,
+// the maximum (log2 domain) and the sum; worker w keeps at most two: slot 2w
+// for an item begun before its stretch, slot 2w + 1 for one that begins in it
+// and goes on after it.  The worker an item begins in leaves a record of it,
+// from which combine_partials joins the parts in worker order, so the same
+// lengths always give the same bits.
+//
+// Keys.  The row at position p sees keys j <= p, with a window only
+// j > p - window or j < sinks; an item visits the blocks that hold a visible
+// sink, then those from its first row's window to its last row's position.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace b200fa {
+
+constexpr int kPagedBlock = 128;  // keys per block
+constexpr uint32_t kDevPage = 4u;
+constexpr uint32_t kPagedHeader = 256;  // status words
+constexpr int kMaxWorkers = 512;
+constexpr uint32_t kPagedRecord = 32;   // bytes of a worker's record
+constexpr uint32_t kPagedPartials = kPagedHeader + kMaxWorkers * kPagedRecord;  // offset of the partial results
+
+struct PagedParams {
+  CUtensorMap tm_k, tm_v;   // (128, page_size, heads_kv, num_pages), box (64, min(page_size, 128), 1, 1)
+  CUtensorMap tm_q;         // chunk kernel: (128, group, heads_kv, tokens), box (64, group, 1, tokens_per_tile / 2)
+  const void* q;
+  void* o;
+  int64_t q_tok, q_head, o_tok, o_head;  // elements
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* kv_lens;
+  const int32_t* cu_q;
+  int32_t requests, width, page_shift, num_pages;
+  int32_t tokens, heads_kv, group;
+  int32_t tokens_per_tile;
+  int32_t window, sinks;
+  float scale_log2;
+  int32_t workers;
+  int32_t part_rows;        // rows of a partial result
+  uint64_t timeout_ns;
+  uint8_t* ws;
+};
+
+struct PagedRequest {
+  int q0, len;     // its rows of q
+  int kv;          // its keys
+  __device__ __forceinline__ int tiles(const PagedParams& p) const {
+    return (len + p.tokens_per_tile - 1) / p.tokens_per_tile;
+  }
+};
+
+// Lengths as the kernels use them: rows inside q, keys inside the table, so
+// that a malformed length cannot lead outside a tensor.
+__device__ __forceinline__ PagedRequest paged_request(const PagedParams& p, int r) {
+  int a = p.cu_q[r], b = p.cu_q[r + 1];
+  a = a < 0 ? 0 : a > p.tokens ? p.tokens : a;
+  b = b < a ? a : b > p.tokens ? p.tokens : b;
+  const int64_t most = int64_t(p.width) << p.page_shift;
+  int kv = p.kv_lens[r];
+  kv = kv < 0 ? 0 : kv > most ? int(most) : kv;
+  return PagedRequest{a, b - a, kv};
+}
+
+// The key blocks of a tile: block j is key block j for j < sink, else
+// j + skip.  At least one, so that a tile whose rows see nothing still
+// writes its zeros.  Pages are loaded that hold a key of [first_key, end_key)
+// or, below end_key, a sink.
+struct PagedBlocks {
+  int n, sink, skip;
+  int pos0;        // position of the tile's first row (may be negative)
+  int first_key;   // first key of the first row's window
+  int end_key;     // past the position of the last row
+  __device__ __forceinline__ int key_block(int j) const { return j < sink ? j : j + skip; }
+};
+
+__device__ __forceinline__ PagedBlocks paged_blocks(const PagedParams& p, const PagedRequest& q, int tile) {
+  const int t0 = tile * p.tokens_per_tile;
+  const int left = q.len - t0;
+  const int pos0 = q.kv - q.len + t0;
+  const int pos1 = pos0 + (left < p.tokens_per_tile ? left : p.tokens_per_tile) - 1;
+  const int end = pos1 >= 0 ? pos1 / kPagedBlock + 1 : 0;
+  PagedBlocks b;
+  b.pos0 = pos0;
+  b.end_key = pos1 >= 0 ? pos1 + 1 : 0;
+  b.first_key = 0;
+  b.sink = 0;
+  int first = 0;
+  if (p.window > 0) {
+    b.first_key = pos0 > p.window - 1 ? pos0 - (p.window - 1) : 0;
+    first = b.first_key / kPagedBlock;
+    int s = p.sinks / kPagedBlock + (p.sinks % kPagedBlock != 0);
+    if (s > end) s = end;
+    b.sink = s < first ? s : first;
+  }
+  b.n = b.sink + (end > first ? end - first : 0);
+  b.skip = first - b.sink;
+  if (b.n == 0) b.n = 1, b.sink = 1, b.skip = 0;
+  return b;
+}
+
+__device__ __forceinline__ int64_t request_blocks(const PagedParams& p, int r) {
+  const PagedRequest q = paged_request(p, r);
+  const int tiles = q.tiles(p);
+  int64_t n = 0;
+  for (int t = 0; t < tiles; ++t) n += paged_blocks(p, q, t).n;
+  return n * p.heads_kv;
+}
+
+// A worker's place in the line of blocks.
+struct PagedStart {
+  int r, h, tile, off;   // first item and the block of it to begin with
+  int64_t count;         // blocks of the stretch
+  int64_t total;         // blocks of all
+  int workers;           // stretches they are cut into: no more than blocks
+};
+
+__device__ __forceinline__ int64_t stretch_begin(int64_t total, int w, int n) { return total / n * w + total % n * w / n; }
+
+// The same for every worker; all threads of the block call it.  `scratch`:
+// blockDim.x / 32 + 1 shared int64; `start`: shared.
+__device__ __forceinline__ void find_start(const PagedParams& p, int worker, int64_t* scratch, PagedStart* start) {
+  const int tid = int(threadIdx.x), nt = int(blockDim.x), warps = nt / 32;
+  const int per = (p.requests + nt - 1) / nt;
+  const int r0 = min(p.requests, tid * per), r1 = min(p.requests, r0 + per);
+  int64_t sum = 0;
+  for (int r = r0; r < r1; ++r) sum += request_blocks(p, r);
+  int64_t inc = sum;
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t a = __shfl_up_sync(0xffffffffu, inc, d);
+    if ((tid & 31) >= d) inc += a;
+  }
+  if ((tid & 31) == 31) scratch[tid >> 5] = inc;
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < warps; ++w) {
+    if (w < (tid >> 5)) inc += scratch[w];
+    total += scratch[w];
+  }
+  const int workers = total < p.workers ? int(total) : p.workers;
+  int64_t begin = 0, end = 0;
+  if (worker < workers) begin = stretch_begin(total, worker, workers), end = stretch_begin(total, worker + 1, workers);
+  int64_t at = inc - sum;
+  if (tid == 0) *start = PagedStart{0, 0, 0, 0, end - begin, total, workers};
+  __syncthreads();
+  if (end > begin && at <= begin && begin < inc) {
+    for (int r = r0; r < r1; ++r) {
+      const int64_t n = request_blocks(p, r);
+      if (begin >= at + n) {
+        at += n;
+        continue;
+      }
+      const int64_t head = n / p.heads_kv, x = begin - at;
+      const PagedRequest q = paged_request(p, r);
+      int64_t left = x % head;
+      int t = 0;
+      for (int b; left >= (b = paged_blocks(p, q, t).n); ++t) left -= b;
+      start->r = r;
+      start->h = int(x / head);
+      start->tile = t;
+      start->off = int(left);
+      break;
+    }
+  }
+  __syncthreads();
+}
+
+// Walks a worker's items; every role of a kernel walks the same ones.
+struct PagedWalk {
+  int r, h, tile, off;
+  int64_t left;
+  PagedRequest req;
+  PagedBlocks blocks;
+  int take;  // blocks of the current item in this stretch, from block `off` on
+
+  __device__ __forceinline__ PagedWalk(const PagedParams& p, const PagedStart& s)
+      : r(s.r), h(s.h), tile(s.tile), off(s.off), left(s.count) {
+    if (left > 0) load(p);
+  }
+  __device__ __forceinline__ bool more() const { return left > 0; }
+  __device__ __forceinline__ void load(const PagedParams& p) {
+    req = paged_request(p, r);
+    set(p);
+  }
+  __device__ __forceinline__ void set(const PagedParams& p) {
+    blocks = paged_blocks(p, req, tile);
+    const int n = blocks.n - off;
+    take = n < left ? n : int(left);
+  }
+  __device__ __forceinline__ bool begins() const { return off == 0; }
+  __device__ __forceinline__ bool ends() const { return off + take == blocks.n; }
+  __device__ __forceinline__ void next(const PagedParams& p) {
+    left -= take;
+    off = 0;
+    if (left <= 0) return;
+    if (++tile == req.tiles(p)) {
+      tile = 0;
+      if (++h == p.heads_kv) {
+        h = 0;
+        do req = paged_request(p, ++r);
+        while (req.len == 0 && r + 1 < p.requests);
+      }
+    }
+    set(p);
+  }
+};
+
+// The record of an item that begins in a worker's stretch and ends in another's.
+struct PagedRecord {
+  int32_t parts;   // stretches the item covers; 0: the worker has no such item
+  int32_t row0;    // its first token in q
+  int32_t tokens;  // tokens of the tile
+  int32_t h;
+  int32_t spare[4];
+};
+static_assert(sizeof(PagedRecord) == kPagedRecord, "record size");
+
+__device__ __forceinline__ PagedRecord* paged_record(const PagedParams& p, int worker) {
+  return reinterpret_cast<PagedRecord*>(p.ws + kPagedHeader) + worker;
+}
+
+// Partial slot s: [rows][128] outputs, then [rows] maxima, then [rows] sums.
+__device__ __forceinline__ float* paged_partial(const PagedParams& p, int slot) {
+  return reinterpret_cast<float*>(p.ws + kPagedPartials) + size_t(slot) * size_t(p.part_rows) * 130u;
+}
+
+// Stretches covered by an item that begins in `worker` and has `rest` blocks
+// behind that worker's end.
+__device__ __forceinline__ int paged_parts(const PagedStart& s, int worker, int64_t rest) {
+  const int64_t end = stretch_begin(s.total, worker + 1, s.workers) + rest;
+  int w = worker + 1;
+  while (w < s.workers && stretch_begin(s.total, w, s.workers) < end) ++w;
+  return w - worker;
+}
+
+__device__ __forceinline__ void paged_status(const PagedParams& p, uint32_t code, uint32_t site) {
+  uint32_t* ws = reinterpret_cast<uint32_t*>(p.ws);
+  if (atomicCAS(&ws[0], 0u, code) == 0u) {
+    ws[1] = site;
+    ws[2] = blockIdx.x;
+  }
+}
+
+}  // namespace b200fa

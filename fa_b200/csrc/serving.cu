@@ -1,0 +1,432 @@
+// serving.cu -- the light kernels of a serving step: page tables from request
+// lengths, rotary positions, and the cache append (rotary included).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "b200fa.h"
+#include "host.h"
+
+namespace b200fa {
+namespace {
+
+constexpr int64_t kInt32Max = (int64_t(1) << 31) - 1;
+
+// ------------------------------------------------------------ page tables
+// Latency-bound: a few KB in, 12 bytes per token out.  Every block scans all
+// requests (two prefix sums in shared memory, <= 32 KB) instead of waiting for
+// another block's scan, so one launch without any grid-wide step does it; the
+// token and page loops are then split over the blocks.
+constexpr int kTableThreads = 256;
+
+struct TableParams {
+  const int32_t* ctx;
+  const int32_t* add;
+  int32_t* table;
+  int64_t table_stride;
+  const int32_t* free_pages;
+  const int32_t* free_count;
+  int64_t* slots;
+  int32_t* positions;
+  int32_t* cu_q;
+  int32_t* kv_lens;
+  int32_t* free_left;
+  int32_t* status;
+  int64_t num_tokens, free_capacity;
+  int32_t requests, width, shift;
+};
+
+__device__ __forceinline__ int64_t length(int32_t x) { return x > 0 ? x : 0; }
+
+// Last index r of the non-decreasing prefix sums cum[0..n] with cum[r] <= x;
+// x < cum[n].
+__device__ __forceinline__ int owner(const int32_t* cum, int n, int32_t x) {
+  int lo = 0, hi = n;  // cum[lo] <= x < cum[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cum[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kTableThreads) b200_build_tables_kernel(const TableParams p) {
+  extern __shared__ int32_t sm[];
+  const int R = p.requests, tid = int(threadIdx.x);
+  int32_t* cum_tok = sm;            // [R + 1]
+  int32_t* cum_page = sm + R + 1;   // [R + 1]
+  __shared__ int64_t warp_tok[kTableThreads / 32], warp_page[kTableThreads / 32];
+  const int64_t mask = (int64_t(1) << p.shift) - 1;
+  auto pages = [&](int64_t n) { return (n + mask) >> p.shift; };
+
+  // Each thread sums a run of requests; warp and block scans give its offset.
+  const int per = (R + kTableThreads - 1) / kTableThreads;
+  const int r0 = min(R, tid * per), r1 = min(R, r0 + per);
+  int64_t tok = 0, page = 0;
+  int wide = 0;
+  for (int r = r0; r < r1; ++r) {
+    const int64_t c = length(p.ctx[r]), n = length(p.add[r]);
+    tok += n;
+    page += pages(c + n) - pages(c);
+    wide |= pages(c + n) > p.width;
+  }
+  int64_t it = tok, ip = page;
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t a = __shfl_up_sync(0xffffffffu, it, d), b = __shfl_up_sync(0xffffffffu, ip, d);
+    if ((tid & 31) >= d) it += a, ip += b;
+  }
+  if ((tid & 31) == 31) warp_tok[tid >> 5] = it, warp_page[tid >> 5] = ip;
+  wide = __syncthreads_or(wide);
+  int64_t total_tok = 0, total_page = 0;
+  for (int w = 0; w < kTableThreads / 32; ++w) {
+    if (w < (tid >> 5)) it += warp_tok[w], ip += warp_page[w];
+    total_tok += warp_tok[w];
+    total_page += warp_page[w];
+  }
+  it -= tok;
+  ip -= page;
+  for (int r = r0; r < r1; ++r) {
+    cum_tok[r] = int32_t(min(it, kInt32Max));
+    cum_page[r] = int32_t(min(ip, kInt32Max));
+    const int64_t c = length(p.ctx[r]), n = length(p.add[r]);
+    it += n;
+    ip += pages(c + n) - pages(c);
+  }
+  if (tid == 0) {
+    cum_tok[R] = int32_t(min(total_tok, kInt32Max));
+    cum_page[R] = int32_t(min(total_page, kInt32Max));
+  }
+  const int64_t have = min(length(*p.free_count), p.free_capacity);
+  const int status = total_tok > p.num_tokens ? 3 : wide ? 2 : total_page > have ? 1 : 0;
+  __syncthreads();
+
+  const int64_t first = int64_t(blockIdx.x) * kTableThreads + tid;
+  const int64_t step = int64_t(gridDim.x) * kTableThreads;
+  const int64_t known = min(total_tok, p.num_tokens);
+  for (int64_t t = first; t < p.num_tokens; t += step) {
+    int64_t slot = -1;
+    int32_t pos = 0;
+    if (t < known) {
+      const int r = owner(cum_tok, R, int32_t(t));
+      const int64_t c = length(p.ctx[r]), at = c + (t - cum_tok[r]);
+      pos = int32_t(at);
+      if (status == 0) {
+        const int64_t held = pages(c), i = at >> p.shift;
+        const int32_t pg = i < held ? p.table[r * p.table_stride + i]
+                                    : p.free_pages[have - 1 - (cum_page[r] + (i - held))];
+        if (pg >= 0) slot = (int64_t(pg) << p.shift) + (at & mask);
+      }
+    }
+    p.slots[t] = slot;
+    p.positions[t] = pos;
+  }
+  if (status == 0) {
+    for (int64_t i = first; i < total_page; i += step) {
+      const int r = owner(cum_page, R, int32_t(i));
+      p.table[r * p.table_stride + pages(length(p.ctx[r])) + (i - cum_page[r])] = p.free_pages[have - 1 - i];
+    }
+  }
+  for (int64_t r = first; r <= R; r += step) {
+    p.cu_q[r] = cum_tok[r];
+    if (r < R) p.kv_lens[r] = int32_t(length(p.ctx[r]) + (status == 0 ? length(p.add[r]) : 0));
+  }
+  if (first == 0) {
+    *p.free_left = int32_t(status == 0 ? have - total_page : length(*p.free_count));
+    *p.status = status;
+  }
+}
+
+// ------------------------------------------------- rotary and cache append
+// Bound by memory: every element is read and written once.  Sixteen elements
+// of a row -- eight pairs -- belong to one thread, which computes their eight
+// angles once and applies them to `heads_per_thread` heads of its token, so
+// that the sines cost a fraction of the loads they run under.
+//
+// The angle: position times frequency in turns as a 64-bit binary fraction,
+// reduced mod 1 by the integer product's wrap-around.  It is exact whatever
+// the position, where a 32-bit product of position and frequency is off by
+// position * 2^-24 radians (0.008 at 131072).
+struct Segment {  // a run of heads: rows [batch][n][heads][dim] -> the same, or the cache
+  const void* src;
+  void* dst;
+  int64_t src_b, src_n, src_h;
+  int64_t dst_b, dst_n, dst_h;  // scattered: page, token, head
+  int32_t heads;
+  int32_t rotate, scatter;
+};
+
+struct RotaryParams {
+  Segment seg[3];
+  int32_t segments, heads;   // heads of all segments
+  int64_t n, tokens;         // tokens = batch * n
+  const void* positions;
+  int32_t pos_bits;
+  int64_t pos_stride;
+  const uint64_t* freq;
+  int32_t lanes;             // threads per row: dim / 16
+  int32_t rot;
+  float magnitude, sign;
+  const int64_t* slots;
+  int64_t num_slots;
+  int32_t shift;
+  int32_t heads_per_thread, head_chunks;
+};
+
+template <typename T>
+struct Sixteen {  // 16 elements as 16-byte pieces
+  static constexpr int kPer = 16 / int(sizeof(T));   // elements of a piece
+  static constexpr int kPieces = 16 / kPer;
+  uint4 v[kPieces];
+};
+
+__device__ __forceinline__ void to_float(float x, float& o) { o = x; }
+__device__ __forceinline__ void to_float(__half x, float& o) { o = __half2float(x); }
+__device__ __forceinline__ void to_float(__nv_bfloat16 x, float& o) { o = __bfloat162float(x); }
+__device__ __forceinline__ void from_float(float x, float& o) { o = x; }
+__device__ __forceinline__ void from_float(float x, __half& o) { o = __float2half_rn(x); }
+__device__ __forceinline__ void from_float(float x, __nv_bfloat16& o) { o = __float2bfloat16_rn(x); }
+
+// kLayout 0: the thread's pairs are elements (8 c + i, rot/2 + 8 c + i); 1:
+// (16 c + 2 i, 16 c + 2 i + 1).  Lanes at or behind rot copy elements 16 c ...
+template <typename T, int kLayout>
+__global__ void __launch_bounds__(256) b200_rotary_kernel(const RotaryParams p) {
+  constexpr int kPer = Sixteen<T>::kPer, kPieces = Sixteen<T>::kPieces;
+  const int64_t id = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int c = int(id % p.lanes);
+  const int64_t rest = id / p.lanes;
+  const int chunk = int(rest % p.head_chunks);
+  const int64_t token = rest / p.head_chunks;
+  if (token >= p.tokens) return;
+  const int64_t b = token / p.n, n = token - b * p.n;
+
+  const bool turn = 16 * c < p.rot;
+  float cs[8], sn[8];
+  bool have_angles = false;
+  // Element offset of the thread's first and second eight elements.
+  const int lo = (turn && kLayout == 0) ? 8 * c : 16 * c;
+  const int hi = (turn && kLayout == 0) ? p.rot / 2 + 8 * c : 16 * c + 8;
+
+  const int h1 = min(p.heads, (chunk + 1) * p.heads_per_thread);
+  for (int h = chunk * p.heads_per_thread; h < h1; ++h) {
+    int k = 0, hh = h;
+    while (k + 1 < p.segments && hh >= p.seg[k].heads) hh -= p.seg[k++].heads;
+    const Segment& s = p.seg[k];
+    T* dst = static_cast<T*>(s.dst);
+    if (s.scatter) {
+      const int64_t slot = p.slots[token];
+      if (slot < 0 || slot >= p.num_slots) continue;
+      dst += (slot >> p.shift) * s.dst_b + (slot & ((int64_t(1) << p.shift) - 1)) * s.dst_n + hh * s.dst_h;
+    } else {
+      dst += b * s.dst_b + n * s.dst_n + hh * s.dst_h;
+    }
+    const T* src = static_cast<const T*>(s.src) + b * s.src_b + n * s.src_n + hh * s.src_h;
+    Sixteen<T> x;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      x.v[i] = *reinterpret_cast<const uint4*>(src + (i < kPieces / 2 ? lo + i * kPer : hi + (i - kPieces / 2) * kPer));
+    if (s.rotate && turn) {
+      if (!have_angles) {
+        have_angles = true;
+        int64_t pos = n;
+        if (p.positions) {
+          const int64_t at = b * p.pos_stride + n;
+          pos = p.pos_bits == 64 ? static_cast<const int64_t*>(p.positions)[at]
+                                 : int64_t(static_cast<const int32_t*>(p.positions)[at]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint64_t phase = uint64_t(pos) * p.freq[8 * c + i];
+          const float turns = float(int32_t(phase >> 32)) * 0x1p-32f;  // in [-1/2, 1/2)
+          sincospif(2.f * turns, &sn[i], &cs[i]);
+          sn[i] *= p.sign * p.magnitude;
+          cs[i] *= p.magnitude;
+        }
+      }
+      T* e = reinterpret_cast<T*>(x.v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        T& u = e[kLayout == 0 ? i : 2 * i];
+        T& v = e[kLayout == 0 ? 8 + i : 2 * i + 1];
+        float a, d;
+        to_float(u, a);
+        to_float(v, d);
+        from_float(a * cs[i] - d * sn[i], u);
+        from_float(d * cs[i] + a * sn[i], v);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      *reinterpret_cast<uint4*>(dst + (i < kPieces / 2 ? lo + i * kPer : hi + (i - kPieces / 2) * kPer)) = x.v[i];
+  }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int element_size(int32_t dtype) { return dtype == B200FA_DTYPE_FP32 ? 4 : 2; }
+
+int check_rotary(const b200fa_rotary_desc* r, int32_t dim) {
+  if (dim < 16 || dim > 1024 || dim % 16)
+    return fail(B200FA_ERR_HEAD_DIM, "head dim must be a multiple of 16 in [16, 1024], got %d", dim);
+  if (!r) return B200FA_OK;
+  if (r->struct_size != sizeof(b200fa_rotary_desc)) return fail(B200FA_ERR_ROTARY, "b200fa_rotary_desc.struct_size mismatch");
+  if (r->dim != dim || r->rot < 16 || r->rot > dim || r->rot % 16 || r->layout < 0 || r->layout > 1 || !r->freq)
+    return fail(B200FA_ERR_ROTARY, "rotary dim %d, rot %d, layout %d: rot is a multiple of 16 up to the head dim %d", r->dim,
+                r->rot, r->layout, dim);
+  return B200FA_OK;
+}
+
+int check_strides(const int64_t* s, int count, int64_t unit, const char* what) {
+  for (int i = 0; i < count; ++i)
+    if (s[i] < 0 || s[i] % unit)
+      return fail(B200FA_ERR_STRIDE, "%s: stride %lld is not a non-negative multiple of 16 bytes", what, (long long)s[i]);
+  return B200FA_OK;
+}
+
+// As many heads in turn per thread as leave the card full (148 x 2048
+// threads); one each when there is little work, for the shortest chain.
+int launch_rotary(RotaryParams& p, const b200fa_rotary_desc* r, int32_t dim, int32_t dtype, void* stream) {
+  p.lanes = dim / 16;
+  p.rot = r ? r->rot : 0;
+  p.freq = r ? r->freq : nullptr;
+  p.magnitude = r ? r->magnitude : 1.f;
+  p.sign = r && r->inverse ? -1.f : 1.f;
+  int hpt = 1;
+  while (hpt < 8 && hpt < p.heads && p.tokens * p.lanes * p.heads / (2 * hpt) >= 148 * 2048) hpt *= 2;
+  p.heads_per_thread = hpt;
+  p.head_chunks = (p.heads + hpt - 1) / hpt;
+  const int64_t threads = p.tokens * p.head_chunks * p.lanes;
+  const int64_t blocks = (threads + 255) / 256;
+  if (blocks > kInt32Max) return fail(B200FA_ERR_TOO_LARGE, "too many rows for one launch");
+  const int layout = r ? r->layout : 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+#define B200FA_ROTARY(T)                                                       \
+  if (layout == 0) b200_rotary_kernel<T, 0><<<unsigned(blocks), 256, 0, st>>>(p); \
+  else b200_rotary_kernel<T, 1><<<unsigned(blocks), 256, 0, st>>>(p)
+  if (dtype == B200FA_DTYPE_FP16) { B200FA_ROTARY(__half); }
+  else if (dtype == B200FA_DTYPE_BF16) { B200FA_ROTARY(__nv_bfloat16); }
+  else { B200FA_ROTARY(float); }
+#undef B200FA_ROTARY
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? B200FA_OK : cuda_fail(e, "rotary kernel launch");
+}
+
+int page_shift(int32_t page_size) {
+  if (page_size < 8 || page_size > (1 << 20) || (page_size & (page_size - 1))) return -1;
+  int s = 0;
+  while ((1 << s) < page_size) ++s;
+  return s;
+}
+
+}  // namespace
+}  // namespace b200fa
+
+using namespace b200fa;
+
+extern "C" {
+
+int b200fa_build_tables(const int32_t* ctx_lens, const int32_t* new_lens, int32_t requests, int32_t* block_table,
+                        int64_t table_stride, int32_t width, const int32_t* free_pages, int64_t free_capacity,
+                        const int32_t* free_count, int32_t page_size, int64_t* slots, int32_t* positions,
+                        int64_t num_tokens, int32_t* cu_q, int32_t* kv_lens, int32_t* free_left, int32_t* status,
+                        void* stream) {
+  clear_error();
+  if (!ctx_lens || !new_lens || !block_table || !free_count || !cu_q || !kv_lens || !free_left || !status ||
+      (free_capacity > 0 && !free_pages) || (num_tokens > 0 && (!slots || !positions)))
+    return fail(B200FA_ERR_NULL, "a required pointer is NULL");
+  if (requests < 1 || width < 1 || table_stride < width || num_tokens < 0 || free_capacity < 0)
+    return fail(B200FA_ERR_SHAPE, "requests %d, width %d, stride %lld, tokens %lld", requests, width,
+                (long long)table_stride, (long long)num_tokens);
+  if (requests > B200FA_MAX_REQUESTS || num_tokens > kInt32Max)
+    return fail(B200FA_ERR_TOO_LARGE, "at most %d requests and 2^31-1 tokens", B200FA_MAX_REQUESTS);
+  const int shift = page_shift(page_size);
+  if (shift < 0) return fail(B200FA_ERR_PAGE_SIZE, "page size must be a power of two in [8, 2^20], got %d", page_size);
+  TableParams p{ctx_lens, new_lens, block_table, table_stride, free_pages, free_count, slots, positions, cu_q, kv_lens,
+                free_left, status, num_tokens, free_capacity, requests, width, shift};
+  int64_t blocks = (num_tokens + 4 * kTableThreads - 1) / (4 * kTableThreads);
+  blocks = blocks < 1 ? 1 : blocks > 296 ? 296 : blocks;
+  b200_build_tables_kernel<<<unsigned(blocks), kTableThreads, size_t(2 * (requests + 1)) * 4,
+                             static_cast<cudaStream_t>(stream)>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? B200FA_OK : cuda_fail(e, "page table kernel launch");
+}
+
+int b200fa_rotary(const void* x, void* out, int64_t batch, int64_t n, int64_t heads, const int64_t* x_strides,
+                  const int64_t* out_strides, const void* positions, int32_t pos_bits, int64_t pos_stride,
+                  const b200fa_rotary_desc* rotary, int32_t dtype, void* stream) {
+  clear_error();
+  if (!x_strides || !out_strides || !rotary) return fail(B200FA_ERR_NULL, "strides and rotary must not be NULL");
+  if (dtype < B200FA_DTYPE_FP16 || dtype > B200FA_DTYPE_FP32) return fail(B200FA_ERR_DTYPE, "unknown dtype %d", dtype);
+  int rc = check_rotary(rotary, rotary->dim);
+  if (rc != B200FA_OK) return rc;
+  if (batch < 0 || n < 0 || heads < 0 || batch > kInt32Max || n > kInt32Max || heads > kInt32Max ||
+      (positions && pos_bits != 32 && pos_bits != 64) || pos_stride < 0)
+    return fail(B200FA_ERR_SHAPE, "invalid rotary geometry");
+  if (batch == 0 || n == 0 || heads == 0) return B200FA_OK;
+  if (!x || !out) return fail(B200FA_ERR_NULL, "x and out must be device pointers");
+  if (!aligned16(x) || !aligned16(out)) return fail(B200FA_ERR_ALIGNMENT, "tensor pointers must be 16-byte aligned");
+  const int64_t unit = 16 / element_size(dtype);
+  if ((rc = check_strides(x_strides, 3, unit, "x")) != B200FA_OK) return rc;
+  if ((rc = check_strides(out_strides, 3, unit, "out")) != B200FA_OK) return rc;
+  RotaryParams p{};
+  p.seg[0] = Segment{x, out, x_strides[0], x_strides[1], x_strides[2], out_strides[0], out_strides[1], out_strides[2],
+                     int32_t(heads), 1, 0};
+  p.segments = 1;
+  p.heads = int32_t(heads);
+  p.n = n;
+  p.tokens = batch * n;
+  p.positions = positions;
+  p.pos_bits = pos_bits;
+  p.pos_stride = pos_stride;
+  return launch_rotary(p, rotary, rotary->dim, dtype, stream);
+}
+
+int b200fa_append(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, const void* k,
+                  const int64_t* k_strides, const void* v, const int64_t* v_strides, void* k_pages,
+                  const int64_t* k_page_strides, void* v_pages, const int64_t* v_page_strides, int64_t tokens,
+                  int32_t heads_q, int32_t heads_kv, int32_t dim, int64_t num_pages, int32_t page_size,
+                  const int64_t* slots, const void* positions, int32_t pos_bits, const b200fa_rotary_desc* rotary,
+                  int32_t dtype, void* stream) {
+  clear_error();
+  if (dtype != B200FA_DTYPE_FP16 && dtype != B200FA_DTYPE_BF16) return fail(B200FA_ERR_DTYPE, "unknown dtype %d", dtype);
+  int rc = check_rotary(rotary, dim);
+  if (rc != B200FA_OK) return rc;
+  if (tokens < 0 || tokens > kInt32Max || heads_kv < 1 || (q && heads_q < 1) || num_pages < 1 || num_pages > kInt32Max)
+    return fail(B200FA_ERR_SHAPE, "tokens %lld, heads %d and %d, pages %lld", (long long)tokens, heads_q, heads_kv,
+                (long long)num_pages);
+  const int shift = page_shift(page_size);
+  if (shift < 0) return fail(B200FA_ERR_PAGE_SIZE, "page size must be a power of two in [8, 2^20], got %d", page_size);
+  if (!k_strides || !v_strides || !k_page_strides || !v_page_strides || (q && (!q_strides || !q_out_strides || !q_out)))
+    return fail(B200FA_ERR_NULL, "a required pointer is NULL");
+  if (rotary && positions && pos_bits != 32 && pos_bits != 64) return fail(B200FA_ERR_SHAPE, "positions are int32 or int64");
+  if (tokens == 0) return B200FA_OK;
+  if (!k || !v || !k_pages || !v_pages || !slots || (rotary && !positions))
+    return fail(B200FA_ERR_NULL, "k, v, pages, slots and (with rotary) positions must be device pointers");
+  if (!aligned16(q) || !aligned16(q_out) || !aligned16(k) || !aligned16(v) || !aligned16(k_pages) || !aligned16(v_pages))
+    return fail(B200FA_ERR_ALIGNMENT, "tensor pointers must be 16-byte aligned");
+  if ((q && ((rc = check_strides(q_strides, 2, 8, "q")) || (rc = check_strides(q_out_strides, 2, 8, "q_out")))) ||
+      (rc = check_strides(k_strides, 2, 8, "k")) || (rc = check_strides(v_strides, 2, 8, "v")) ||
+      (rc = check_strides(k_page_strides, 3, 8, "k_pages")) || (rc = check_strides(v_page_strides, 3, 8, "v_pages")))
+    return rc;
+  RotaryParams p{};
+  int n = 0;
+  p.seg[n++] = Segment{k, k_pages, 0, k_strides[0], k_strides[1], k_page_strides[0], k_page_strides[1],
+                       k_page_strides[2], heads_kv, rotary != nullptr, 1};
+  p.seg[n++] = Segment{v, v_pages, 0, v_strides[0], v_strides[1], v_page_strides[0], v_page_strides[1],
+                       v_page_strides[2], heads_kv, 0, 1};
+  if (q) p.seg[n++] = Segment{q, q_out, 0, q_strides[0], q_strides[1], 0, q_out_strides[0], q_out_strides[1], heads_q,
+                              rotary != nullptr, 0};
+  p.segments = n;
+  p.heads = 2 * heads_kv + (q ? heads_q : 0);
+  p.n = tokens;
+  p.tokens = tokens;
+  p.positions = positions;
+  p.pos_bits = pos_bits;
+  p.slots = slots;
+  p.num_slots = num_pages << shift;
+  p.shift = shift;
+  return launch_rotary(p, rotary, dim, dtype, stream);
+}
+
+}  // extern "C"

@@ -33,6 +33,12 @@ DEV_OK = 0
 DEV_TIMEOUT = 1
 DEV_BOUNDS = 2
 DEV_PHASE = 3
+DEV_PAGE = 4
+
+DTYPE_FP16 = 0
+DTYPE_BF16 = 1
+DTYPE_FP32 = 2
+MAX_REQUESTS = 4096
 CHECK_SITE = 0x80  # low byte of the status site of a failed check: 0x80 + check number
 
 WS_HEADER_BYTES = 256
@@ -56,6 +62,25 @@ class Options(C.Structure):
                 ("window", C.c_int32), ("sinks", C.c_int32)]
 
 
+class RotaryDesc(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("dim", C.c_int32), ("rot", C.c_int32), ("layout", C.c_int32),
+                ("inverse", C.c_int32), ("magnitude", C.c_float), ("freq", C.c_void_p)]
+
+
+class PagedArgs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("dtype", C.c_int32),
+                ("q", C.c_void_p), ("o", C.c_void_p), ("k_pages", C.c_void_p), ("v_pages", C.c_void_p),
+                ("q_strides", _i64 * 2), ("o_strides", _i64 * 2), ("k_strides", _i64 * 3), ("v_strides", _i64 * 3),
+                ("block_table", C.c_void_p), ("table_stride", _i64), ("kv_lens", C.c_void_p), ("cu_q", C.c_void_p),
+                ("tokens", _i64), ("num_pages", _i64),
+                ("requests", _i32), ("width", _i32), ("page_size", _i32), ("heads_q", _i32), ("heads_kv", _i32),
+                ("max_q", _i32), ("scale", _f), ("window", _i32), ("sinks", _i32), ("timeout_us", _u32),
+                ("workspace", C.c_void_p), ("ws_bytes", _u64)]
+
+
+Strides2, Strides3 = _i64 * 2, _i64 * 3
+_s = C.POINTER(_i64)
+
 SIGNATURES = {
     "b200fa_num_units": (_i64, [_i64, _i64, _i64]),
     "b200fa_partition": (C.c_int, [_i64, _i32, _i32, C.POINTER(_i64), C.POINTER(_i64)]),
@@ -75,6 +100,13 @@ SIGNATURES = {
     "b200fa_test_exp2": (C.c_int, [_p, _p, _p, _i64, _p]),
     "b200fa_fwd_noalloc": (C.c_int, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _f, _i32,
                                      _i64, _i64, _p, C.POINTER(Options), C.POINTER(_p)]),
+    "b200fa_build_tables": (C.c_int, [_p, _p, _i32, _p, _i64, _i32, _p, _i64, _p, _i32, _p, _p, _i64,
+                                      _p, _p, _p, _p, _p]),
+    "b200fa_rotary": (C.c_int, [_p, _p, _i64, _i64, _i64, _s, _s, _p, _i32, _i64, C.POINTER(RotaryDesc), _i32, _p]),
+    "b200fa_append": (C.c_int, [_p, _s, _p, _s, _p, _s, _p, _s, _p, _s, _p, _s, _i64, _i32, _i32, _i32, _i64, _i32,
+                                _p, _p, _i32, C.POINTER(RotaryDesc), _i32, _p]),
+    "b200fa_paged_workspace_size": (_i64, []),
+    "b200fa_paged_fwd": (C.c_int, [C.POINTER(PagedArgs), _p]),
 }
 
 _lock = threading.Lock()

@@ -95,13 +95,16 @@ class Operator:
     def __call__(self, q, k, v, *, scale: float | None = None, out: torch.Tensor | None = None,
                  unit_range: tuple[int, int] | None = None, flags: int = 0,
                  capture: torch.Tensor | None = None, causal: bool = False, window: int = 0,
-                 sinks: int = 0) -> torch.Tensor:
+                 sinks: int = 0, rotary=None, positions: torch.Tensor | None = None) -> torch.Tensor:
         """O = softmax(Q K^T * scale) V.  ``causal``: query row i attends keys
         0..i only (top-left aligned, as torch's ``is_causal``; an addition,
         the reference's operator is non-causal).  ``window`` > 0 (with
         ``causal``): only keys i - window < j <= i of those, and the first
         ``sinks`` keys; a row that sees no key (Nq > Nk) gets zeros, and key
-        blocks that no row of a work item sees are not read.  ``capture`` (FP32, at least
+        blocks that no row of a work item sees are not read.  ``rotary`` (a
+        ``fa_b200.rotary.Rotary``): Q and K are turned by it first, into new
+        tensors, by ``positions`` ([N] or [B, N]; None: 0 .. N-1; given
+        positions need Nq == Nk).  ``capture`` (FP32, at least
         ``capture_bytes(...)`` bytes, on Q's device) turns on the debug
         capture of the per-block online-softmax state (``capture_view``)."""
         if causal:
@@ -110,6 +113,12 @@ class Operator:
         if window:
             flags |= lib.FLAG_WINDOW
         B, Hq, Hkv, Nq, Nk = _geometry(q, k, v)
+        if rotary is not None:
+            if positions is not None and Nq != Nk:
+                raise ValueError("positions serve Q and K alike and need Nq == Nk")
+            q, k = rotary(q, positions), rotary(k, positions)
+        elif positions is not None:
+            raise ValueError("positions need a rotary")
         if out is None:
             out = torch.empty_like(q)
         elif out.shape != q.shape or out.dtype != torch.float16 or not out.is_contiguous() \

@@ -1,0 +1,136 @@
+"""Rotary positions: ``Rotary`` turns pairs of a head's elements by angles that
+grow with the token's position.
+
+Frequencies: pair i of ``rotary_dim`` / 2 turns by base^(-2i/rotary_dim) per
+position; ``scaling`` stretches them for contexts longer than trained on:
+
+* ``"linear"``: all divided by ``factor``;
+* ``"banded"``: pairs that turn more than ``high`` times within
+  ``original_length`` positions are left, those that turn less than ``low``
+  times are divided by ``factor``, those between are blended linearly in the
+  number of turns.
+
+``magnitude`` multiplies the rotated elements.  The kernel keeps each
+frequency as a 64-bit fraction of a turn, so the angle of any position is
+exact before its sine is taken.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from . import lib
+
+LAYOUTS = {"half": 0, "interleaved": 1}
+DTYPES = {torch.float16: lib.DTYPE_FP16, torch.bfloat16: lib.DTYPE_BF16, torch.float32: lib.DTYPE_FP32}
+
+
+class Rotary:
+    """``rotary(x, positions) -> y`` with y shaped like x.
+
+    dim:        elements of a head (a multiple of 16).
+    rotary_dim: the first elements that are turned (a multiple of 16; default
+                all); the rest is copied.
+    layout:     "half" pairs elements (i, i + rotary_dim/2), "interleaved"
+                (2i, 2i + 1).
+    """
+
+    def __init__(self, dim: int = 128, *, rotary_dim: int | None = None, base: float = 10000.0,
+                 layout: str = "half", scaling: str | None = None, factor: float = 1.0,
+                 original_length: int = 0, low: float = 1.0, high: float = 4.0, magnitude: float = 1.0):
+        rotary_dim = dim if rotary_dim is None else rotary_dim
+        if dim < 16 or dim > 1024 or dim % 16 or rotary_dim < 16 or rotary_dim > dim or rotary_dim % 16:
+            raise ValueError("dim and rotary_dim must be multiples of 16, rotary_dim at most dim, dim at most 1024")
+        if layout not in LAYOUTS:
+            raise ValueError(f"layout must be one of {sorted(LAYOUTS)}")
+        if scaling not in (None, "linear", "banded"):
+            raise ValueError('scaling must be None, "linear" or "banded"')
+        if not (base > 0 and math.isfinite(base) and factor > 0 and math.isfinite(factor) and math.isfinite(magnitude)):
+            raise ValueError("base and factor must be positive and finite, magnitude finite")
+        if scaling == "banded" and not (original_length > 0 and high > low):
+            raise ValueError("banded scaling needs original_length > 0 and high > low")
+        self.dim, self.rotary_dim, self.layout = dim, rotary_dim, layout
+        self.magnitude = float(magnitude)
+        self.frequencies = []  # angle per position of each pair
+        for i in range(rotary_dim // 2):
+            f = base ** (-2.0 * i / rotary_dim)
+            if scaling == "linear":
+                f /= factor
+            elif scaling == "banded":
+                turns = original_length * f / (2.0 * math.pi)
+                keep = min(1.0, max(0.0, (turns - low) / (high - low)))
+                f = f * keep + f / factor * (1.0 - keep)
+            self.frequencies.append(f)
+        self._tables = {}  # device -> int64 tensor of 0.64 fixed-point turns
+        self._descs = {}   # (device, inverse) -> RotaryDesc
+
+    def table(self, device) -> torch.Tensor:
+        """The frequencies on ``device`` (made at its first use: outside a stream capture)."""
+        t = self._tables.get(device)
+        if t is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the first use of a Rotary on a device cannot be captured: call table(device) before")
+            turns = [round(f / (2.0 * math.pi) * 2.0**64) % 2**64 for f in self.frequencies]
+            t = torch.tensor([x - 2**64 if x >= 2**63 else x for x in turns], dtype=torch.int64).to(device)
+            self._tables[device] = t
+        return t
+
+    def desc(self, device, inverse: bool = False) -> lib.RotaryDesc:
+        d = self._descs.get((device, inverse))
+        if d is None:
+            d = self._descs[(device, inverse)] = lib.RotaryDesc(
+                C.sizeof(lib.RotaryDesc), self.dim, self.rotary_dim, LAYOUTS[self.layout], int(inverse), self.magnitude,
+                self.table(device).data_ptr())
+        return d
+
+    def __call__(self, x: torch.Tensor, positions: torch.Tensor | None = None, *, out: torch.Tensor | None = None,
+                 inverse: bool = False) -> torch.Tensor:
+        """x: [B,H,N,dim] (the attention operator's layout) or [N,H,dim] (a
+        token batch), FP16, BF16 or FP32, last dimension contiguous, any
+        other strides of whole 16 bytes.  positions: [N] or [B,N], int32 or
+        int64 on x's device; None is 0 .. N-1.  out may be x.  ``inverse``
+        turns back; with the magnitude it is the transposed map, so it carries
+        a gradient of y to x."""
+        if x.ndim not in (3, 4) or x.shape[-1] != self.dim:
+            raise ValueError(f"x must be [B,H,N,{self.dim}] or [N,H,{self.dim}]")
+        dtype = DTYPES.get(x.dtype)
+        if dtype is None or x.device.type != "cuda":
+            raise ValueError("x must be FP16, BF16 or FP32 on a CUDA device")
+        if out is None:
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+            raise ValueError("out must be shaped and typed like x, on its device")
+        if x.ndim == 4:
+            B, H, N, _ = x.shape
+            xs, os = x.stride(), out.stride()
+            xs, os = (xs[0], xs[2], xs[1], xs[3]), (os[0], os[2], os[1], os[3])
+        else:
+            B, (N, H, _) = 1, x.shape
+            xs, os = (0, *x.stride()), (0, *out.stride())
+        if xs[3] != 1 or os[3] != 1:
+            raise ValueError("the last dimension of x and out must be contiguous")
+        bits, pos_ptr, pos_stride = 32, None, 0
+        if positions is not None:
+            bits = _position_bits(positions, x.device)
+            if positions.shape == (N,):
+                pass
+            elif positions.shape == (B, N):
+                pos_stride = N
+            else:
+                raise ValueError("positions must be [N] or [B,N]")
+            pos_ptr = positions.data_ptr()
+        with torch.cuda.device(x.device):
+            stream = torch.cuda.current_stream(x.device).cuda_stream
+            lib.check(lib.load().b200fa_rotary(
+                x.data_ptr(), out.data_ptr(), B, N, H, lib.Strides3(*xs[:3]), lib.Strides3(*os[:3]), pos_ptr, bits,
+                pos_stride, C.byref(self.desc(x.device, bool(inverse))), dtype, stream), "b200fa_rotary")
+        return out
+
+
+def _position_bits(positions, device) -> int:
+    if positions.dtype not in (torch.int32, torch.int64) or positions.device != device or not positions.is_contiguous():
+        raise ValueError("positions must be contiguous int32 or int64 on the same device")
+    return 64 if positions.dtype == torch.int64 else 32

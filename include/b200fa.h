@@ -69,6 +69,10 @@ extern "C" {
 #define B200FA_ERR_OPTIONS      -11   /* malformed b200fa_options              */
 #define B200FA_ERR_NO_DRIVER    -12   /* cuTensorMapEncodeTiled unavailable    */
 #define B200FA_ERR_TENSOR_MAP   -13   /* cuTensorMapEncodeTiled rejected a map */
+#define B200FA_ERR_DTYPE        -14   /* unknown element type                  */
+#define B200FA_ERR_PAGE_SIZE    -15   /* page size not a power of two, 8..2^20 */
+#define B200FA_ERR_STRIDE       -16   /* a stride that the kernels cannot read */
+#define B200FA_ERR_ROTARY       -17   /* malformed rotary description          */
 
 /* Device status word values (b200fa_read_status, status[0]). */
 #define B200FA_DEV_OK             0
@@ -77,6 +81,15 @@ extern "C" {
 #define B200FA_DEV_BOUNDS         2   /* a coordinate, index or layout check failed;
                                          site low byte = 0x80 + check number    */
 #define B200FA_DEV_PHASE          3   /* the roles' key-block counts disagreed at exit */
+
+#define B200FA_DEV_PAGE           4   /* paged attention: a request's block table ended
+                                         early or named a page outside the cache; the
+                                         keys there were read as zeros          */
+
+/* Element types of the serving operators. */
+#define B200FA_DTYPE_FP16         0
+#define B200FA_DTYPE_BF16         1
+#define B200FA_DTYPE_FP32         2   /* b200fa_rotary only                     */
 
 /* Option flags (b200fa_options.flags). */
 #define B200FA_FLAG_TRACE          1u /* write one trace record per CTA        */
@@ -284,6 +297,115 @@ int b200fa_fwd_noalloc(const void* q, const void* k, const void* v, void* o,
                        int64_t D, float scale, int32_t variant,
                        int64_t unit_begin, int64_t unit_end,
                        void* stream, const b200fa_options* opts, void** scratch_out);
+
+/* ------------------------------------------------------------------------
+ * Serving: a paged K/V cache, the tables of a step, and the attention that
+ * reads them (additions; the reference has no cache).
+ *
+ * A cache is two tensors of pages, K and V, [num_pages][page_size][Hkv][128]
+ * in any order of the outer three dimensions (strides in elements, multiples
+ * of 8; the head dim is contiguous).  Token i of request r lives at offset
+ * i % page_size of page block_table[r][i / page_size]; its slot is
+ * page * page_size + offset.  Page sizes are powers of two. */
+
+/* The tables of one step, from request lengths, on the device.  Request r
+ * holds ctx_lens[r] tokens in ceil(ctx/page_size) pages and adds new_lens[r];
+ * the pages it needs beyond those are taken from the end of the free list
+ * (free_pages[*free_count - 1] first), in request order.  Writes
+ *   block_table[r][...]  the entries of the new pages (others untouched)
+ *   slots, positions     [num_tokens], requests after one another; places
+ *                        behind the last token get slot -1, position 0
+ *   cu_q [requests + 1]  prefix sums of new_lens
+ *   kv_lens [requests]   ctx + new
+ *   free_left, status    [1]: pages left; 0, or 1 the free list is too short,
+ *                        2 a request outgrows its table row (width), 3 more
+ *                        new tokens than num_tokens.  With a status other
+ *                        than 0 nothing is handed out: every slot is -1,
+ *                        kv_lens = ctx_lens, free_left = *free_count, the
+ *                        table is untouched.
+ * Lengths below 0 count as 0.  No output may overlap an input (the table
+ * apart).  At most B200FA_MAX_REQUESTS requests.  One launch on `stream`. */
+#define B200FA_MAX_REQUESTS 4096
+int b200fa_build_tables(const int32_t* ctx_lens, const int32_t* new_lens, int32_t requests, int32_t* block_table,
+                        int64_t table_stride, int32_t width, const int32_t* free_pages, int64_t free_capacity,
+                        const int32_t* free_count, int32_t page_size, int64_t* slots, int32_t* positions,
+                        int64_t num_tokens, int32_t* cu_q, int32_t* kv_lens, int32_t* free_left, int32_t* status,
+                        void* stream);
+
+/* Rotary positions.  freq[i] is pair i's angle per position in turns, as a
+ * 64-bit binary fraction (0.64 fixed point); the angle of position p is
+ * p * freq[i] mod 1, exact for any 63-bit p.  layout 0: pair (i, i + rot/2);
+ * 1: pair (2i, 2i + 1).  Elements rot.. of a head are copied.  magnitude
+ * multiplies the rotated ones; inverse turns by the negative angle. */
+typedef struct b200fa_rotary_desc {
+    uint32_t        struct_size;
+    int32_t         dim;        /* head dim, a multiple of 16, <= 1024          */
+    int32_t         rot;        /* rotated elements, a multiple of 16, <= dim   */
+    int32_t         layout;
+    int32_t         inverse;
+    float           magnitude;
+    const uint64_t* freq;       /* device, [rot / 2]                            */
+} b200fa_rotary_desc;
+
+/* out = rotation of x, both [batch][n][heads][dim] with strides in elements
+ * (batch, n, heads; multiples of 16 bytes; the last dimension contiguous).
+ * positions: device int32 or int64 (pos_bits 32 / 64), [n] with pos_stride
+ * elements between batches (0: shared), or NULL for 0 .. n-1.  out may be x. */
+int b200fa_rotary(const void* x, void* out, int64_t batch, int64_t n, int64_t heads, const int64_t* x_strides,
+                  const int64_t* out_strides, const void* positions, int32_t pos_bits, int64_t pos_stride,
+                  const b200fa_rotary_desc* rotary, int32_t dtype, void* stream);
+
+/* Writes a step's K and V [tokens][heads_kv][dim] into the cache at `slots`
+ * (int64; a slot outside [0, num_pages * page_size) is a padded token and
+ * skipped; slots of real tokens are distinct), with K rotated by its token's
+ * position, and writes the rotated q [tokens][heads_q][dim] to q_out (q NULL:
+ * none; q_out may be q).  rotary NULL: plain copies, positions ignored.
+ * *_strides: token, head (q, k, v, q_out) or page, token, head (pages). */
+int b200fa_append(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides,
+                  const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                  void* k_pages, const int64_t* k_page_strides, void* v_pages, const int64_t* v_page_strides,
+                  int64_t tokens, int32_t heads_q, int32_t heads_kv, int32_t dim, int64_t num_pages,
+                  int32_t page_size, const int64_t* slots, const void* positions, int32_t pos_bits,
+                  const b200fa_rotary_desc* rotary, int32_t dtype, void* stream);
+
+/* Attention of new tokens over a paged cache.  Request r's new tokens are rows
+ * cu_q[r] .. cu_q[r+1]-1 of q and o; row i of them stands at position
+ * p = kv_lens[r] - (cu_q[r+1] - cu_q[r]) + i and attends the cached keys
+ * j <= p, with window > 0 only j > p - window or j < sinks.  A row that sees
+ * no key gets zeros; rows of o that belong to no request are not written.
+ * Pages that no row of a work item sees are not read, nor are values behind a
+ * request's last key used, so both may hold anything. */
+typedef struct b200fa_paged_args {
+    uint32_t    struct_size;    /* sizeof(b200fa_paged_args)                     */
+    int32_t     dtype;          /* FP16 or BF16 (q, cache and o alike)           */
+    const void* q;              /* [tokens][heads_q][128]                        */
+    void*       o;
+    const void* k_pages;
+    const void* v_pages;
+    int64_t     q_strides[2];   /* token, head                                   */
+    int64_t     o_strides[2];
+    int64_t     k_strides[3];   /* page, token, head                             */
+    int64_t     v_strides[3];
+    const int32_t* block_table; /* [requests][width]                             */
+    int64_t     table_stride;
+    const int32_t* kv_lens;     /* [requests]                                    */
+    const int32_t* cu_q;        /* [requests + 1]                                */
+    int64_t     tokens;
+    int64_t     num_pages;
+    int32_t     requests, width, page_size;
+    int32_t     heads_q, heads_kv;
+    int32_t     max_q;          /* the longest chunk (a hint: picks the kernel)  */
+    float       scale;
+    int32_t     window, sinks;  /* window 0: none                                */
+    uint32_t    timeout_us;     /* bound of every device-side wait; 0 = 2 s      */
+    void*       workspace;      /* 256-byte aligned, its header zeroed once      */
+    uint64_t    ws_bytes;
+} b200fa_paged_args;
+
+/* Bytes of workspace on the current device (status header + partial results);
+ * calls that share a workspace must not overlap on the GPU.  Negative: error. */
+int64_t b200fa_paged_workspace_size(void);
+int b200fa_paged_fwd(const b200fa_paged_args* args, void* stream);
 
 #ifdef __cplusplus
 }
