@@ -49,7 +49,8 @@ NVCC_FLAGS = ARCH_FLAGS + [
     "-shared",
     "-Xptxas", "-v",
 ]
-SOURCES = ("b200fa.cu", "b200fa_causal.cu", "b200fa_window.cu", "serving.cu", "paged.cu")
+SOURCES = ("b200fa.cu", "b200fa_causal.cu", "b200fa_window.cu", "serving.cu", "paged.cu",
+           "paged_chunk.cu")
 
 
 def nvcc_path() -> str:

@@ -72,12 +72,12 @@ PagedKernel short_kernel(bool bf16, int m) {
 
 struct PagedDevice {
   std::once_flag once;
-  int sms = 0;
+  int sms = 0, pairs = 0;
   cudaError_t err = cudaSuccess;
 };
 PagedDevice g_paged[64];
 
-int paged_device(int* sms) {
+int paged_device(const PagedDevice** out) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
@@ -89,34 +89,52 @@ int paged_device(int* sms) {
       for (int m : {1, 2, 4})
         if (e == cudaSuccess)
           e = cudaFuncSetAttribute(short_kernel(bf16, m), cudaFuncAttributeMaxDynamicSharedMemorySize, kShortSmemBytes);
+    if (e == cudaSuccess) e = cudaError_t(paged_chunk_setup(&d.pairs));
     if (d.sms > kMaxWorkers) d.sms = kMaxWorkers;
+    if (d.pairs > kMaxWorkers) d.pairs = kMaxWorkers;
     d.err = e;
   });
   if (d.err != cudaSuccess) return cuda_fail(d.err, "device setup");
-  *sms = d.sms;
+  *out = &d;
   return B200FA_OK;
 }
 
 uint64_t partial_bytes(int workers, int rows) { return uint64_t(2) * workers * rows * 130u * 4u; }
 
-uint64_t workspace_bytes(int sms) { return kPagedPartials + partial_bytes(sms, 64); }
+uint64_t workspace_bytes(const PagedDevice& d) {
+  const uint64_t a = partial_bytes(d.sms, 64), b = partial_bytes(d.pairs, 256);
+  return kPagedPartials + (a > b ? a : b);
+}
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-int encode_pages(CUtensorMap* map, const b200fa_paged_args& a, const void* ptr, const int64_t* strides, const char* what) {
+int encode(CUtensorMap* map, const b200fa_paged_args& a, const void* ptr, const cuuint64_t (&dims)[4],
+           const cuuint64_t (&strides)[3], const cuuint32_t (&box)[4], const char* what) {
   PFN_cuTensorMapEncodeTiled_v12000 fn = encode_fn();
   if (!fn) return fail(B200FA_ERR_NO_DRIVER, "cuTensorMapEncodeTiled is not available from the driver");
-  const cuuint64_t dims[4] = {128, cuuint64_t(a.page_size), cuuint64_t(a.heads_kv), cuuint64_t(a.num_pages)};
-  // A dimension of one element has no stride of its own.
-  const cuuint64_t st[3] = {cuuint64_t(a.page_size > 1 ? strides[1] : 128) * 2, cuuint64_t(a.heads_kv > 1 ? strides[2] : 128) * 2,
-                            cuuint64_t(a.num_pages > 1 ? strides[0] : 128) * 2};
-  const cuuint32_t box[4] = {64, cuuint32_t(a.page_size < kPagedBlock ? a.page_size : kPagedBlock), 1, 1};
   const cuuint32_t one[4] = {1, 1, 1, 1};
   const CUresult r = fn(map, a.dtype == B200FA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                        const_cast<void*>(ptr), dims, st, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        const_cast<void*>(ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(B200FA_ERR_TENSOR_MAP, "cuTensorMapEncodeTiled failed for %s (%d)", what, int(r));
   return B200FA_OK;
+}
+
+// Byte stride of a dimension; one of a single element has no stride of its own.
+cuuint64_t stride_of(int64_t count, int64_t stride) { return cuuint64_t(count > 1 ? stride : 128) * 2; }
+
+// Boxes of 64 columns and up to `rows` tokens of a page.
+int encode_pages(CUtensorMap* map, const b200fa_paged_args& a, const void* ptr, const int64_t* s, int rows, const char* what) {
+  return encode(map, a, ptr, {128, cuuint64_t(a.page_size), cuuint64_t(a.heads_kv), cuuint64_t(a.num_pages)},
+                {stride_of(a.page_size, s[1]), stride_of(a.heads_kv, s[2]), stride_of(a.num_pages, s[0])},
+                {64, cuuint32_t(a.page_size < rows ? a.page_size : rows), 1, 1}, what);
+}
+
+// Boxes of 64 columns of the group's heads of `tokens` tokens.
+int encode_q(CUtensorMap* map, const b200fa_paged_args& a, int32_t group, int32_t tokens) {
+  return encode(map, a, a.q, {128, cuuint64_t(group), cuuint64_t(a.heads_kv), cuuint64_t(a.tokens)},
+                {stride_of(group, a.q_strides[1]), stride_of(a.heads_kv, a.q_strides[1] * group), stride_of(a.tokens, a.q_strides[0])},
+                {64, cuuint32_t(group), 1, cuuint32_t(tokens)}, "q");
 }
 
 int check_paged(const b200fa_paged_args& a) {
@@ -125,7 +143,7 @@ int check_paged(const b200fa_paged_args& a) {
     return fail(B200FA_ERR_SHAPE, "requests %d, tokens %lld, table width %d, pages %lld, heads %d and %d, max_q %d", a.requests,
                 (long long)a.tokens, a.width, (long long)a.num_pages, a.heads_q, a.heads_kv, a.max_q);
   if (a.heads_q % a.heads_kv) return fail(B200FA_ERR_GROUPING, "heads_q (%d) must be a multiple of heads_kv (%d)", a.heads_q, a.heads_kv);
-  if (a.heads_q / a.heads_kv > 64) return fail(B200FA_ERR_GROUPING, "at most 64 query heads per key/value head, got %d", a.heads_q / a.heads_kv);
+  if (a.heads_q / a.heads_kv > 128) return fail(B200FA_ERR_GROUPING, "at most 128 query heads per key/value head, got %d", a.heads_q / a.heads_kv);
   const int64_t most = (int64_t(1) << 31) - 1;
   if (a.page_size < 8 || a.page_size > (1 << 20) || (a.page_size & (a.page_size - 1)))
     return fail(B200FA_ERR_PAGE_SIZE, "page size must be a power of two in [8, 2^20], got %d", a.page_size);
@@ -159,10 +177,10 @@ extern "C" {
 
 int64_t b200fa_paged_workspace_size(void) {
   clear_error();
-  int sms = 0;
-  const int rc = paged_device(&sms);
+  const PagedDevice* d = nullptr;
+  const int rc = paged_device(&d);
   if (rc != B200FA_OK) return rc > 0 ? -int64_t(1000 + rc) : rc;
-  return int64_t(workspace_bytes(sms));
+  return int64_t(workspace_bytes(*d));
 }
 
 int b200fa_paged_fwd(const b200fa_paged_args* args, void* stream) {
@@ -175,15 +193,21 @@ int b200fa_paged_fwd(const b200fa_paged_args* args, void* stream) {
   if (!a.workspace || (reinterpret_cast<uintptr_t>(a.workspace) & 255u))
     return fail(B200FA_ERR_WORKSPACE, "workspace must be 256-byte aligned");
   if (a.requests == 0 || a.tokens == 0) return B200FA_OK;
-  int sms = 0;
-  if ((rc = paged_device(&sms)) != B200FA_OK) return rc;
-  if (a.ws_bytes < workspace_bytes(sms))
-    return fail(B200FA_ERR_WORKSPACE, "workspace must hold %llu bytes", (unsigned long long)workspace_bytes(sms));
+  const PagedDevice* d = nullptr;
+  if ((rc = paged_device(&d)) != B200FA_OK) return rc;
+  if (a.ws_bytes < workspace_bytes(*d))
+    return fail(B200FA_ERR_WORKSPACE, "workspace must hold %llu bytes", (unsigned long long)workspace_bytes(*d));
+
+  const int32_t group = a.heads_q / a.heads_kv;
+  const int64_t rows = int64_t(a.max_q > 0 ? a.max_q : 1) * group;
+  // Up to 64 rows of a request the time is that of its keys' bytes, which the
+  // short kernel reads faster; beyond, that of the products.
+  const bool chunk = rows > 64;
 
   PagedParams p;
   std::memset(&p, 0, sizeof(p));
-  if ((rc = encode_pages(&p.tm_k, a, a.k_pages, a.k_strides, "k_pages")) != B200FA_OK) return rc;
-  if ((rc = encode_pages(&p.tm_v, a, a.v_pages, a.v_strides, "v_pages")) != B200FA_OK) return rc;
+  if ((rc = encode_pages(&p.tm_k, a, a.k_pages, a.k_strides, chunk ? kPagedBlock / 2 : kPagedBlock, "k_pages")) != B200FA_OK) return rc;
+  if ((rc = encode_pages(&p.tm_v, a, a.v_pages, a.v_strides, kPagedBlock, "v_pages")) != B200FA_OK) return rc;
   p.q = a.q;
   p.o = a.o;
   p.q_tok = a.q_strides[0];
@@ -200,24 +224,34 @@ int b200fa_paged_fwd(const b200fa_paged_args* args, void* stream) {
   p.num_pages = int32_t(a.num_pages);
   p.tokens = int32_t(a.tokens);
   p.heads_kv = a.heads_kv;
-  p.group = a.heads_q / a.heads_kv;
+  p.group = group;
   p.window = a.window;
   p.sinks = a.sinks;
   p.scale_log2 = float(double(a.scale) * 1.4426950408889634074);
   p.timeout_ns = uint64_t(a.timeout_us ? a.timeout_us : 2000000u) * 1000ull;
   p.ws = static_cast<uint8_t*>(a.workspace);
-  p.workers = sms;
-
-  const int64_t rows = int64_t(a.max_q > 0 ? a.max_q : 1) * p.group;
-  const int m = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  p.tokens_per_tile = 16 * m / p.group;
-  p.part_rows = 16 * m;
   const bool bf16 = a.dtype == B200FA_DTYPE_BF16;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  short_kernel(bf16, m)<<<p.workers, kShortThreads, kShortSmemBytes, st>>>(p);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e;
+  unsigned row_blocks;
+  if (chunk) {
+    p.workers = d->pairs;
+    p.tokens_per_tile = 2 * (128 / group);  // half of them per CTA of the pair
+    p.part_rows = 256;
+    row_blocks = 8;
+    if ((rc = encode_q(&p.tm_q, a, group, p.tokens_per_tile / 2)) != B200FA_OK) return rc;
+    e = cudaError_t(paged_chunk_launch(p, bf16, st));
+  } else {
+    const int m = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    p.workers = d->sms;
+    p.tokens_per_tile = 16 * m / group;
+    p.part_rows = 16 * m;
+    row_blocks = unsigned(m);
+    short_kernel(bf16, m)<<<p.workers, kShortThreads, kShortSmemBytes, st>>>(p);
+    e = cudaGetLastError();
+  }
   if (e != cudaSuccess) return cuda_fail(e, "paged attention launch");
-  const dim3 grid(unsigned(p.workers), unsigned(m));
+  const dim3 grid(unsigned(p.workers), row_blocks);
   if (bf16) b200_paged_combine_kernel<true><<<grid, 256, 0, st>>>(p);
   else b200_paged_combine_kernel<false><<<grid, 256, 0, st>>>(p);
   e = cudaGetLastError();

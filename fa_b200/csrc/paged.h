@@ -114,12 +114,54 @@ __device__ __forceinline__ PagedBlocks paged_blocks(const PagedParams& p, const 
   return b;
 }
 
+// sum over i < n of floor((a i + b) / m), a, b >= 0, by the Euclidean
+// reduction of (a, m) (the lattice points under a line).
+__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+  int64_t sum = 0;
+  while (n > 0) {
+    sum += a / m * (n * (n - 1) / 2) + b / m * n;
+    a %= m;
+    b %= m;
+    const int64_t top = a * n + b;
+    if (top < m) break;
+    n = top / m;
+    b = top % m;
+    const int64_t t = m;
+    m = a;
+    a = t;
+  }
+  return sum;
+}
+
+// Key blocks of the request's first `tiles` tiles, for one key/value head: the
+// sum of paged_blocks(...).n in closed form, so that a prompt of thousands of
+// tiles takes no longer to place than a token.  With c the position of the
+// request's first row and k the tokens of a tile, tile t ends in block
+// (c + k t + k - 1) / 128 (the last tile of the request: (kv - 1) / 128), and
+// skips the blocks between the sinks' and that of c + k t - window + 1.
+__device__ __forceinline__ int64_t blocks_before(const PagedParams& p, const PagedRequest& q, int tiles) {
+  const int64_t k = p.tokens_per_tile, c = int64_t(q.kv) - q.len;
+  if (tiles <= 0) return 0;
+  const int64_t last = q.tiles(p) - 1;
+  int64_t n = 0, t1 = 0;  // tiles before t1 end before position 0: one masked block each
+  if (c + k - 1 < 0) t1 = (-(c + k - 1) + k - 1) / k;
+  const int64_t full = tiles < last ? tiles : last;  // tiles that are not the request's last
+  if (t1 > full) t1 = full;
+  n += t1;
+  n += floor_sum(full - t1, kPagedBlock, k, c + k * t1 + k - 1) + (full - t1);
+  if (tiles > last) n += q.kv > 0 ? (q.kv - 1) / kPagedBlock + 1 : 1;
+  if (p.window > 0) {
+    const int64_t s = p.sinks / kPagedBlock + (p.sinks % kPagedBlock != 0);
+    const int64_t b = c - (p.window - 1) - s * kPagedBlock;  // keys of tile 0 between its window and the sinks' blocks
+    int64_t t2 = b < 0 ? (-b + k - 1) / k : 0;
+    if (t2 < tiles) n -= floor_sum(tiles - t2, kPagedBlock, k, b + k * t2);
+  }
+  return n;
+}
+
 __device__ __forceinline__ int64_t request_blocks(const PagedParams& p, int r) {
   const PagedRequest q = paged_request(p, r);
-  const int tiles = q.tiles(p);
-  int64_t n = 0;
-  for (int t = 0; t < tiles; ++t) n += paged_blocks(p, q, t).n;
-  return n * p.heads_kv;
+  return blocks_before(p, q, q.tiles(p)) * p.heads_kv;
 }
 
 // A worker's place in the line of blocks.
@@ -166,18 +208,34 @@ __device__ __forceinline__ void find_start(const PagedParams& p, int worker, int
         continue;
       }
       const int64_t head = n / p.heads_kv, x = begin - at;
-      const PagedRequest q = paged_request(p, r);
-      int64_t left = x % head;
-      int t = 0;
-      for (int b; left >= (b = paged_blocks(p, q, t).n); ++t) left -= b;
       start->r = r;
       start->h = int(x / head);
-      start->tile = t;
-      start->off = int(left);
+      scratch[0] = x % head;
       break;
     }
   }
   __syncthreads();
+  if (end <= begin) return;
+  // The tile: every thread looks at the beginning of one in `step`.
+  const PagedRequest q = paged_request(p, start->r);
+  const int64_t rest = scratch[0];
+  int lo = 0, n = q.tiles(p);
+  while (true) {
+    const int step = (n + nt - 1) / nt;
+    const int t = lo + tid * step;
+    __syncthreads();
+    if (t < lo + n) {
+      const int64_t before = blocks_before(p, q, t);
+      if (before <= rest && rest < blocks_before(p, q, min(t + step, lo + n))) {
+        start->tile = t;
+        start->off = int(rest - before);
+      }
+    }
+    __syncthreads();
+    lo = start->tile;
+    if (step == 1) break;
+    n = min(step, q.tiles(p) - lo);
+  }
 }
 
 // Walks a worker's items; every role of a kernel walks the same ones.
@@ -255,5 +313,10 @@ __device__ __forceinline__ void paged_status(const PagedParams& p, uint32_t code
     ws[2] = blockIdx.x;
   }
 }
+
+// The chunk kernel (paged_chunk.cu): workers are CTA pairs.  0 or a CUDA error.
+using PagedChunkKernel = void (*)(PagedParams);
+int paged_chunk_setup(int* pairs);
+int paged_chunk_launch(const PagedParams& p, bool bf16, cudaStream_t stream);
 
 }  // namespace b200fa

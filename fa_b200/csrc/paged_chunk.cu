@@ -1,0 +1,635 @@
+// paged_chunk.cu -- attention over a paged cache for many rows: chunks of
+// prompts.  Bound by the tensor cores (4 * 128 * rows flops per key), so the
+// products run as the dense attention kernel's do (fa_kernel.cuh, whose
+// pipeline, tensor memory layout and register split this kernel shares):
+// pairs of CTAs, tcgen05 cta_group::2, M = 256, S and PV issued by a thread
+// each, two softmax warpgroups on alternate key blocks, TMA rings for K and V.
+//
+// What differs:
+//   * a work item is a tile of new tokens times the heads that share their
+//     keys (rank r of the pair holds the tile's r-th half), cut out of a
+//     worker's stretch of the line of key blocks (paged.h); the worker is the
+//     pair.  A Q tile is one box of the [tokens][heads_kv][group][128] view,
+//     so its rows land in the order token * group + head.
+//   * K and V come page by page: the boxes of a block are issued by the lanes
+//     of the producer warp, each with its own page from the block table, one
+//     block ahead of their use.
+//   * V rows behind the last key that any row sees are cleared in shared
+//     memory before the product (0 * NaN is no 0): warp 11 of each rank passes
+//     every V stage on to rank 0's PV issuer and clears the item's last one.
+//   * scores are masked in tensor memory before the softmax loads them, so
+//     blocks without a mask run without selects.
+//   * an item that lies in the stretch is normalised and stored; one that a
+//     stretch's end cuts leaves FP32 partial results, joined by
+//     b200_paged_combine_kernel.
+#define B200FA_CAUSAL 1
+#define B200FA_WINDOW 1  // for its masking in tensor memory
+#define s_issuer_role s_issuer_role_paged_unused
+#define pv_issuer_role pv_issuer_role_paged_unused
+#define watch_role watch_role_paged_unused
+#define forward_role forward_role_paged_unused
+#define load_role load_role_paged_unused
+#include "fa_kernel.cuh"
+
+#include "b200fa.h"
+#include "paged.h"
+#include "paged_common.cuh"
+
+namespace b200fa {
+namespace chunk {
+
+// Barrier slots: the dense kernel's, and one per V stage between its landing
+// and its hand-over to the PV issuer.
+constexpr int kBarVLand = kNumBars;            // [kRing] V stage landed, local
+constexpr int kBars = kBarVLand + kRing;
+constexpr int kSmBar = kSmemV + kRing * kStageBytes;
+constexpr int kSmXchg = kSmBar + kBars * 8;             // float [2][128]
+constexpr int kSmTmem = kSmXchg + 2 * kBlockM * 4;      // TMEM base, abort flag
+constexpr int kSmStart = kSmTmem + 16;                  // PagedStart
+constexpr int kSmScan = kSmStart + 64;                  // int64 [12]
+constexpr int kSmUsed = kSmScan + (kThreads / 32) * 8;
+constexpr int kBytes = kSmUsed + 1024;
+static_assert(kBytes <= 232448, "shared memory budget exceeded");
+static_assert(kSmBar % 8 == 0 && kSmStart % 8 == 0 && kSmScan % 8 == 0 && sizeof(PagedStart) <= 64, "layout");
+
+struct Sm {
+  uint32_t base;
+  __device__ __forceinline__ uint32_t bar(int i) const { return base + kSmBar + 8 * i; }
+  __device__ __forceinline__ uint32_t q(int t) const { return base + kSmemQ + t * kQTileBytes; }
+  __device__ __forceinline__ uint32_t k(uint32_t e) const { return base + kSmemK + e * kStageBytes; }
+  __device__ __forceinline__ uint32_t v(uint32_t e) const { return base + kSmemV + e * kStageBytes; }
+  __device__ __forceinline__ uint32_t xchg(uint32_t slot, int row) const { return base + kSmXchg + (slot * kBlockM + uint32_t(row)) * 4u; }
+  __device__ __forceinline__ uint32_t tmem_slot() const { return base + kSmTmem; }
+  __device__ __forceinline__ uint32_t abort_slot() const { return base + kSmTmem + 4; }
+};
+
+__device__ __forceinline__ Sm sm_of(uint8_t* raw) { return Sm{(smem_addr(raw) + 1023u) & ~1023u}; }
+__device__ __forceinline__ const PagedStart* start_of(uint8_t* raw) {
+  return reinterpret_cast<const PagedStart*>(raw + (sm_of(raw).base - smem_addr(raw)) + kSmStart);
+}
+
+// Bounded waits; a wait that runs out raises the abort flag of both CTAs.
+struct Wait {
+  uint32_t abort_slot;
+  const PagedParams* p;
+  __device__ __forceinline__ void fail(uint32_t site) const {
+    st_volatile_shared(abort_slot, 1u);
+    st_cluster_u32(map_shared(abort_slot, cluster_rank() ^ 1u), 1u);
+    paged_status(*p, kDevTimeout, site);
+  }
+  template <bool kCluster = false>
+  __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity, uint32_t site) const {
+    auto test = [&] { return kCluster ? mbar_test_cluster(bar, parity) : mbar_test(bar, parity); };
+    if (test()) return true;
+    const uint64_t t0 = global_timer_ns();
+    while (true) {
+#pragma unroll 1
+      for (int i = 0; i < 16; ++i)
+        if (test()) return true;
+      if (ld_volatile_shared(abort_slot) != 0u) return false;
+      if (global_timer_ns() - t0 > p->timeout_ns) {
+        fail(site);
+        return false;
+      }
+    }
+  }
+  __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity, uint64_t limit_ns) const {
+    const uint64_t t0 = global_timer_ns();
+    while (!mbar_test_cluster(bar, parity))
+      if (global_timer_ns() - t0 > limit_ns) return;
+  }
+};
+
+template <bool kBf16>
+constexpr uint32_t kIdescS = kIdescQK | (kBf16 ? (1u << 7) | (1u << 10) : 0u);
+template <bool kBf16>
+constexpr uint32_t kIdescO = kIdescPV | (kBf16 ? (1u << 7) | (1u << 10) : 0u);
+
+// Rank 0, one thread: S = Q K^T of every block.
+template <bool kBf16>
+__device__ __forceinline__ void s_issuer(const PagedParams& p, const PagedStart& start, const Sm& sm, uint32_t tmem, const Wait& wait) {
+  const uint32_t site = uint32_t(kSIssuerWarp) << 8;
+  uint32_t g = 0;
+  bool ok = true;
+  int it = 0;
+  for (PagedWalk w(p, start); ok && w.more(); w.next(p), ++it) {
+    const int qt = it & 1;
+    const uint64_t q_desc = smem_desc(sm.q(qt));
+    if (!wait(sm.bar(kBarQFull + qt), uint32_t(it >> 1) & 1u, site | uint32_t(kBarQFull + qt))) break;
+    for (int j = 0; j < w.take; ++j, ++g) {
+      const uint32_t b = buf(g), e = ring_entry(g);
+      if ((g >= 2 && !wait(sm.bar(kBarSFree + int(b)), buf_parity(g - 2u), site | uint32_t(kBarSFree + int(b)))) ||
+          !wait(sm.bar(kBarKFull + int(e)), ring_parity(g), site | uint32_t(kBarKFull + int(e)))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint64_t k_desc = smem_desc(sm.k(e));
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk)
+        mma_pair_ss(tmem + kTmemS + 128u * b, q_desc + uint64_t((kk >> 2) * (kQHalfBytes >> 4) + (kk & 3) * 2),
+                    k_desc + uint64_t((kk >> 2) * (kKBoxBytes >> 4) + (kk & 3) * 2), kIdescS<kBf16>, kk > 0 ? 1u : 0u);
+      mma_commit_pair_both(sm.bar(kBarSFull + int(b)));
+      mma_commit_pair_both(sm.bar(kBarKEmpty + int(e)));
+    }
+  }
+  mma_commit_pair(sm.bar(kBarDrain + 0));
+  wait.drain(sm.bar(kBarDrain + 0), 0u, 100000000ull);
+}
+
+// Rank 0, one thread: O += P V of every block, in order.
+template <bool kBf16>
+__device__ __forceinline__ void pv_issuer(const PagedParams& p, const PagedStart& start, const Sm& sm, uint32_t tmem, const Wait& wait) {
+  const uint32_t site = uint32_t(kPVIssuerWarp) << 8;
+  uint32_t g = 0;
+  bool ok = true;
+  for (PagedWalk w(p, start); ok && w.more(); w.next(p)) {
+    for (int j = 0; j < w.take; ++j, ++g) {
+      const uint32_t b = buf(g), e = ring_entry(g);
+      // Cluster scope: rank 1's rows of V may have been cleared by plain stores.
+      if (!wait.operator()<true>(sm.bar(kBarVFull + int(e)), ring_parity(g), site | uint32_t(kBarVFull + int(e))) ||
+          !wait(sm.bar(kBarPFull + int(b)), buf_parity(g), site | uint32_t(kBarPFull + int(b)))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint64_t v_desc = smem_desc(sm.v(e));
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk)
+        mma_pair_ts(tmem + kTmemO, tmem + kTmemP + 64u * b + 8u * uint32_t(kk), v_desc + uint64_t(kk * 128), kIdescO<kBf16>,
+                    kk > 0 || j > 0 ? 1u : 0u);
+      mma_commit_pair_both(sm.bar(kBarPVDone + int(b)));
+      mma_commit_pair_both(sm.bar(kBarVEmpty + int(e)));
+    }
+  }
+  mma_commit_pair(sm.bar(kBarDrain + 1));
+  wait.drain(sm.bar(kBarDrain + 1), 0u, 100000000ull);
+}
+
+// Both ranks, a whole warp: passes rank 1's Q and K stages and both ranks' V
+// stages on to rank 0's barriers, clearing V rows that no row of the item sees.
+__device__ __forceinline__ void forward(const PagedParams& p, const PagedStart& start, const Sm& sm, const Wait& wait,
+                                        uint32_t rank, uint32_t lane) {
+  const uint32_t site = (rank << 16) | (uint32_t(kForwardWarp) << 8);
+  uint32_t g = 0;
+  bool ok = true;
+  int it = 0;
+  // Bounded wait of lane 0 with a warp-uniform outcome.
+  auto landed = [&](int bar, uint32_t parity) -> bool {
+    uint32_t got = 1;
+    if (lane == 0) got = wait(sm.bar(bar), parity, site | uint32_t(bar)) ? 1u : 0u;
+    return __shfl_sync(0xffffffffu, got, 0) != 0u;
+  };
+  auto pass = [&](int bar) {
+    if (lane == 0) mbar_arrive_cluster_relaxed(map_shared(sm.bar(bar), 0));
+  };
+  for (PagedWalk w(p, start); ok && w.more(); w.next(p), ++it) {
+    if (rank == 1) {
+      if (!(ok = landed(kBarQFull + (it & 1), uint32_t(it >> 1) & 1u))) break;
+      pass(kBarQFull + (it & 1));
+    }
+    for (int j = 0; j < w.take; ++j, ++g) {
+      const int e = int(ring_entry(g));
+      if (rank == 1) {
+        if (!(ok = landed(kBarKFull + e, ring_parity(g)))) break;
+        pass(kBarKFull + e);
+      }
+      if (!(ok = landed(kBarVLand + e, ring_parity(g)))) break;
+      const int from = w.blocks.end_key - w.blocks.key_block(w.off + j) * kPagedBlock;
+      if (from < kPagedBlock) {
+        mbar_test(sm.bar(kBarVLand + e), ring_parity(g));  // every lane observes the copy
+        for (int i = int(lane) + (from > 0 ? from : 0) * 8; i < kPagedBlock * 8; i += 32) st_shared_v4(sm.v(uint32_t(e)) + uint32_t(i) * 16u, 0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_shared(sm.bar(kBarVFull + e), 0));
+      } else {
+        pass(kBarVFull + e);
+      }
+    }
+  }
+}
+
+// Both ranks, a whole warp: this CTA's Q tiles and its halves of every block.
+__device__ __forceinline__ void load(const PagedParams& p, const PagedStart& start, const Sm& sm, const Wait& wait,
+                                     uint32_t rank, uint32_t lane) {
+  const uint32_t site = (rank << 16) | (uint32_t(kLoadWarp) << 8);
+  const int half_tok = p.tokens_per_tile / 2;
+  const uint32_t q_bytes = uint32_t(half_tok * p.group) * 256u;
+  const int shift = p.page_shift, size_mask = (1 << shift) - 1;
+  const int k_rows = shift < 6 ? 1 << shift : kPairKeys, v_rows = shift < 7 ? 1 << shift : kPagedBlock;
+  // Lane l: box l of K (half l % 2 of rows k_rows * (l / 2)) and of V; at most 16 each.
+  const int k_boxes = 2 * (kPairKeys / k_rows), v_boxes = kPagedBlock / v_rows;
+  const int k_row = int(lane >> 1) * k_rows, v_row = int(lane) * v_rows;
+  uint32_t g = 0, issued_k = 0, issued_v = 0, q_issued = 0;
+  bool ok = true;
+  int it = 0;
+  auto waited = [&](int bar, uint32_t parity) -> bool {
+    uint32_t got = 1;
+    if (lane == 0) got = wait(sm.bar(bar), parity, site | uint32_t(bar)) ? 1u : 0u;
+    return __shfl_sync(0xffffffffu, got, 0) != 0u;
+  };
+  for (PagedWalk w(p, start); ok && w.more(); w.next(p), ++it) {
+    const int qt = it & 1;
+    if (!(ok = waited(kBarQEmpty + qt, (uint32_t(it >> 1) & 1u) ^ 1u))) break;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(sm.bar(kBarQFull + qt), q_bytes);
+      const int tok = w.req.q0 + w.tile * p.tokens_per_tile + int(rank) * half_tok;
+      tma_load_4d(sm.q(qt), &p.tm_q, sm.bar(kBarQFull + qt), 0, 0, w.h, tok);
+      tma_load_4d(sm.q(qt) + kQHalfBytes, &p.tm_q, sm.bar(kBarQFull + qt), 64, 0, w.h, tok);
+    }
+    ++q_issued;
+    int k_page = p.num_pages, v_page = p.num_pages;
+    auto pages = [&](int j) {
+      const int key0 = w.blocks.key_block(w.off + j) * kPagedBlock;
+      if (int(lane) < k_boxes) k_page = page_of(p, w.r, w.blocks, key0 + int(rank) * kPairKeys + k_row);
+      if (int(lane) < v_boxes) v_page = page_of(p, w.r, w.blocks, key0 + v_row);
+    };
+    pages(0);
+    for (int j = 0; j < w.take; ++j, ++g) {
+      const uint32_t e = ring_entry(g);
+      const int key0 = w.blocks.key_block(w.off + j) * kPagedBlock;
+      const int kp = k_page, vp = v_page;
+      if (j + 1 < w.take) pages(j + 1);
+      if (!(ok = waited(kBarKEmpty + int(e), ring_parity(g) ^ 1u))) break;
+      if (lane == 0) mbar_arrive_expect_tx(sm.bar(kBarKFull + int(e)), kStageBytes);
+      __syncwarp();
+      if (int(lane) < k_boxes)
+        tma_load_4d(sm.k(e) + (lane & 1) * kKBoxBytes + uint32_t(k_row) * 128u, &p.tm_k, sm.bar(kBarKFull + int(e)),
+                    64 * int(lane & 1), (key0 + int(rank) * kPairKeys + k_row) & size_mask, w.h, kp);
+      ++issued_k;
+      if (!(ok = waited(kBarVEmpty + int(e), ring_parity(g) ^ 1u))) break;
+      if (lane == 0) mbar_arrive_expect_tx(sm.bar(kBarVLand + int(e)), kStageBytes);
+      __syncwarp();
+      if (int(lane) < v_boxes)
+        tma_load_4d(sm.v(e) + uint32_t(v_row) * 128u, &p.tm_v, sm.bar(kBarVLand + int(e)), int(rank) * kPairDims,
+                    (key0 + v_row) & size_mask, w.h, vp);
+      ++issued_v;
+    }
+  }
+  // The last copies land before the CTA exits, also when a role gave up.
+  if (lane == 0) {
+    for (uint32_t i = issued_k > kRing ? issued_k - kRing : 0; i < issued_k; ++i)
+      wait.drain(sm.bar(kBarKFull + int(ring_entry(i))), ring_parity(i), 50000000ull);
+    for (uint32_t i = issued_v > kRing ? issued_v - kRing : 0; i < issued_v; ++i)
+      wait.drain(sm.bar(kBarVLand + int(ring_entry(i))), ring_parity(i), 50000000ull);
+    for (uint32_t i = q_issued > 2 ? q_issued - 2 : 0; i < q_issued; ++i)
+      wait.drain(sm.bar(kBarQFull + int(i & 1u)), (i >> 1) & 1u, 50000000ull);
+  }
+  __syncwarp();
+}
+
+// Exponentials of 64 keys of one row (fa_kernel.cuh's exp_keys with FP32 sums
+// and P in the cache's type): of every 8 pairs one through the polynomial.
+template <bool kBf16>
+__device__ __forceinline__ void exp64(const uint32_t* r, uint64_t sl2x2, uint64_t nmx2, uint32_t* pk, uint64_t* acc) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), sl2x2, nmx2);
+    uint64_t p2;
+    float a, b;
+    if ((i & 7) == 7) {
+      p2 = exp2_poly2(x2);
+    } else {
+      f2_unpack(x2, a, b);
+      p2 = f2_pack(ex2_approx(a), ex2_approx(b));
+    }
+    f2_unpack(p2, a, b);
+    pk[i] = pack2<kBf16>(a, b);
+    acc[i & 3] = f2_add(acc[i & 3], p2);
+  }
+}
+
+// The softmax of the CTA's half tile: group grp takes the item's blocks j with
+// j % 2 == grp, one thread per row; fa_kernel.cuh's softmax_role on the walk.
+template <bool kBf16>
+__device__ __forceinline__ void softmax(const PagedParams& p, const PagedStart& start, const Sm& sm, uint32_t tmem,
+                                        const Wait& wait, uint32_t warp, uint32_t lane, uint32_t rank) {
+  const int grp = int(warp >> 2);
+  const int row = int(warp & 3) * 32 + int(lane);
+  const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
+  const uint32_t tO = tmem + lane_off + kTmemO;
+  const uint32_t site = (rank << 16) | (warp << 8);
+  const float sl2 = p.scale_log2;
+  const uint64_t sl2x2 = f2_pack(sl2, sl2);
+  const int half_tok = p.tokens_per_tile / 2;
+  const int row_tok = row / p.group + int(rank) * half_tok;  // this row's token in the tile
+  constexpr float kFirstRef = -1e30f;  // finite: a row may see nothing of its first blocks
+  auto arrive_rank0 = [&](int bar) {
+    __syncwarp();
+    if (lane == 0) {
+      if (rank == 0) mbar_arrive(sm.bar(bar));
+      else mbar_arrive_cluster_relaxed(map_shared(sm.bar(bar), 0));
+    }
+  };
+  auto arrive_local = [&](int bar) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(sm.bar(bar));
+  };
+  auto wait_warp = [&](int bar, uint32_t parity) -> bool {
+    return __all_sync(0xffffffffu, wait(sm.bar(bar), parity, site | uint32_t(bar)));
+  };
+  auto wait_pv = [&](uint32_t gp) -> bool { return wait_warp(kBarPVDone + int(buf(gp)), buf_parity(gp)); };
+  bool ok = true;
+  uint32_t g0 = 0;
+  int it = 0;
+  for (PagedWalk w(p, start); ok && w.more(); w.next(p), ++it) {
+    const int n = w.take;
+    const int pos = w.blocks.pos0 + row_tok;
+    float m_cur = kFirstRef, l_g = 0.f;
+    for (int j = grp; j < n; j += 2) {
+      const uint32_t gb = g0 + uint32_t(j);
+      const uint32_t b = buf(gb);
+      const uint32_t tS = tmem + lane_off + kTmemS + 128u * b;
+      const uint32_t tP = tmem + lane_off + kTmemP + 64u * b;
+      float m_prev = kFirstRef;
+      if (!wait_warp(kBarSFull + int(b), buf_parity(gb))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      {
+        const int key0 = w.blocks.key_block(w.off + j) * kPagedBlock;
+        const int valid = pos + 1 - key0;
+        const int lo = p.window > 0 ? valid - p.window : 0, sink = p.sinks - key0;
+        if (__any_sync(0xffffffffu, valid < kPagedBlock || (lo > 0 && sink < lo))) mask_window(tS, valid, lo, sink);
+      }
+      uint32_t r[kBlockN];
+      tmem_ld32(tS, r);
+      tmem_ld32(tS + 32u, r + 32);
+      tmem_ld32(tS + 64u, r + 64);
+      tmem_ld32(tS + 96u, r + 96);
+      if (gb > 0) {
+        if (!wait_warp(kBarRef + int((gb - 1u) & 1u), ((gb - 1u) >> 1) & 1u)) {
+          tmem_wait_ld();
+          ok = false;
+          break;
+        }
+        if (j > 0) m_prev = ld_shared_f32(sm.xchg((gb - 1u) & 1u, row));
+      }
+      tmem_wait_ld();
+      arrive_rank0(kBarSFree + int(b));
+      const float mx = fmaxf(row_max64(r), row_max64(r + 64)) * sl2;
+      if (j >= 2 && m_prev != m_cur) l_g *= ex2_approx(m_cur - m_prev);
+      float m_new = m_prev, alpha = 1.f;
+      bool moved = false;
+      if (mx > m_prev + kRescaleLog2) {
+        m_new = mx;
+        moved = j > 0;
+        alpha = ex2_approx(m_prev - mx);
+      }
+      st_shared_f32(sm.xchg(gb & 1u, row), m_new);
+      arrive_local(kBarRef + int(gb & 1u));
+      if (moved) l_g *= alpha;
+      m_cur = m_new;
+      uint32_t pk[kBlockN / 2];
+      uint64_t acc[4] = {0ull, 0ull, 0ull, 0ull};
+      const uint64_t nm = f2_pack(-m_new, -m_new);
+      exp64<kBf16>(r, sl2x2, nm, pk, acc);
+      exp64<kBf16>(r + 64, sl2x2, nm, pk + 32, acc);
+      if (__any_sync(0xffffffffu, moved)) {
+        if (!wait_pv(gb - 1u)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        scale_o_row(tO, moved ? alpha : 1.f);
+      }
+      float a0, b0, a1, b1;
+      f2_unpack(f2_add(acc[0], acc[2]), a0, b0);
+      f2_unpack(f2_add(acc[1], acc[3]), a1, b1);
+      l_g += (a0 + b0) + (a1 + b1);
+      if (gb >= 2 && !wait_pv(gb - 2u)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      tmem_st32(tP, pk);
+      tmem_st32(tP + 32u, pk + 32);
+      tmem_wait_st();
+      tc_fence_before();
+      // The item's first product overwrites O: both groups have read the last
+      // item's by then.
+      if (j == 0 && it > 0 && warp == 0 && !wait_warp(kBarOStaged, uint32_t(it - 1) & 1u)) {
+        ok = false;
+        break;
+      }
+      arrive_rank0(kBarPFull + int(b));
+    }
+    if (!ok) break;
+
+    // ---- the item's end: the row's sum, then O
+    const uint32_t g_last = g0 + uint32_t(n) - 1u;
+    g0 += uint32_t(n);
+    if (!wait_pv(g_last)) {
+      ok = false;
+      break;
+    }
+    tc_fence_after();
+    float m_final = m_cur;
+    if ((n - 1) % 2 != grp) {
+      if (!wait_warp(kBarRef + int(g_last & 1u), (g_last >> 1) & 1u)) {
+        ok = false;
+        break;
+      }
+      m_final = ld_shared_f32(sm.xchg(g_last & 1u, row));
+    }
+    if (l_g != 0.f && m_final != m_cur) l_g *= ex2_approx(m_cur - m_final);
+    arrive_local(kBarXchg);
+    if (!wait_warp(kBarXchg, 0u)) {
+      ok = false;
+      break;
+    }
+    const uint32_t mine = grp == 0 ? (g_last & 1u) : ((g_last + 1u) & 1u);
+    st_shared_f32(sm.xchg(mine, row), l_g);
+    arrive_local(kBarXchg);
+    if (!wait_warp(kBarXchg, 1u)) {
+      ok = false;
+      break;
+    }
+    // Every product of the item is done: its Q tile is free.
+    if (warp == 0 && lane == 0) mbar_arrive(sm.bar(kBarQEmpty + (it & 1)));
+    // A row that saw no key kept the floor as its reference (masked keys of the
+    // polynomial's share count 2^-120 each, so its sum is not quite 0).
+    const float l = m_final > 0.5f * kFirstRef ? l_g + ld_shared_f32(sm.xchg(mine ^ 1u, row)) : 0.f;
+    const int t0 = w.tile * p.tokens_per_tile;
+    const int toks = w.req.len - t0 < p.tokens_per_tile ? w.req.len - t0 : p.tokens_per_tile;
+    const bool real = row < half_tok * p.group && row_tok < toks;
+    if (w.begins() && w.ends()) {
+      const float inv_l = l > 0.f ? 1.f / l : 0.f;
+      uint16_t* dst = static_cast<uint16_t*>(p.o) + int64_t(w.req.q0 + t0 + row_tok) * p.o_tok +
+                      int64_t(w.h * p.group + row % p.group) * p.o_head + 64 * grp;
+#pragma unroll 1
+      for (int c = 0; c < 2; ++c) {
+        uint32_t o[32];
+        tmem_ld32(tO + 64u * uint32_t(grp) + 32u * uint32_t(c), o);
+        tmem_wait_ld();
+        if (real) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            uint32_t h[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              h[i] = pack2<kBf16>(__uint_as_float(o[8 * u + 2 * i]) * inv_l, __uint_as_float(o[8 * u + 2 * i + 1]) * inv_l);
+            *reinterpret_cast<uint4*>(dst + 32 * c + 8 * u) = make_uint4(h[0], h[1], h[2], h[3]);
+          }
+        }
+      }
+    } else {
+      const int worker = int(cluster_id_x());
+      float* part = paged_partial(p, 2 * worker + (w.begins() ? 1 : 0));
+      const int prow = row + int(rank) * half_tok * p.group;  // token * group + head in the tile
+      float* dst = part + prow * 128 + 64 * grp;
+#pragma unroll 1
+      for (int c = 0; c < 2; ++c) {
+        uint32_t o[32];
+        tmem_ld32(tO + 64u * uint32_t(grp) + 32u * uint32_t(c), o);
+        tmem_wait_ld();
+        if (real) {
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            *reinterpret_cast<float4*>(dst + 32 * c + 4 * u) =
+                make_float4(__uint_as_float(o[4 * u]), __uint_as_float(o[4 * u + 1]), __uint_as_float(o[4 * u + 2]),
+                            __uint_as_float(o[4 * u + 3]));
+        }
+      }
+      if (real && grp == 0) {
+        part[p.part_rows * 128 + prow] = m_final;
+        part[p.part_rows * 129 + prow] = l;
+      }
+      if (w.begins() && rank == 0 && warp == 0 && lane == 0)
+        *paged_record(p, worker) = PagedRecord{paged_parts(start, worker, w.blocks.n - (w.off + w.take)), w.req.q0 + t0, toks, w.h, {0, 0, 0, 0}};
+    }
+    tc_fence_before();
+    arrive_local(kBarOStaged);
+  }
+}
+
+__device__ __forceinline__ void setup(const PagedParams& p, uint8_t* raw) {
+  const Sm sm = sm_of(raw);
+  uint8_t* smem = raw + (sm.base - smem_addr(raw));
+  const uint32_t tid = tid_x();
+  const uint32_t rank = cluster_rank();
+  if (tid == 0) {
+    const uint32_t fed = rank == 0 ? 2u : 1u;  // rank 0's full barriers also count rank 1's forward
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(sm.bar(kBarQFull + t), fed);
+      mbar_init(sm.bar(kBarQEmpty + t), 1);
+      mbar_init(sm.bar(kBarSFull + t), 1);
+      mbar_init(sm.bar(kBarSFree + t), kGroupWarps);
+      mbar_init(sm.bar(kBarPFull + t), kGroupWarps);
+      mbar_init(sm.bar(kBarPVDone + t), 1);
+      mbar_init(sm.bar(kBarRef + t), 4);
+      mbar_init(sm.bar(kBarDrain + t), 1);
+    }
+    mbar_init(sm.bar(kBarXchg), 8);
+    mbar_init(sm.bar(kBarOStaged), 8);
+    for (int e = 0; e < kRing; ++e) {
+      mbar_init(sm.bar(kBarKFull + e), fed);
+      mbar_init(sm.bar(kBarKEmpty + e), 1);
+      mbar_init(sm.bar(kBarVFull + e), 2);  // rank 0: both ranks' hand-overs
+      mbar_init(sm.bar(kBarVEmpty + e), 1);
+      mbar_init(sm.bar(kBarVLand + e), 1);
+    }
+    st_volatile_shared(sm.abort_slot(), 0u);
+    fence_mbarrier_init();
+    tma_prefetch_map(&p.tm_q);
+    tma_prefetch_map(&p.tm_k);
+    tma_prefetch_map(&p.tm_v);
+    if (rank == 0) paged_record(p, int(cluster_id_x()))->parts = 0;
+  }
+  // Rows of a Q tile that no box covers stay zeros.
+  for (uint32_t i = tid; i < 2 * kQTileBytes / 16; i += kThreads) st_shared_v4(sm.base + kSmemQ + i * 16u, 0, 0, 0, 0);
+  fence_proxy_async_smem();
+  find_start(p, int(cluster_id_x()), reinterpret_cast<int64_t*>(smem + kSmScan), reinterpret_cast<PagedStart*>(smem + kSmStart));
+  if ((tid >> 5) == 0) {
+    __syncwarp();
+    tmem_alloc_pair(sm.tmem_slot(), kTmemCols);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+}
+
+template <bool kBf16>
+__device__ __forceinline__ void roles(const PagedParams& p, uint8_t* raw) {
+  const Sm sm = sm_of(raw);
+  const uint32_t tid = tid_x();
+  const uint32_t warp = tid >> 5, lane = tid & 31u;
+  if (warp < 8) {
+    regs_increase<kSoftmaxRegs>();
+    softmax<kBf16>(p, *start_of(raw), sm, ld_volatile_shared(sm.tmem_slot()), Wait{sm.abort_slot(), &p}, warp, lane, cluster_rank());
+  } else {
+    regs_decrease<kControlRegs>();
+    const uint32_t rank = cluster_rank();
+    const Wait wait{sm.abort_slot(), &p};
+    const PagedStart& start = *start_of(raw);
+    if (warp == kLoadWarp) {
+      load(p, start, sm, wait, rank, lane);
+    } else if (warp == kForwardWarp) {
+      forward(p, start, sm, wait, rank, lane);
+    } else if (rank == 0 && lane == 0) {
+      const uint32_t tmem = ld_volatile_shared(sm.tmem_slot());
+      if (warp == kSIssuerWarp) s_issuer<kBf16>(p, start, sm, tmem, wait);
+      else pv_issuer<kBf16>(p, start, sm, tmem, wait);
+    }
+  }
+  __syncwarp();
+}
+
+__device__ __forceinline__ void teardown(uint8_t* raw) {
+  const Sm sm = sm_of(raw);
+  tc_fence_before();
+  cluster_sync();
+  if ((tid_x() >> 5) == 0) {
+    tc_fence_after();
+    tmem_dealloc_pair(ld_volatile_shared(sm.tmem_slot()), kTmemCols);
+  }
+}
+
+}  // namespace chunk
+}  // namespace b200fa
+
+using namespace b200fa;
+
+#define B200FA_PAGED_CHUNK_KERNEL(name, bf16)                                                                  \
+  __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) name(const __grid_constant__ PagedParams p) { \
+    extern __shared__ uint8_t smem_raw[];                                                                      \
+    chunk::setup(p, smem_raw);                                                                                 \
+    chunk::roles<bf16>(p, smem_raw);                                                                           \
+    chunk::teardown(smem_raw);                                                                                 \
+  }
+B200FA_PAGED_CHUNK_KERNEL(b200_paged_chunk_fp16_kernel, false)
+B200FA_PAGED_CHUNK_KERNEL(b200_paged_chunk_bf16_kernel, true)
+
+namespace b200fa {
+
+PagedChunkKernel paged_chunk_kernel(bool bf16) { return bf16 ? b200_paged_chunk_bf16_kernel : b200_paged_chunk_fp16_kernel; }
+
+int paged_chunk_setup(int* pairs) {
+  cudaError_t e = cudaSuccess;
+  for (bool bf16 : {false, true})
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_chunk_kernel(bf16), cudaFuncAttributeMaxDynamicSharedMemorySize, chunk::kBytes);
+  if (e != cudaSuccess) return int(e);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(2, 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = chunk::kBytes;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaOccupancyMaxActiveClusters(pairs, b200_paged_chunk_fp16_kernel, &cfg);
+  if (e == cudaSuccess && *pairs < 1) e = cudaErrorInvalidConfiguration;
+  return int(e);
+}
+
+int paged_chunk_launch(const PagedParams& p, bool bf16, cudaStream_t stream) {
+  paged_chunk_kernel(bf16)<<<2 * p.workers, kThreads, chunk::kBytes, stream>>>(p);
+  return int(cudaGetLastError());
+}
+
+}  // namespace b200fa

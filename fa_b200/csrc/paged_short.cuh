@@ -16,6 +16,7 @@
 
 #include "b200fa.h"
 #include "paged.h"
+#include "paged_common.cuh"
 #include "ptx.cuh"
 
 namespace b200fa {
@@ -37,15 +38,6 @@ constexpr int kSmStart = kSmScan + (kShortThreads / 32) * 8;
 constexpr int kSmAbort = kSmStart + 48;
 constexpr int kShortSmemBytes = kSmAbort + 16 + 1024;
 static_assert(sizeof(PagedStart) <= 48 && kShortSmemBytes <= 232448, "shared memory budget");
-
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y,
-                                            int32_t z, int32_t w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
-      : "memory");
-}
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -75,18 +67,6 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Two floats rounded to the cache's type (lo in bits 0..15).
-template <bool kBf16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (kBf16) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-  } else {
-    return pack_h2(lo, hi);
-  }
-}
-
 // Bounded wait of one thread; false when the block gave up.
 __device__ __forceinline__ bool paged_wait(const PagedParams& p, uint32_t bar, uint32_t parity, uint32_t abort_slot,
                                            uint32_t site) {
@@ -103,18 +83,6 @@ __device__ __forceinline__ bool paged_wait(const PagedParams& p, uint32_t bar, u
       return false;
     }
   }
-}
-
-// The page that holds key `key` of request r, for a load: num_pages (outside
-// the tensor, so the copy delivers zeros) where no row of the tile sees any
-// of the page's keys, or where the table names no page of the cache.
-__device__ __forceinline__ int page_of(const PagedParams& p, int r, const PagedBlocks& b, int key) {
-  const int size = 1 << p.page_shift, page = key >> p.page_shift, k0 = page << p.page_shift;
-  if (k0 >= b.end_key || (k0 + size <= b.first_key && k0 >= p.sinks)) return p.num_pages;
-  const int id = page < p.width ? p.table[int64_t(r) * p.table_stride + page] : -1;
-  if (id >= 0 && id < p.num_pages) return id;
-  paged_status(p, B200FA_DEV_PAGE, uint32_t(r));
-  return p.num_pages;
 }
 
 // The producer warp: K and V of every block of the worker's stretch.  The
@@ -148,9 +116,8 @@ __device__ __forceinline__ void short_load(const PagedParams& p, const PagedStar
       }
     }
   }
-  // Copies in flight must land before the block exits (only after an abort:
-  // otherwise the consumers waited for each of them).
-  if (!ok && lane == 0) {
+  // The last copies land before the block exits, also when a warp gave up.
+  if (lane == 0) {
     const uint64_t t0 = global_timer_ns();
     const uint32_t first = g > kShortRing ? g - kShortRing : 0;
     for (uint32_t i = first; i < g; ++i)
