@@ -58,9 +58,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // Causal-mask kernels, defined in b200fa_causal.cu (B200FA_FLAG_CAUSAL).
 __global__ void b200_fa_fp16_causal_kernel(const __grid_constant__ FwdParams p);
 __global__ void b200_fa_fp32_causal_kernel(const __grid_constant__ FwdParams p);
-// Sliding-window kernels, defined in b200fa_window.cu (B200FA_FLAG_WINDOW).
-__global__ void b200_fa_fp16_window_kernel(const __grid_constant__ FwdParams p);
-__global__ void b200_fa_fp32_window_kernel(const __grid_constant__ FwdParams p);
+// Sliding-window kernel of both variants, defined in b200fa_window.cu (B200FA_FLAG_WINDOW).
+__global__ void b200_fa_window_kernel(const __grid_constant__ FwdParams p);
 
 // Test hook (b200fa_test_exp2): the softmax's two exponential forms on an
 // array, pairwise as the softmax evaluates them -- exp2_poly2 (FMA pipe) into
@@ -83,7 +82,7 @@ __global__ void __launch_bounds__(256) exp2_probe_kernel(const float* x, float* 
 using KernelFn = void (*)(FwdParams);
 
 KernelFn kernel_for(int variant, bool capture, bool causal, bool window = false) {
-  if (window) return variant == B200FA_VARIANT_FP16 ? b200_fa_fp16_window_kernel : b200_fa_fp32_window_kernel;
+  if (window) return b200_fa_window_kernel;
   if (capture) return variant == B200FA_VARIANT_FP16 ? b200_fa_fp16_capture_kernel : b200_fa_fp32_capture_kernel;
   if (causal) return variant == B200FA_VARIANT_FP16 ? b200_fa_fp16_causal_kernel : b200_fa_fp32_causal_kernel;
   return variant == B200FA_VARIANT_FP16 ? b200_fa_fp16_kernel : b200_fa_fp32_kernel;
@@ -318,6 +317,7 @@ int fill_params(const void* q, const void* k, const void* v, void* o, int64_t B,
   p->heads = int32_t(B * Hq);
   p->nq = int32_t(Nq);
   if (opts.flags & B200FA_FLAG_WINDOW) {
+    p->o = static_cast<__half*>(o);
     p->window = opts.window;
     p->sinks = opts.sinks < Nk ? opts.sinks : int32_t(Nk);
   }

@@ -5,6 +5,9 @@
 // window and not of the sequence.  Launched by b200fa.cu.
 #define B200FA_CAUSAL 1
 #define B200FA_WINDOW 1
+#ifndef B200FA_POLY_PAIRS_FP32
+#define B200FA_POLY_PAIRS_FP32 0  // all exponentials through MUFU
+#endif
 // The roles that are plain (non-template) device functions get their own
 // names here, as in the causal translation unit.
 #define s_issuer_role s_issuer_role_window
@@ -16,12 +19,8 @@
 
 using namespace b200fa;
 
+// One kernel for both variants: FP32 softmax statistics and sums, P in FP16.
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    b200_fa_fp16_window_kernel(const __grid_constant__ FwdParams p) {
-  attention_fwd_body<0, false>(p);
-}
-
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    b200_fa_fp32_window_kernel(const __grid_constant__ FwdParams p) {
+    b200_fa_window_kernel(const __grid_constant__ FwdParams p) {
   attention_fwd_body<1, false>(p);
 }

@@ -78,6 +78,7 @@
 #pragma once
 #include <cstdint>
 #include <cuda.h>
+#include <cuda_fp16.h>
 #include "ptx.cuh"
 
 // B200FA_CAUSAL = 1: this translation unit's kernels apply the causal mask
@@ -251,6 +252,7 @@ struct FwdParams {
   float* capture;           // capture kernels: [4][heads][n_kv][nq] + [heads][n_kv][nq][128] FP32
   int32_t heads;            // B * Hq
   int32_t nq;               // query rows per head
+  __half* o;                // window kernel: the output, [heads][nq][128]
   int32_t window, sinks;    // window kernels: keys behind a row that stay visible, first keys that always do
 };
 
@@ -931,6 +933,7 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
     int qrow_g;
 #if B200FA_WINDOW
     WindowBlocks blocks;
+    int first_row;
 #endif
     {
       int bh_i, qb_i, cnt_i;
@@ -938,10 +941,20 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
       qrow_g = (qb_i + (int(rank) < cnt_i ? int(rank) : cnt_i - 1)) * kBlockM + row;
 #if B200FA_WINDOW
       blocks = window_blocks(p, qb_i, cnt_i);
+      first_row = qrow_g - row;
 #endif
     }
 #else
     const uint32_t g0 = uint32_t(it) * uint32_t(n);  // the CTA's block count before this item
+#endif
+#if B200FA_WINDOW
+    // Key blocks that some row of this CTA does not see in full: from its first
+    // row's diagonal, or a short last key block, on, and up to the end of its
+    // last row's window.
+    int kb_hi = first_row / kBlockN;
+    if (p.nk_tail < kBlockN && p.n_kv - 1 < kb_hi) kb_hi = p.n_kv - 1;
+    const int behind = first_row + (kBlockM - 1) - p.window;
+    const int kb_lo = behind >= 0 ? behind / kBlockN : -1;
 #endif
     float m_cur = -INFINITY;  // reference of this group's last block (log2 domain)
     float l_g = 0.f;          // this group's row sum over its blocks, relative to m_cur
@@ -1007,7 +1020,7 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
       if (ahead + 1 < valid) valid = ahead + 1;
       const int lo = ahead - p.window + 1;
       const int sink = p.sinks - kb * kBlockN;
-      if (__any_sync(0xffffffffu, valid < kBlockN || (lo > 0 && sink < lo))) mask_window(tS, valid, lo, sink);
+      if (kb >= kb_hi || kb <= kb_lo) mask_window(tS, valid, lo, sink);
 #elif B200FA_CAUSAL
       // Valid keys of the block for this row: the last block's key count
       // and the keys up to the row.
@@ -1020,7 +1033,7 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
       // The scores: one 128-column load in the FP16 kernel, four 32-column
       // loads in the FP32 kernel (each measured the faster for its kernel).
       uint32_t r[kBlockN];
-      if constexpr (kVariant == 0) {
+      if constexpr (kVariant == 0 || B200FA_WINDOW) {
         tmem_ld128(tS, r);
       } else {
         tmem_ld32(tS, r);
@@ -1127,6 +1140,14 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
       tmem_wait_st();
       tl.mark(int(warp), j, 5);
       tc_fence_before();
+#if B200FA_WINDOW
+      // The item's first product overwrites O: both groups have read the last
+      // item's by then.
+      if (j == 0 && it > 0 && warp == 0 && !wait_warp(kBarOStaged, uint32_t(it - 1) & 1u)) {
+        ok = false;
+        break;
+      }
+#endif
       if (!(withhold && it == 0 && j == 1)) arrive_rank0(kBarPFull + int(b));
       if constexpr (kLateSum) l_g += fp16_row_sum64(pk) + fp16_row_sum64(pk + 32);
       ++blocks_done;
@@ -1134,6 +1155,59 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
     }
     if (!ok) break;
 
+#if B200FA_WINDOW
+    // ---- epilogue of short items: the groups' sums meet in the item's Q tile,
+    // which nothing reads any more (a group here has seen, or waited for the
+    // reference after, the scores of the last block), while the last product of
+    // P and V is under way; O / l goes to global memory from the registers.
+    const uint32_t g_last = g0 + uint32_t(n) - 1u;
+    float m_final = m_cur;
+    if ((n - 1) % 2 != grp) {
+      if (!wait_warp(kBarRef + int(g_last & 1u), (g_last >> 1) & 1u)) {
+        ok = false;
+        break;
+      }
+      m_final = ld_shared_f32(sm.xchg(g_last & 1u, row));
+    }
+    if (l_g != 0.f && m_final != m_cur) l_g *= ex2_approx(m_cur - m_final);
+    const uint32_t sums = sm.q(it & 1) + uint32_t(row) * 4u;
+    st_shared_f32(sums + uint32_t(grp) * 512u, l_g);
+    arrive_local(kBarXchg);
+    if (!wait_warp(kBarXchg, uint32_t(it) & 1u)) { ok = false; break; }
+    const float l = l_g + ld_shared_f32(sums + uint32_t(grp ^ 1) * 512u);
+    const float inv_l = l > 0.f ? 1.f / l : 0.f;  // a row that sees no key: zeros
+    fence_proxy_async_smem();
+    arrive_local(kBarQEmpty + (it & 1));
+    if (!wait_pv(g_last)) { ok = false; break; }
+    tc_fence_after();
+    {
+      int bh, qb, cnt;
+      plan_decode<int>(p.nqb, p.unit_begin, p.unit_end, item, bh, qb, cnt);
+      const int orow = (qb + int(rank)) * kBlockM + row;
+      const bool stored = int(rank) < cnt && orow < p.nq &&
+                          w.check(bh >= 0 && bh < p.heads && orow >= 0, site | (kCheckSite + 4u));
+      uint4* dst = reinterpret_cast<uint4*>(p.o + (size_t(bh) * size_t(p.nq) + size_t(orow)) * kHeadDim + 64 * grp);
+#pragma unroll 1
+      for (int c = 0; c < 2; ++c) {
+        uint32_t o[32];
+        tmem_ld32(tO + 64u * uint32_t(grp) + 32u * uint32_t(c), o);
+        tmem_wait_ld();
+        if (stored) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            uint32_t h[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              h[i] = pack_h2(__uint_as_float(o[8 * u + 2 * i]) * inv_l, __uint_as_float(o[8 * u + 2 * i + 1]) * inv_l);
+            dst[4 * c + u] = make_uint4(h[0], h[1], h[2], h[3]);
+          }
+        }
+      }
+    }
+    tc_fence_before();
+    arrive_local(kBarOStaged);
+  }
+#else
     // ---- epilogue: O / l -> FP16 -> swizzled smem (this item's Q tile) -> TMA store.
     // Group grp converts head-dim columns [64 grp, +64) of its rows.
     const int qt = it & 1;
@@ -1164,11 +1238,7 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
     arrive_local(kBarXchg);
     if (!wait_warp(kBarXchg, 1u)) { ok = false; break; }
     const float l = l_g + ld_shared_f32(sm.xchg(mine ^ 1u, row));
-#if B200FA_WINDOW
-    const float inv_l = l > 0.f ? 1.f / l : 0.f;  // a row that sees no key: zeros
-#else
     const float inv_l = 1.f / l;
-#endif
 #pragma unroll 1
     for (int c = 0; c < 2; ++c) {
       uint32_t o[32];
@@ -1212,6 +1282,7 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
     ok = __all_sync(0xffffffffu, ok);
   }
   if (warp == 0 && lane == 0) bulk_wait_group0();
+#endif
   if constexpr (kDebug) {
     if (wq == 0 && lane == 0) st_volatile_shared(sm.count_slot(4 + grp), blocks_done);
   }
@@ -1234,7 +1305,7 @@ __device__ __forceinline__ void setup_phase(const FwdParams& p, uint8_t* smem_ra
     const uint32_t fed = rank == 0 ? 2u : 1u;  // rank 0's full barriers also count rank 1's forward
     for (int t = 0; t < 2; ++t) {
       mbar_init(sm.bar(kBarQFull + t), fed);
-      mbar_init(sm.bar(kBarQEmpty + t), 1);
+      mbar_init(sm.bar(kBarQEmpty + t), B200FA_WINDOW ? 8 : 1);
       mbar_init(sm.bar(kBarSFull + t), 1);
       mbar_init(sm.bar(kBarSFree + t), kGroupWarps);
       mbar_init(sm.bar(kBarPFull + t), kGroupWarps);
@@ -1295,7 +1366,11 @@ __device__ __forceinline__ void role_phase(const FwdParams& p, uint8_t* smem_raw
   } else {
     regs_decrease<kControlRegs>();
     const uint32_t rank = cluster_rank();
+#if B200FA_WINDOW
+    if (elect_one()) {
+#else
     if (lane == 0) {
+#endif
       const uint32_t tmem_base = ld_volatile_shared(sm.tmem_slot());
       const Waiter w = waiter_of(p, sm);
       if (rank == 0 && warp == kSIssuerWarp) s_issuer_role(p, sm, tmem_base, w);

@@ -108,12 +108,13 @@ uint64_t workspace_bytes(const PagedDevice& d) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-int encode(CUtensorMap* map, const b200fa_paged_args& a, const void* ptr, const cuuint64_t (&dims)[4],
-           const cuuint64_t (&strides)[3], const cuuint32_t (&box)[4], const char* what) {
+template <int kDims>
+int encode(CUtensorMap* map, const b200fa_paged_args& a, const void* ptr, const cuuint64_t (&dims)[kDims],
+           const cuuint64_t (&strides)[kDims - 1], const cuuint32_t (&box)[kDims], const char* what) {
   PFN_cuTensorMapEncodeTiled_v12000 fn = encode_fn();
   if (!fn) return fail(B200FA_ERR_NO_DRIVER, "cuTensorMapEncodeTiled is not available from the driver");
-  const cuuint32_t one[4] = {1, 1, 1, 1};
-  const CUresult r = fn(map, a.dtype == B200FA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+  const cuuint32_t one[5] = {1, 1, 1, 1, 1};
+  const CUresult r = fn(map, a.dtype == B200FA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, kDims,
                         const_cast<void*>(ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(B200FA_ERR_TENSOR_MAP, "cuTensorMapEncodeTiled failed for %s (%d)", what, int(r));
@@ -123,16 +124,23 @@ int encode(CUtensorMap* map, const b200fa_paged_args& a, const void* ptr, const 
 // Byte stride of a dimension; one of a single element has no stride of its own.
 cuuint64_t stride_of(int64_t count, int64_t stride) { return cuuint64_t(count > 1 ? stride : 128) * 2; }
 
-// Boxes of 64 columns and up to `rows` tokens of a page.
+// Boxes of 64 columns and up to `rows` tokens of a page ...
 int encode_pages(CUtensorMap* map, const b200fa_paged_args& a, const void* ptr, const int64_t* s, int rows, const char* what) {
-  return encode(map, a, ptr, {128, cuuint64_t(a.page_size), cuuint64_t(a.heads_kv), cuuint64_t(a.num_pages)},
-                {stride_of(a.page_size, s[1]), stride_of(a.heads_kv, s[2]), stride_of(a.num_pages, s[0])},
-                {64, cuuint32_t(a.page_size < rows ? a.page_size : rows), 1, 1}, what);
+  return encode<4>(map, a, ptr, {128, cuuint64_t(a.page_size), cuuint64_t(a.heads_kv), cuuint64_t(a.num_pages)},
+                   {stride_of(a.page_size, s[1]), stride_of(a.heads_kv, s[2]), stride_of(a.num_pages, s[0])},
+                   {64, cuuint32_t(a.page_size < rows ? a.page_size : rows), 1, 1}, what);
+}
+
+// ... and of both halves of up to 128 tokens.
+int encode_halves(CUtensorMap* map, const b200fa_paged_args& a, const void* ptr, const int64_t* s, const char* what) {
+  return encode<5>(map, a, ptr, {64, cuuint64_t(a.page_size), 2, cuuint64_t(a.heads_kv), cuuint64_t(a.num_pages)},
+                   {stride_of(a.page_size, s[1]), 128, stride_of(a.heads_kv, s[2]), stride_of(a.num_pages, s[0])},
+                   {64, cuuint32_t(a.page_size < kPagedBlock ? a.page_size : kPagedBlock), 2, 1, 1}, what);
 }
 
 // Boxes of 64 columns of the group's heads of `tokens` tokens.
 int encode_q(CUtensorMap* map, const b200fa_paged_args& a, int32_t group, int32_t tokens) {
-  return encode(map, a, a.q, {128, cuuint64_t(group), cuuint64_t(a.heads_kv), cuuint64_t(a.tokens)},
+  return encode<4>(map, a, a.q, {128, cuuint64_t(group), cuuint64_t(a.heads_kv), cuuint64_t(a.tokens)},
                 {stride_of(group, a.q_strides[1]), stride_of(a.heads_kv, a.q_strides[1] * group), stride_of(a.tokens, a.q_strides[0])},
                 {64, cuuint32_t(group), 1, cuuint32_t(tokens)}, "q");
 }
@@ -206,8 +214,13 @@ int b200fa_paged_fwd(const b200fa_paged_args* args, void* stream) {
 
   PagedParams p;
   std::memset(&p, 0, sizeof(p));
-  if ((rc = encode_pages(&p.tm_k, a, a.k_pages, a.k_strides, chunk ? kPagedBlock / 2 : kPagedBlock, "k_pages")) != B200FA_OK) return rc;
-  if ((rc = encode_pages(&p.tm_v, a, a.v_pages, a.v_strides, kPagedBlock, "v_pages")) != B200FA_OK) return rc;
+  if (chunk) {  // K: each CTA of a pair loads its half of a block's keys; V: its half of the columns
+    if ((rc = encode_pages(&p.tm_k, a, a.k_pages, a.k_strides, kPagedBlock / 2, "k_pages")) != B200FA_OK) return rc;
+    if ((rc = encode_pages(&p.tm_v, a, a.v_pages, a.v_strides, kPagedBlock, "v_pages")) != B200FA_OK) return rc;
+  } else {
+    if ((rc = encode_halves(&p.tm_k, a, a.k_pages, a.k_strides, "k_pages")) != B200FA_OK) return rc;
+    if ((rc = encode_halves(&p.tm_v, a, a.v_pages, a.v_strides, "v_pages")) != B200FA_OK) return rc;
+  }
   p.q = a.q;
   p.o = a.o;
   p.q_tok = a.q_strides[0];
@@ -229,6 +242,7 @@ int b200fa_paged_fwd(const b200fa_paged_args* args, void* stream) {
   p.sinks = a.sinks;
   p.scale_log2 = float(double(a.scale) * 1.4426950408889634074);
   p.timeout_ns = uint64_t(a.timeout_us ? a.timeout_us : 2000000u) * 1000ull;
+  p.wait_probes = uint32_t(p.timeout_ns / 20 < 0xffffffffull ? p.timeout_ns / 20 + 1 : 0xffffffffull);
   p.ws = static_cast<uint8_t*>(a.workspace);
   const bool bf16 = a.dtype == B200FA_DTYPE_BF16;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

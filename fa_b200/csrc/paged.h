@@ -37,7 +37,8 @@ constexpr uint32_t kPagedRecord = 32;   // bytes of a worker's record
 constexpr uint32_t kPagedPartials = kPagedHeader + kMaxWorkers * kPagedRecord;  // offset of the partial results
 
 struct PagedParams {
-  CUtensorMap tm_k, tm_v;   // (128, page_size, heads_kv, num_pages), box (64, min(page_size, 128), 1, 1)
+  CUtensorMap tm_k, tm_v;   // (128, page_size, heads_kv, num_pages), boxes of 64 columns; short kernel:
+                            // (64, page_size, 2, heads_kv, num_pages), boxes of both halves of the head dim
   CUtensorMap tm_q;         // chunk kernel: (128, group, heads_kv, tokens), box (64, group, 1, tokens_per_tile / 2)
   const void* q;
   void* o;
@@ -54,6 +55,7 @@ struct PagedParams {
   int32_t workers;
   int32_t part_rows;        // rows of a partial result
   uint64_t timeout_ns;
+  uint32_t wait_probes;     // chunk kernel: bound of a wait, in probes of at least 20 ns
   uint8_t* ws;
 };
 

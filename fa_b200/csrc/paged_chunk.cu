@@ -11,12 +11,12 @@
 //     worker's stretch of the line of key blocks (paged.h); the worker is the
 //     pair.  A Q tile is one box of the [tokens][heads_kv][group][128] view,
 //     so its rows land in the order token * group + head.
-//   * K and V come page by page: the boxes of a block are issued by the lanes
-//     of the producer warp, each with its own page from the block table, one
-//     block ahead of their use.
+//   * K and V come page by page, a box (K: one per 64 columns) for each page
+//     of a block; the producer warp reads the block table 32 entries ahead.
 //   * V rows behind the last key that any row sees are cleared in shared
-//     memory before the product (0 * NaN is no 0): warp 11 of each rank passes
-//     every V stage on to rank 0's PV issuer and clears the item's last one.
+//     memory before the product (0 * NaN is no 0), in an item's last
+//     stage: by the PV issuer's warp for rank 0, by the forwarding warp for
+//     rank 1.
 //   * scores are masked in tensor memory before the softmax loads them, so
 //     blocks without a mask run without selects.
 //   * an item that lies in the stretch is normalised and stored; one that a
@@ -47,7 +47,8 @@ constexpr int kSmXchg = kSmBar + kBars * 8;             // float [2][128]
 constexpr int kSmTmem = kSmXchg + 2 * kBlockM * 4;      // TMEM base, abort flag
 constexpr int kSmStart = kSmTmem + 16;                  // PagedStart
 constexpr int kSmScan = kSmStart + 64;                  // int64 [12]
-constexpr int kSmUsed = kSmScan + (kThreads / 32) * 8;
+constexpr int kSmPages = kSmScan + (kThreads / 32) * 8;  // 32 page numbers
+constexpr int kSmUsed = kSmPages + 128;
 constexpr int kBytes = kSmUsed + 1024;
 static_assert(kBytes <= 232448, "shared memory budget exceeded");
 static_assert(kSmBar % 8 == 0 && kSmStart % 8 == 0 && kSmScan % 8 == 0 && sizeof(PagedStart) <= 64, "layout");
@@ -61,6 +62,7 @@ struct Sm {
   __device__ __forceinline__ uint32_t xchg(uint32_t slot, int row) const { return base + kSmXchg + (slot * kBlockM + uint32_t(row)) * 4u; }
   __device__ __forceinline__ uint32_t tmem_slot() const { return base + kSmTmem; }
   __device__ __forceinline__ uint32_t abort_slot() const { return base + kSmTmem + 4; }
+  __device__ __forceinline__ uint32_t pages() const { return base + kSmPages; }
 };
 
 __device__ __forceinline__ Sm sm_of(uint8_t* raw) { return Sm{(smem_addr(raw) + 1023u) & ~1023u}; }
@@ -68,35 +70,26 @@ __device__ __forceinline__ const PagedStart* start_of(uint8_t* raw) {
   return reinterpret_cast<const PagedStart*>(raw + (sm_of(raw).base - smem_addr(raw)) + kSmStart);
 }
 
-// Bounded waits; a wait that runs out raises the abort flag of both CTAs.
+// Bounded waits: a number of probes, each of which may suspend the thread for
+// the probe's time hint.  A wait that runs out leaves its site in the abort
+// slot, which the teardown reports; the roles behind it run out in turn.  The
+// loop is kept this short on purpose: it is inlined at every wait of every
+// role, the hot loops of an SM sub-partition share a small instruction cache,
+// and with clock reads and an abort check in each, chunks ran slower.
 struct Wait {
   uint32_t abort_slot;
   const PagedParams* p;
-  __device__ __forceinline__ void fail(uint32_t site) const {
-    st_volatile_shared(abort_slot, 1u);
-    st_cluster_u32(map_shared(abort_slot, cluster_rank() ^ 1u), 1u);
-    paged_status(*p, kDevTimeout, site);
-  }
   template <bool kCluster = false>
   __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity, uint32_t site) const {
-    auto test = [&] { return kCluster ? mbar_test_cluster(bar, parity) : mbar_test(bar, parity); };
-    if (test()) return true;
-    const uint64_t t0 = global_timer_ns();
-    while (true) {
 #pragma unroll 1
-      for (int i = 0; i < 16; ++i)
-        if (test()) return true;
-      if (ld_volatile_shared(abort_slot) != 0u) return false;
-      if (global_timer_ns() - t0 > p->timeout_ns) {
-        fail(site);
-        return false;
-      }
-    }
+    for (uint32_t n = p->wait_probes; n != 0u; --n)
+      if (kCluster ? mbar_test_cluster(bar, parity) : mbar_test(bar, parity)) return true;
+    st_volatile_shared(abort_slot, site | 0x80000000u);
+    return false;
   }
-  __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity, uint64_t limit_ns) const {
-    const uint64_t t0 = global_timer_ns();
-    while (!mbar_test_cluster(bar, parity))
-      if (global_timer_ns() - t0 > limit_ns) return;
+  __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) const {
+#pragma unroll 1
+    for (uint32_t n = 1u << 20; n != 0u && !mbar_test_cluster(bar, parity); --n) {}
   }
 };
 
@@ -134,24 +127,43 @@ __device__ __forceinline__ void s_issuer(const PagedParams& p, const PagedStart&
     }
   }
   mma_commit_pair(sm.bar(kBarDrain + 0));
-  wait.drain(sm.bar(kBarDrain + 0), 0u, 100000000ull);
+  wait.drain(sm.bar(kBarDrain + 0), 0u);
 }
 
-// Rank 0, one thread: O += P V of every block, in order.
+// V rows from key `from` of the block on, which no row of the item sees, become
+// zeros: by a whole warp whose lanes have all observed the copy.
+__device__ __forceinline__ void clear_rows(uint32_t stage, int from, uint32_t lane) {
+  for (int i = int(lane) + (from > 0 ? from : 0) * 8; i < kPagedBlock * 8; i += 32) st_shared_v4(stage + uint32_t(i) * 16u, 0, 0, 0, 0);
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// First key of the block that no row of the item sees, relative to the block:
+// below kPagedBlock only in an item's last block.
+__device__ __forceinline__ int clear_from(const PagedBlocks& b, int block) { return b.end_key - b.key_block(block) * kPagedBlock; }
+
+// Rank 0, one warp, of which one lane issues: O += P V of every block, in order.
+// Where an item's last V stage needs clearing the warp does it for rank 0's
+// half and hands it over itself; the idle lanes wait at the warp barrier, so
+// none of them polls beside the issuing one (a warp that watched for those
+// stages alone cost every other wait of the CTA issue slots).
 template <bool kBf16>
 __device__ __forceinline__ void pv_issuer(const PagedParams& p, const PagedStart& start, const Sm& sm, uint32_t tmem, const Wait& wait) {
   const uint32_t site = uint32_t(kPVIssuerWarp) << 8;
-  uint32_t g = 0;
+  const uint32_t lane = tid_x() & 31u;
+  uint32_t g0 = 0, cleared = 0;  // bit e: parity of the next cleared stage in entry e
   bool ok = true;
-  for (PagedWalk w(p, start); ok && w.more(); w.next(p)) {
-    for (int j = 0; j < w.take; ++j, ++g) {
-      const uint32_t b = buf(g), e = ring_entry(g);
-      // Cluster scope: rank 1's rows of V may have been cleared by plain stores.
-      if (!wait.operator()<true>(sm.bar(kBarVFull + int(e)), ring_parity(g), site | uint32_t(kBarVFull + int(e))) ||
-          !wait(sm.bar(kBarPFull + int(b)), buf_parity(g), site | uint32_t(kBarPFull + int(b)))) {
-        ok = false;
-        break;
-      }
+  for (PagedWalk w(p, start); w.more(); w.next(p)) {
+    const int from = clear_from(w.blocks, w.off + w.take - 1);
+    const int plain = w.take - (from < kPagedBlock ? 1 : 0);
+    auto pv = [&](int j, bool cluster) -> bool {
+      const uint32_t g = g0 + uint32_t(j), b = buf(g), e = ring_entry(g);
+      const uint32_t bar = sm.bar(kBarVFull + int(e));
+      // Cluster scope where rank 1's rows of V were cleared by plain stores.
+      if (!(cluster ? wait.operator()<true>(bar, ring_parity(g), site | uint32_t(kBarVFull + int(e)))
+                    : wait(bar, ring_parity(g), site | uint32_t(kBarVFull + int(e)))) ||
+          !wait(sm.bar(kBarPFull + int(b)), buf_parity(g), site | uint32_t(kBarPFull + int(b))))
+        return false;
       tc_fence_after();
       const uint64_t v_desc = smem_desc(sm.v(e));
 #pragma unroll
@@ -160,17 +172,38 @@ __device__ __forceinline__ void pv_issuer(const PagedParams& p, const PagedStart
                     kk > 0 || j > 0 ? 1u : 0u);
       mma_commit_pair_both(sm.bar(kBarPVDone + int(b)));
       mma_commit_pair_both(sm.bar(kBarVEmpty + int(e)));
+      return true;
+    };
+    if (elect_one())
+      for (int j = 0; ok && j < plain; ++j) ok = pv(j, false);
+    ok = __all_sync(0xffffffffu, ok);
+    if (ok && plain < w.take) {
+      const uint32_t e = ring_entry(g0 + uint32_t(plain));
+      ok = __all_sync(0xffffffffu, wait(sm.bar(kBarVLand + int(e)), (cleared >> e) & 1u, site | uint32_t(kBarVLand + int(e))));
+      if (ok) {
+        clear_rows(sm.v(e), from, lane);
+        cleared ^= 1u << e;
+        if (elect_one()) {
+          mbar_arrive(sm.bar(kBarVFull + int(e)));
+          ok = pv(plain, true);
+        }
+        ok = __all_sync(0xffffffffu, ok);
+      }
     }
+    if (!ok) break;
+    g0 += uint32_t(w.take);
   }
-  mma_commit_pair(sm.bar(kBarDrain + 1));
-  wait.drain(sm.bar(kBarDrain + 1), 0u, 100000000ull);
+  // Issued by the lane that issued the products: commits follow a thread's own.
+  if (elect_one()) {
+    mma_commit_pair(sm.bar(kBarDrain + 1));
+    wait.drain(sm.bar(kBarDrain + 1), 0u);
+  }
 }
 
-// Both ranks, a whole warp: passes rank 1's Q and K stages and both ranks' V
-// stages on to rank 0's barriers, clearing V rows that no row of the item sees.
-__device__ __forceinline__ void forward(const PagedParams& p, const PagedStart& start, const Sm& sm, const Wait& wait,
-                                        uint32_t rank, uint32_t lane) {
-  const uint32_t site = (rank << 16) | (uint32_t(kForwardWarp) << 8);
+// Rank 1, one warp: passes its Q, K and V stages on to rank 0's barriers, and
+// clears V rows that no row of the item sees.
+__device__ __forceinline__ void forward(const PagedParams& p, const PagedStart& start, const Sm& sm, const Wait& wait, uint32_t lane) {
+  const uint32_t site = (1u << 16) | (uint32_t(kForwardWarp) << 8);
   uint32_t g = 0;
   bool ok = true;
   int it = 0;
@@ -184,23 +217,17 @@ __device__ __forceinline__ void forward(const PagedParams& p, const PagedStart& 
     if (lane == 0) mbar_arrive_cluster_relaxed(map_shared(sm.bar(bar), 0));
   };
   for (PagedWalk w(p, start); ok && w.more(); w.next(p), ++it) {
-    if (rank == 1) {
-      if (!(ok = landed(kBarQFull + (it & 1), uint32_t(it >> 1) & 1u))) break;
-      pass(kBarQFull + (it & 1));
-    }
+    if (!(ok = landed(kBarQFull + (it & 1), uint32_t(it >> 1) & 1u))) break;
+    pass(kBarQFull + (it & 1));
     for (int j = 0; j < w.take; ++j, ++g) {
       const int e = int(ring_entry(g));
-      if (rank == 1) {
-        if (!(ok = landed(kBarKFull + e, ring_parity(g)))) break;
-        pass(kBarKFull + e);
-      }
+      if (!(ok = landed(kBarKFull + e, ring_parity(g)))) break;
+      pass(kBarKFull + e);
       if (!(ok = landed(kBarVLand + e, ring_parity(g)))) break;
-      const int from = w.blocks.end_key - w.blocks.key_block(w.off + j) * kPagedBlock;
+      const int from = clear_from(w.blocks, w.off + j);
       if (from < kPagedBlock) {
         mbar_test(sm.bar(kBarVLand + e), ring_parity(g));  // every lane observes the copy
-        for (int i = int(lane) + (from > 0 ? from : 0) * 8; i < kPagedBlock * 8; i += 32) st_shared_v4(sm.v(uint32_t(e)) + uint32_t(i) * 16u, 0, 0, 0, 0);
-        fence_proxy_async_smem();
-        __syncwarp();
+        clear_rows(sm.v(uint32_t(e)), from, lane);
         if (lane == 0) mbar_arrive_cluster(map_shared(sm.bar(kBarVFull + e), 0));
       } else {
         pass(kBarVFull + e);
@@ -215,87 +242,89 @@ __device__ __forceinline__ void load(const PagedParams& p, const PagedStart& sta
   const uint32_t site = (rank << 16) | (uint32_t(kLoadWarp) << 8);
   const int half_tok = p.tokens_per_tile / 2;
   const uint32_t q_bytes = uint32_t(half_tok * p.group) * 256u;
-  const int shift = p.page_shift, size_mask = (1 << shift) - 1;
-  const int k_rows = shift < 6 ? 1 << shift : kPairKeys, v_rows = shift < 7 ? 1 << shift : kPagedBlock;
-  // Lane l: box l of K (half l % 2 of rows k_rows * (l / 2)) and of V; at most 16 each.
-  const int k_boxes = 2 * (kPairKeys / k_rows), v_boxes = kPagedBlock / v_rows;
-  const int k_row = int(lane >> 1) * k_rows, v_row = int(lane) * v_rows;
-  uint32_t g = 0, issued_k = 0, issued_v = 0, q_issued = 0;
+  const int size_mask = (1 << p.page_shift) - 1;
+  const int k_rows = p.page_shift < 6 ? 1 << p.page_shift : kPairKeys;  // of a K box: this rank's keys of a page
+  uint32_t g0 = 0, issued_k = 0, issued_v = 0, q_issued = 0;  // issued_*: in the issuing lane
   bool ok = true;
   int it = 0;
-  auto waited = [&](int bar, uint32_t parity) -> bool {
-    uint32_t got = 1;
-    if (lane == 0) got = wait(sm.bar(bar), parity, site | uint32_t(bar)) ? 1u : 0u;
-    return __shfl_sync(0xffffffffu, got, 0) != 0u;
+  // Bounded wait for a free stage, then the announcement of its bytes.
+  auto claim = [&](int empty, uint32_t parity, int full, uint32_t bytes) -> bool {
+    if (!wait(sm.bar(empty), parity, site | uint32_t(empty))) return false;
+    mbar_arrive_expect_tx(sm.bar(full), bytes);
+    return true;
   };
+  PageFeed feed(p, sm.pages());
+  const int k_first = feed.per > 1 ? int(rank) * (feed.per / 2) : 0, k_pages = kPairKeys / k_rows;
   for (PagedWalk w(p, start); ok && w.more(); w.next(p), ++it) {
     const int qt = it & 1;
-    if (!(ok = waited(kBarQEmpty + qt, (uint32_t(it >> 1) & 1u) ^ 1u))) break;
-    if (lane == 0) {
-      mbar_arrive_expect_tx(sm.bar(kBarQFull + qt), q_bytes);
-      const int tok = w.req.q0 + w.tile * p.tokens_per_tile + int(rank) * half_tok;
-      tma_load_4d(sm.q(qt), &p.tm_q, sm.bar(kBarQFull + qt), 0, 0, w.h, tok);
-      tma_load_4d(sm.q(qt) + kQHalfBytes, &p.tm_q, sm.bar(kBarQFull + qt), 64, 0, w.h, tok);
+    feed.begin(w, lane);
+    if (elect_one()) {
+      if ((ok = claim(kBarQEmpty + qt, (uint32_t(it >> 1) & 1u) ^ 1u, kBarQFull + qt, q_bytes))) {
+        const int tok = w.req.q0 + w.tile * p.tokens_per_tile + int(rank) * half_tok;
+        tma_load_4d(sm.q(qt), &p.tm_q, sm.bar(kBarQFull + qt), 0, 0, w.h, tok);
+        tma_load_4d(sm.q(qt) + kQHalfBytes, &p.tm_q, sm.bar(kBarQFull + qt), 64, 0, w.h, tok);
+        ++q_issued;
+      }
     }
-    ++q_issued;
-    int k_page = p.num_pages, v_page = p.num_pages;
-    auto pages = [&](int j) {
-      const int key0 = w.blocks.key_block(w.off + j) * kPagedBlock;
-      if (int(lane) < k_boxes) k_page = page_of(p, w.r, w.blocks, key0 + int(rank) * kPairKeys + k_row);
-      if (int(lane) < v_boxes) v_page = page_of(p, w.r, w.blocks, key0 + v_row);
-    };
-    pages(0);
-    for (int j = 0; j < w.take; ++j, ++g) {
-      const uint32_t e = ring_entry(g);
-      const int key0 = w.blocks.key_block(w.off + j) * kPagedBlock;
-      const int kp = k_page, vp = v_page;
-      if (j + 1 < w.take) pages(j + 1);
-      if (!(ok = waited(kBarKEmpty + int(e), ring_parity(g) ^ 1u))) break;
-      if (lane == 0) mbar_arrive_expect_tx(sm.bar(kBarKFull + int(e)), kStageBytes);
-      __syncwarp();
-      if (int(lane) < k_boxes)
-        tma_load_4d(sm.k(e) + (lane & 1) * kKBoxBytes + uint32_t(k_row) * 128u, &p.tm_k, sm.bar(kBarKFull + int(e)),
-                    64 * int(lane & 1), (key0 + int(rank) * kPairKeys + k_row) & size_mask, w.h, kp);
-      ++issued_k;
-      if (!(ok = waited(kBarVEmpty + int(e), ring_parity(g) ^ 1u))) break;
-      if (lane == 0) mbar_arrive_expect_tx(sm.bar(kBarVLand + int(e)), kStageBytes);
-      __syncwarp();
-      if (int(lane) < v_boxes)
-        tma_load_4d(sm.v(e) + uint32_t(v_row) * 128u, &p.tm_v, sm.bar(kBarVLand + int(e)), int(rank) * kPairDims,
-                    (key0 + v_row) & size_mask, w.h, vp);
-      ++issued_v;
+    ok = __all_sync(0xffffffffu, ok);
+    for (int j0 = 0; ok && j0 < w.take; j0 += feed.blocks_per_batch()) {
+      feed.batch(w, j0, lane);
+      const int n = min(feed.blocks_per_batch(), w.take - j0);
+      if (elect_one()) {
+        for (int j = 0; j < n; ++j) {
+          const uint32_t g = g0 + uint32_t(j), e = ring_entry(g);
+          const int key0 = w.blocks.key_block(w.off + j0 + j) * kPagedBlock;
+          // Rank 1's V is handed over by its warp 11; rank 0's where it needs clearing.
+          const bool hand = rank == 1 || w.blocks.end_key < key0 + kPagedBlock;
+          const int v_bar = (hand ? kBarVLand : kBarVFull) + int(e);
+          if (!(ok = claim(kBarKEmpty + int(e), ring_parity(g) ^ 1u, kBarKFull + int(e), kStageBytes))) break;
+          uint32_t dst = sm.k(e);
+          int key = key0 + int(rank) * kPairKeys;
+          for (int i = 0; i < k_pages; ++i, dst += uint32_t(k_rows) * 128u, key += k_rows) {
+            const int page = feed(j, k_first + i);
+            tma_load_4d(dst, &p.tm_k, sm.bar(kBarKFull + int(e)), 0, key & size_mask, w.h, page);
+            tma_load_4d(dst + kKBoxBytes, &p.tm_k, sm.bar(kBarKFull + int(e)), 64, key & size_mask, w.h, page);
+          }
+          ++issued_k;
+          if (!(ok = claim(kBarVEmpty + int(e), ring_parity(g) ^ 1u, v_bar, kStageBytes))) break;
+          dst = sm.v(e);
+          key = key0;
+          for (int i = 0; i < feed.per; ++i, dst += uint32_t(feed.rows) * 128u, key += feed.rows)
+            tma_load_4d(dst, &p.tm_v, sm.bar(v_bar), int(rank) * kPairDims, key & size_mask, w.h, feed(j, i));
+          ++issued_v;
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      g0 += uint32_t(n);
     }
   }
   // The last copies land before the CTA exits, also when a role gave up.
-  if (lane == 0) {
+  if (elect_one()) {
     for (uint32_t i = issued_k > kRing ? issued_k - kRing : 0; i < issued_k; ++i)
-      wait.drain(sm.bar(kBarKFull + int(ring_entry(i))), ring_parity(i), 50000000ull);
+      wait.drain(sm.bar(kBarKFull + int(ring_entry(i))), ring_parity(i));
     for (uint32_t i = issued_v > kRing ? issued_v - kRing : 0; i < issued_v; ++i)
-      wait.drain(sm.bar(kBarVLand + int(ring_entry(i))), ring_parity(i), 50000000ull);
+      wait.drain(sm.bar((rank == 1 ? kBarVLand : kBarVFull) + int(ring_entry(i))), ring_parity(i));
     for (uint32_t i = q_issued > 2 ? q_issued - 2 : 0; i < q_issued; ++i)
-      wait.drain(sm.bar(kBarQFull + int(i & 1u)), (i >> 1) & 1u, 50000000ull);
+      wait.drain(sm.bar(kBarQFull + int(i & 1u)), (i >> 1) & 1u);
   }
   __syncwarp();
 }
 
-// Exponentials of 64 keys of one row (fa_kernel.cuh's exp_keys with FP32 sums
-// and P in the cache's type): of every 8 pairs one through the polynomial.
+// Exponentials of 64 keys of one row: P in the cache's type, four chains of
+// FP32 sums.  All through MUFU: with one pair of eight on the FMA pipe, as in
+// the dense kernel, chunks took 4 to 10 % longer here (4 x 512 tokens over 32768
+// keys, 12 heads on 1: 248 against 225 us) -- the pipe's turn comes while the
+// other group loads and reduces, and the loop is shorter without it.
 template <bool kBf16>
 __device__ __forceinline__ void exp64(const uint32_t* r, uint64_t sl2x2, uint64_t nmx2, uint32_t* pk, uint64_t* acc) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
-    const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), sl2x2, nmx2);
-    uint64_t p2;
     float a, b;
-    if ((i & 7) == 7) {
-      p2 = exp2_poly2(x2);
-    } else {
-      f2_unpack(x2, a, b);
-      p2 = f2_pack(ex2_approx(a), ex2_approx(b));
-    }
-    f2_unpack(p2, a, b);
+    f2_unpack(f2_fma(f2_pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), sl2x2, nmx2), a, b);
+    a = ex2_approx(a);
+    b = ex2_approx(b);
     pk[i] = pack2<kBf16>(a, b);
-    acc[i & 3] = f2_add(acc[i & 3], p2);
+    acc[i & 3] = f2_add(acc[i & 3], f2_pack(a, b));
   }
 }
 
@@ -335,6 +364,11 @@ __device__ __forceinline__ void softmax(const PagedParams& p, const PagedStart& 
   for (PagedWalk w(p, start); ok && w.more(); w.next(p), ++it) {
     const int n = w.take;
     const int pos = w.blocks.pos0 + row_tok;
+    // Key blocks that some row of this CTA does not see in full: from its first
+    // row's position on, and up to the end of its last row's window.
+    const int first_pos = w.blocks.pos0 + int(rank) * half_tok, behind = first_pos + half_tok - 1 - p.window;
+    const int kb_hi = first_pos > 0 ? (first_pos + 1) / kPagedBlock : 0;
+    const int kb_lo = p.window > 0 && behind >= 0 ? behind / kPagedBlock : -1;
     float m_cur = kFirstRef, l_g = 0.f;
     for (int j = grp; j < n; j += 2) {
       const uint32_t gb = g0 + uint32_t(j);
@@ -348,16 +382,14 @@ __device__ __forceinline__ void softmax(const PagedParams& p, const PagedStart& 
       }
       tc_fence_after();
       {
-        const int key0 = w.blocks.key_block(w.off + j) * kPagedBlock;
-        const int valid = pos + 1 - key0;
-        const int lo = p.window > 0 ? valid - p.window : 0, sink = p.sinks - key0;
-        if (__any_sync(0xffffffffu, valid < kPagedBlock || (lo > 0 && sink < lo))) mask_window(tS, valid, lo, sink);
+        const int kb = w.blocks.key_block(w.off + j);
+        if (kb >= kb_hi || kb <= kb_lo) {
+          const int valid = pos + 1 - kb * kPagedBlock;
+          mask_window(tS, valid, p.window > 0 ? valid - p.window : 0, p.sinks - kb * kPagedBlock);
+        }
       }
       uint32_t r[kBlockN];
-      tmem_ld32(tS, r);
-      tmem_ld32(tS + 32u, r + 32);
-      tmem_ld32(tS + 64u, r + 64);
-      tmem_ld32(tS + 96u, r + 96);
+      tmem_ld128(tS, r);
       if (gb > 0) {
         if (!wait_warp(kBarRef + int((gb - 1u) & 1u), ((gb - 1u) >> 1) & 1u)) {
           tmem_wait_ld();
@@ -420,11 +452,6 @@ __device__ __forceinline__ void softmax(const PagedParams& p, const PagedStart& 
     // ---- the item's end: the row's sum, then O
     const uint32_t g_last = g0 + uint32_t(n) - 1u;
     g0 += uint32_t(n);
-    if (!wait_pv(g_last)) {
-      ok = false;
-      break;
-    }
-    tc_fence_after();
     float m_final = m_cur;
     if ((n - 1) % 2 != grp) {
       if (!wait_warp(kBarRef + int(g_last & 1u), (g_last >> 1) & 1u)) {
@@ -434,23 +461,24 @@ __device__ __forceinline__ void softmax(const PagedParams& p, const PagedStart& 
       m_final = ld_shared_f32(sm.xchg(g_last & 1u, row));
     }
     if (l_g != 0.f && m_final != m_cur) l_g *= ex2_approx(m_cur - m_final);
+    // The groups' sums meet in the item's Q tile, which nothing reads any more
+    // (a group here has seen, or waited for the reference after, the scores of
+    // the last block), while the last product of P and V is under way.
+    const uint32_t sums = sm.q(it & 1) + uint32_t(row) * 4u;
+    st_shared_f32(sums + uint32_t(grp) * 512u, l_g);
     arrive_local(kBarXchg);
-    if (!wait_warp(kBarXchg, 0u)) {
+    if (!wait_warp(kBarXchg, uint32_t(it) & 1u)) {
       ok = false;
       break;
     }
-    const uint32_t mine = grp == 0 ? (g_last & 1u) : ((g_last + 1u) & 1u);
-    st_shared_f32(sm.xchg(mine, row), l_g);
-    arrive_local(kBarXchg);
-    if (!wait_warp(kBarXchg, 1u)) {
+    const float l = l_g + ld_shared_f32(sums + uint32_t(grp ^ 1) * 512u);  // 0: the row saw no key
+    fence_proxy_async_smem();
+    arrive_local(kBarQEmpty + (it & 1));
+    if (!wait_pv(g_last)) {
       ok = false;
       break;
     }
-    // Every product of the item is done: its Q tile is free.
-    if (warp == 0 && lane == 0) mbar_arrive(sm.bar(kBarQEmpty + (it & 1)));
-    // A row that saw no key kept the floor as its reference (masked keys of the
-    // polynomial's share count 2^-120 each, so its sum is not quite 0).
-    const float l = m_final > 0.5f * kFirstRef ? l_g + ld_shared_f32(sm.xchg(mine ^ 1u, row)) : 0.f;
+    tc_fence_after();
     const int t0 = w.tile * p.tokens_per_tile;
     const int toks = w.req.len - t0 < p.tokens_per_tile ? w.req.len - t0 : p.tokens_per_tile;
     const bool real = row < half_tok * p.group && row_tok < toks;
@@ -513,7 +541,7 @@ __device__ __forceinline__ void setup(const PagedParams& p, uint8_t* raw) {
     const uint32_t fed = rank == 0 ? 2u : 1u;  // rank 0's full barriers also count rank 1's forward
     for (int t = 0; t < 2; ++t) {
       mbar_init(sm.bar(kBarQFull + t), fed);
-      mbar_init(sm.bar(kBarQEmpty + t), 1);
+      mbar_init(sm.bar(kBarQEmpty + t), 8);
       mbar_init(sm.bar(kBarSFull + t), 1);
       mbar_init(sm.bar(kBarSFree + t), kGroupWarps);
       mbar_init(sm.bar(kBarPFull + t), kGroupWarps);
@@ -567,20 +595,24 @@ __device__ __forceinline__ void roles(const PagedParams& p, uint8_t* raw) {
     if (warp == kLoadWarp) {
       load(p, start, sm, wait, rank, lane);
     } else if (warp == kForwardWarp) {
-      forward(p, start, sm, wait, rank, lane);
-    } else if (rank == 0 && lane == 0) {
+      if (rank == 1) forward(p, start, sm, wait, lane);
+    } else if (rank == 0) {
       const uint32_t tmem = ld_volatile_shared(sm.tmem_slot());
-      if (warp == kSIssuerWarp) s_issuer<kBf16>(p, start, sm, tmem, wait);
-      else pv_issuer<kBf16>(p, start, sm, tmem, wait);
+      if (warp == kPVIssuerWarp) pv_issuer<kBf16>(p, start, sm, tmem, wait);
+      else if (elect_one()) s_issuer<kBf16>(p, start, sm, tmem, wait);
     }
   }
   __syncwarp();
 }
 
-__device__ __forceinline__ void teardown(uint8_t* raw) {
+__device__ __forceinline__ void teardown(const PagedParams& p, uint8_t* raw) {
   const Sm sm = sm_of(raw);
   tc_fence_before();
   cluster_sync();
+  if (tid_x() == 0) {
+    const uint32_t site = ld_volatile_shared(sm.abort_slot());
+    if (site != 0u) paged_status(p, kDevTimeout, site & 0x7fffffffu);
+  }
   if ((tid_x() >> 5) == 0) {
     tc_fence_after();
     tmem_dealloc_pair(ld_volatile_shared(sm.tmem_slot()), kTmemCols);
@@ -597,7 +629,7 @@ using namespace b200fa;
     extern __shared__ uint8_t smem_raw[];                                                                      \
     chunk::setup(p, smem_raw);                                                                                 \
     chunk::roles<bf16>(p, smem_raw);                                                                           \
-    chunk::teardown(smem_raw);                                                                                 \
+    chunk::teardown(p, smem_raw);                                                                                \
   }
 B200FA_PAGED_CHUNK_KERNEL(b200_paged_chunk_fp16_kernel, false)
 B200FA_PAGED_CHUNK_KERNEL(b200_paged_chunk_bf16_kernel, true)

@@ -3,8 +3,8 @@
 //
 // Bound by reading the cache (2 bytes of K and V each per 4 * rows flops a
 // key), so the layout serves the loads: one block per SM, one warp that does
-// nothing but keep five 32 KiB entries of K and V in flight (a page's 64
-// columns per TMA box, 128-byte swizzle), and eight warps that multiply with
+// nothing but keep five 32 KiB entries of K and V in flight (a page per
+// TMA box, in two halves of 64 columns, 128-byte swizzle), and eight warps that multiply with
 // mma.sync -- 16 rows are an eighth of a tcgen05 tile, and the products take
 // under half of the time the bytes do.  A warp owns 16 rows and a share of
 // each block's keys (all eight share the keys of a 16-row tile) with its own
@@ -22,10 +22,12 @@
 namespace b200fa {
 
 constexpr int kShortWarps = 8;                       // consumers
-constexpr int kShortThreads = (kShortWarps + 1) * 32;
+// Three warpgroups, the last one for the producer: registers are handed out
+// per four warps, and 384 x 168 = 256 x 208 + 128 x 88 leaves the consumers 208.
+constexpr int kShortThreads = 384;
+constexpr uint32_t kShortRegs = 208, kShortLoadRegs = 88;
 constexpr int kShortRing = 5;
-constexpr int kTileBytes = kPagedBlock * 256;        // K or V of a block: two halves of 64 columns
-constexpr int kHalfBytes = kTileBytes / 2;
+constexpr int kTileBytes = kPagedBlock * 256;        // K or V of a block
 constexpr int kShortMergeBytes = 4 * 16 * 128 * 4;   // outputs of four warps
 constexpr int kShortQBytes = 64 * 256;
 constexpr int kSmRing = 0;
@@ -35,9 +37,10 @@ constexpr int kSmMl = kSmQ + kShortQBytes;           // float2 [8 warps][16 rows
 constexpr int kSmBars = kSmMl + 8 * 16 * 8;
 constexpr int kSmScan = kSmBars + 2 * kShortRing * 8;
 constexpr int kSmStart = kSmScan + (kShortThreads / 32) * 8;
-constexpr int kSmAbort = kSmStart + 48;
-constexpr int kShortSmemBytes = kSmAbort + 16 + 1024;
-static_assert(sizeof(PagedStart) <= 48 && kShortSmemBytes <= 232448, "shared memory budget");
+constexpr int kSmAbort = kSmStart + 64;
+constexpr int kSmPages = kSmAbort + 16;              // 32 page numbers
+constexpr int kShortSmemBytes = kSmPages + 128 + 1024;
+static_assert(sizeof(PagedStart) <= 64 && kShortSmemBytes <= 232448, "shared memory budget");
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -85,42 +88,44 @@ __device__ __forceinline__ bool paged_wait(const PagedParams& p, uint32_t bar, u
   }
 }
 
-// The producer warp: K and V of every block of the worker's stretch.  The
-// boxes of a block (page_size rows of 64 columns) are dealt over the lanes.
+// The producer warp: K and V of every block of the worker's stretch, a box per
+// page with both 64-column halves.  One lane issues them all: copies issued by
+// many lanes are taken one lane after another anyway, with more to do for each.
 __device__ __forceinline__ void short_load(const PagedParams& p, const PagedStart& s, uint32_t sm, uint32_t lane) {
   const uint32_t abort_slot = sm + kSmAbort;
-  const int rows = p.page_shift < 7 ? 1 << p.page_shift : kPagedBlock;  // of a box
-  const int boxes = 2 * (kPagedBlock / rows);                           // of K or V of a block: at most 32
-  uint32_t g = 0;  // ring uses: K, V of block 0, K, V of block 1, ...
+  const int size_mask = (1 << p.page_shift) - 1;
+  uint32_t g = 0;     // ring uses: K, V of block 0, K, V of block 1, ...
+  uint32_t last = 0;  // uses begun, in the issuing lane
   bool ok = true;
+  PageFeed feed(p, sm + kSmPages);
   for (PagedWalk w(p, s); ok && w.more(); w.next(p)) {
-    for (int j = w.off; ok && j < w.off + w.take; ++j) {
-      const int key0 = w.blocks.key_block(j) * kPagedBlock;
-      // Box b: half b % 2 of the rows [rows * (b / 2), + rows) of the block.
-      int page = p.num_pages;
-      if (int(lane) < boxes) page = page_of(p, w.r, w.blocks, key0 + int(lane >> 1) * rows);
-      for (int kv = 0; kv < 2; ++kv, ++g) {
-        const uint32_t e = g % kShortRing;
-        const uint32_t full = sm + kSmBars + 8 * e, empty = full + 8 * kShortRing;
-        if (lane == 0) ok = paged_wait(p, empty, ((g / kShortRing) & 1u) ^ 1u, abort_slot, 0x800u | e);
-        ok = __shfl_sync(0xffffffffu, int(ok), 0) != 0;
-        if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(full, kTileBytes);
-        __syncwarp();
-        const CUtensorMap* map = kv ? &p.tm_v : &p.tm_k;
-        if (int(lane) < boxes) {
-          const int row = int(lane >> 1) * rows;
-          tma_load_4d(sm + kSmRing + e * kTileBytes + (lane & 1) * kHalfBytes + uint32_t(row) * 128, map, full,
-                      64 * int(lane & 1), (key0 + row) & ((1 << p.page_shift) - 1), w.h, page);
+    feed.begin(w, lane);
+    for (int j0 = 0; ok && j0 < w.take; j0 += feed.blocks_per_batch()) {
+      feed.batch(w, j0, lane);
+      const int n = min(feed.blocks_per_batch(), w.take - j0);
+      if (elect_one()) {
+        for (int j = 0; ok && j < n; ++j) {
+          const int key0 = w.blocks.key_block(w.off + j0 + j) * kPagedBlock;
+          for (int kv = 0; kv < 2; ++kv) {
+            const uint32_t use = g + 2u * uint32_t(j) + uint32_t(kv), e = use % kShortRing;
+            const uint32_t full = sm + kSmBars + 8 * e, empty = full + 8 * kShortRing;
+            if (!(ok = paged_wait(p, empty, ((use / kShortRing) & 1u) ^ 1u, abort_slot, 0x800u | e))) break;
+            mbar_arrive_expect_tx(full, kTileBytes);
+            uint32_t dst = sm + kSmRing + e * kTileBytes;
+            for (int i = 0; i < feed.per; ++i, dst += uint32_t(feed.rows) * 256u)
+              tma_load_5d(dst, kv ? &p.tm_v : &p.tm_k, full, 0, (key0 + i * feed.rows) & size_mask, 0, w.h, feed(j, i));
+            last = use + 1;
+          }
         }
       }
+      ok = __all_sync(0xffffffffu, ok);
+      g += 2u * uint32_t(n);
     }
   }
   // The last copies land before the block exits, also when a warp gave up.
-  if (lane == 0) {
+  if (elect_one()) {
     const uint64_t t0 = global_timer_ns();
-    const uint32_t first = g > kShortRing ? g - kShortRing : 0;
-    for (uint32_t i = first; i < g; ++i)
+    for (uint32_t i = last > kShortRing ? last - kShortRing : 0; i < last; ++i)
       while (!mbar_test(sm + kSmBars + 8 * (i % kShortRing), (i / kShortRing) & 1u) && global_timer_ns() - t0 < 100000000ull) {}
   }
   __syncwarp();
@@ -138,6 +143,19 @@ __device__ __forceinline__ void short_rows(const PagedParams& p, const PagedStar
   const int quad = int(lane & 3), rq = int(lane >> 2);
   float2* ml = reinterpret_cast<float2*>(smem + kSmMl);
   float* merge = reinterpret_cast<float*>(smem + kSmMerge);
+  // Byte offset of a key's row in a tile, [page][half][row][128 B], and the
+  // distance of its halves.
+  const int row_shift = p.page_shift < 7 ? p.page_shift : 7;
+  const uint32_t half_bytes = 128u << row_shift;
+  auto row_of = [&](int key) { return (uint32_t(key >> row_shift) * 2u << row_shift) * 128u + (uint32_t(key) & ((1u << row_shift) - 1u)) * 128u; };
+  // This lane's rows for ldmatrix: of K (8 keys by 8 dims: keys, then dims) ...
+  const int mi = int(lane >> 3), l8 = int(lane & 7);
+  uint32_t k_off[kTiles / 2], v_off[kKeys / 16];
+#pragma unroll
+  for (int i = 0; i < kTiles / 2; ++i) k_off[i] = row_of(wn * kKeys + i * 16 + (mi >> 1) * 8 + l8);
+  // ... and of V (keys and dims swapped).
+#pragma unroll
+  for (int i = 0; i < kKeys / 16; ++i) v_off[i] = row_of(wn * kKeys + i * 16 + (mi & 1) * 8 + l8);
   auto bar_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kShortWarps * 32) : "memory"); };
   uint32_t g = 0;
   bool ok = true;
@@ -197,11 +215,9 @@ __device__ __forceinline__ void short_rows(const PagedParams& p, const PagedStar
       for (int kk = 0; kk < 8; ++kk) {
 #pragma unroll
         for (int i = 0; i < kTiles; i += 2) {
-          const int mi = int(lane >> 3);
-          const int key = wk0 + i * 8 + (mi >> 1) * 8 + int(lane & 7);
           const int c = (kk & 3) * 2 + (mi & 1);
           uint32_t b[4];
-          ldsm4(tile + (kk >> 2) * kHalfBytes + uint32_t(key * 128 + ((c ^ (key & 7)) << 4)), b);
+          ldsm4(tile + k_off[i / 2] + (kk >> 2) * half_bytes + uint32_t((c ^ l8) << 4), b);
           mma16816<kBf16>(sc[i], qf[kk], b[0], b[1]);
           mma16816<kBf16>(sc[i + 1], qf[kk], b[2], b[3]);
         }
@@ -263,7 +279,7 @@ __device__ __forceinline__ void short_rows(const PagedParams& p, const PagedStar
         // 0 * NaN is no 0: this warp's rows of them are cleared.
         const int from = max(wk0, w.blocks.end_key - key0);
         for (int i = int(lane); i < (wk0 + kKeys - from) * 16; i += 32)
-          st_shared_v4(tile + (i & 1) * kHalfBytes + uint32_t((from + (i >> 4)) * 128 + ((i >> 1) & 7) * 16), 0, 0, 0, 0);
+          st_shared_v4(tile + row_of(from + (i >> 4)) + (i & 1) * half_bytes + uint32_t((i >> 1) & 7) * 16u, 0, 0, 0, 0);
         fence_proxy_async_smem();  // the next copy into this entry follows these writes
         __syncwarp();
       }
@@ -272,11 +288,9 @@ __device__ __forceinline__ void short_rows(const PagedParams& p, const PagedStar
         const uint32_t a[4] = {pf[2 * kk][0], pf[2 * kk][1], pf[2 * kk + 1][0], pf[2 * kk + 1][1]};
 #pragma unroll
         for (int d = 0; d < 8; ++d) {  // 16 columns at a time
-          const int mi = int(lane >> 3);
-          const int key = wk0 + kk * 16 + (mi & 1) * 8 + int(lane & 7);
           const int c = (d & 3) * 2 + (mi >> 1);
           uint32_t b[4];
-          ldsm4_trans(tile + (d >> 2) * kHalfBytes + uint32_t(key * 128 + ((c ^ (key & 7)) << 4)), b);
+          ldsm4_trans(tile + v_off[kk] + (d >> 2) * half_bytes + uint32_t((c ^ l8) << 4), b);
           mma16816<kBf16>(o[2 * d], a, b[0], b[1]);
           mma16816<kBf16>(o[2 * d + 1], a, b[2], b[3]);
         }
@@ -399,9 +413,13 @@ __device__ __forceinline__ void paged_short_body(const PagedParams& p) {
   }
   PagedStart* start = reinterpret_cast<PagedStart*>(smem + kSmStart);
   find_start(p, int(blockIdx.x), reinterpret_cast<int64_t*>(smem + kSmScan), start);
-  const PagedStart s = *start;
-  if (warp == kShortWarps) short_load(p, s, sm, lane);
-  else short_rows<kBf16, kM>(p, s, sm, smem, int(blockIdx.x), warp, lane);
+  if (warp < kShortWarps) {
+    regs_increase<kShortRegs>();
+    short_rows<kBf16, kM>(p, *start, sm, smem, int(blockIdx.x), warp, lane);
+  } else {
+    regs_decrease<kShortLoadRegs>();
+    if (warp == kShortWarps) short_load(p, *start, sm, lane);
+  }
 }
 
 }  // namespace b200fa

@@ -36,6 +36,16 @@ __device__ __forceinline__ uint32_t sm_id() {
   return r;
 }
 
+// True in one lane of a converged warp.  A branch on it tells the compiler that
+// one lane runs what follows, so operands of TMA and MMA instructions, which
+// take uniform registers, are moved there once; under `lane == 0` it emits a
+// loop over the active lanes around each of them.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
 // ---------------------------------------------------------------- mbarrier
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");

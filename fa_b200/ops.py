@@ -101,7 +101,8 @@ class Operator:
         the reference's operator is non-causal).  ``window`` > 0 (with
         ``causal``): only keys i - window < j <= i of those, and the first
         ``sinks`` keys; a row that sees no key (Nq > Nk) gets zeros, and key
-        blocks that no row of a work item sees are not read.  ``rotary`` (a
+        blocks that no row of a work item sees are not read; softmax sums are
+        FP32 in both variants.  ``rotary`` (a
         ``fa_b200.rotary.Rotary``): Q and K are turned by it first, into new
         tensors, by ``positions`` ([N] or [B, N]; None: 0 .. N-1; given
         positions need Nq == Nk).  ``capture`` (FP32, at least

@@ -140,7 +140,8 @@ extern "C" {
  * row i attends keys i - window < j <= i and the first `sinks` keys j <= i
  * (b200fa_options.window >= 1, .sinks >= 0).  A row that sees no key (Nq > Nk)
  * gets zeros.  Key blocks that no row of a work item sees are not read.
- * Runs separate kernels (b200_fa_fp{16,32}_window_kernel). */
+ * Runs a separate kernel (b200_fa_window_kernel), the same for both variants:
+ * softmax sums in FP32. */
 #define B200FA_FLAG_WINDOW        64u
 #define B200FA_BLOCK_KEYS        128
 

@@ -4,8 +4,9 @@ sinks=S)``): key j is seen from row i when j <= i and (j > i - W or j < S).
 Tolerance, per output element, with w the softmax weights, A = sum w |v| and
 O the float64 result.  P is rounded to FP16 (half a step, 2^-11 relative) and
 its exponentials are good to 7.5e-5 (the polynomial; the others 2^-22); the
-normalizer's relative error adds to O: FP32 sums 2^-16 at most here, the FP16
-variant's FP16 partial sums 9 roundings (7 adds of a chain of 8, two folds).
+normalizer's relative error adds to O: FP32 sums 2^-16 at most here.  (The
+causal kernel of the FP16 variant: FP16 partial sums, 9 roundings, 7 adds of a
+chain of 8 and two folds.)
 Scores are FP32 sums of 128 products below 2^5 in all: 128 * 2^-24 * 2^5 <
 3e-4 absolute before the exponential.  O itself is rounded to FP16.
 """
@@ -61,7 +62,7 @@ def test_window_against_the_formula(shape, variant, debug):
     torch.cuda.synchronize()
     assert op.status(q.device)[0] == 0
     O, A = ref.window_attention(q, k, v, window, sinks)
-    over = (out.double() - O).abs() - _bound(O, A, variant)
+    over = (out.double() - O).abs() - _bound(O, A, "fp32")
     assert bool((over <= 0).all()), float(over.max())
     assert torch.equal(out[A == 0], torch.zeros_like(out[A == 0]))
 
@@ -76,7 +77,12 @@ def test_a_window_over_everything_is_the_causal_mask(variant):
     a = op(q, k, v, causal=True)
     b = op(q, k, v, causal=True, window=1500)
     torch.cuda.synchronize()
-    assert torch.equal(a, b)
+    # The causal kernels evaluate part of the exponentials on the FMA pipe and
+    # (fp16) sum in FP16; the window kernel does neither, so the two agree to
+    # the sum of their bounds against the formula, not bit for bit.
+    O, A = ref.window_attention(q, k, v, 1500, 0)
+    over = (a.double() - b.double()).abs() - _bound(O, A, variant) - _bound(O, A, "fp32")
+    assert bool((over <= 0).all()), float(over.max())
 
 
 @pytest.mark.gpu
