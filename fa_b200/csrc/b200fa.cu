@@ -317,7 +317,6 @@ int fill_params(const void* q, const void* k, const void* v, void* o, int64_t B,
   p->heads = int32_t(B * Hq);
   p->nq = int32_t(Nq);
   if (opts.flags & B200FA_FLAG_WINDOW) {
-    p->o = static_cast<__half*>(o);
     p->window = opts.window;
     p->sinks = opts.sinks < Nk ? opts.sinks : int32_t(Nk);
   }

@@ -78,7 +78,6 @@
 #pragma once
 #include <cstdint>
 #include <cuda.h>
-#include <cuda_fp16.h>
 #include "ptx.cuh"
 
 // B200FA_CAUSAL = 1: this translation unit's kernels apply the causal mask
@@ -252,7 +251,6 @@ struct FwdParams {
   float* capture;           // capture kernels: [4][heads][n_kv][nq] + [heads][n_kv][nq][128] FP32
   int32_t heads;            // B * Hq
   int32_t nq;               // query rows per head
-  __half* o;                // window kernel: the output, [heads][nq][128]
   int32_t window, sinks;    // window kernels: keys behind a row that stay visible, first keys that always do
 };
 
@@ -833,27 +831,20 @@ __device__ __forceinline__ uint32_t bits_below(int x) {
   return x <= 0 ? 0u : x >= 32 ? 0xffffffffu : (1u << x) - 1u;
 }
 
-// Masks this thread's row of a block's scores in tensor memory, before the
-// softmax loads it: key c stays when c < valid and (c >= lo or c < sink), the
-// others get -inf (one bit of a word per 32 keys rather than three comparisons
-// a key).  In place and ahead of the load, so that blocks no row of the warp
-// masks -- most -- run the same instructions as the kernel without a mask:
-// with the selects on the loaded registers a block took 1.6 us instead of 0.95
-// (B=4, Hq=32, N=8192), masked or not.
-__device__ __forceinline__ void mask_window(uint32_t tS, int valid, int lo, int sink) {
-#pragma unroll 1
+// Masks this thread's 128 loaded scores of a block: key c stays when c < valid
+// and (c >= lo or c < sink), the others get -inf; one bit of a word per 32 keys
+// rather than three comparisons a key.  Only called under a branch that the
+// whole warp takes: with a test per row the compiler made selects of it, which
+// every block then ran (1.6 us a block, masked or not, against 1.3; B=4, Hq=32,
+// N=8192, no key outside the window).
+__device__ __forceinline__ void mask_window(uint32_t* r, int valid, int lo, int sink) {
+#pragma unroll
   for (int c0 = 0; c0 < kBlockN; c0 += 32) {
     const uint32_t keep = bits_below(valid - c0) & (~bits_below(lo - c0) | bits_below(sink - c0));
-    if (__all_sync(0xffffffffu, keep == 0xffffffffu)) continue;
-    uint32_t s[32];
-    tmem_ld32(tS + uint32_t(c0), s);
-    tmem_wait_ld();
 #pragma unroll
     for (int i = 0; i < 32; ++i)
-      if ((keep & (1u << i)) == 0u) s[i] = __float_as_uint(-INFINITY);
-    tmem_st32(tS + uint32_t(c0), s);
+      if ((keep & (1u << i)) == 0u) r[c0 + i] = __float_as_uint(-INFINITY);
   }
-  tmem_wait_st();
 }
 #endif
 
@@ -1020,7 +1011,6 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
       if (ahead + 1 < valid) valid = ahead + 1;
       const int lo = ahead - p.window + 1;
       const int sink = p.sinks - kb * kBlockN;
-      if (kb >= kb_hi || kb <= kb_lo) mask_window(tS, valid, lo, sink);
 #elif B200FA_CAUSAL
       // Valid keys of the block for this row: the last block's key count
       // and the keys up to the row.
@@ -1067,6 +1057,9 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
       }
 #endif
       arrive_rank0(kBarSFree + int(b));  // the S issuer may refill the buffer
+#if B200FA_WINDOW
+      if (kb >= kb_hi || kb <= kb_lo) mask_window(r, valid, lo, sink);
+#endif
       const float mx = fmaxf(row_max64(r), row_max64(r + 64)) * sl2;
       tl.mark(int(warp), j, 2);
       // This group's partial sum follows the reference the other group left.
@@ -1156,10 +1149,10 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
     if (!ok) break;
 
 #if B200FA_WINDOW
-    // ---- epilogue of short items: the groups' sums meet in the item's Q tile,
-    // which nothing reads any more (a group here has seen, or waited for the
-    // reference after, the scores of the last block), while the last product of
-    // P and V is under way; O / l goes to global memory from the registers.
+    // ---- epilogue for short items: the groups' sums are exchanged while the
+    // last product of P and V is under way, and the staged tile is stored by a
+    // warp of its own (store_role), so that the softmax goes on with the next
+    // item's first blocks.
     const uint32_t g_last = g0 + uint32_t(n) - 1u;
     float m_final = m_cur;
     if ((n - 1) % 2 != grp) {
@@ -1170,41 +1163,38 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
       m_final = ld_shared_f32(sm.xchg(g_last & 1u, row));
     }
     if (l_g != 0.f && m_final != m_cur) l_g *= ex2_approx(m_cur - m_final);
-    const uint32_t sums = sm.q(it & 1) + uint32_t(row) * 4u;
+    // Through the Q tile's first rows, which nothing reads any more (a group
+    // here has seen, or waited for the reference after, the scores of the last
+    // block); phase 0: both sums written, phase 1: both read.
+    const uint32_t sQ = sm.q(it & 1);
+    const uint32_t sums = sQ + uint32_t(row) * 4u;
     st_shared_f32(sums + uint32_t(grp) * 512u, l_g);
     arrive_local(kBarXchg);
-    if (!wait_warp(kBarXchg, uint32_t(it) & 1u)) { ok = false; break; }
+    if (!wait_warp(kBarXchg, 0u)) { ok = false; break; }
     const float l = l_g + ld_shared_f32(sums + uint32_t(grp ^ 1) * 512u);
     const float inv_l = l > 0.f ? 1.f / l : 0.f;  // a row that sees no key: zeros
-    fence_proxy_async_smem();
-    arrive_local(kBarQEmpty + (it & 1));
+    arrive_local(kBarXchg);
     if (!wait_pv(g_last)) { ok = false; break; }
     tc_fence_after();
-    {
-      int bh, qb, cnt;
-      plan_decode<int>(p.nqb, p.unit_begin, p.unit_end, item, bh, qb, cnt);
-      const int orow = (qb + int(rank)) * kBlockM + row;
-      const bool stored = int(rank) < cnt && orow < p.nq &&
-                          w.check(bh >= 0 && bh < p.heads && orow >= 0, site | (kCheckSite + 4u));
-      uint4* dst = reinterpret_cast<uint4*>(p.o + (size_t(bh) * size_t(p.nq) + size_t(orow)) * kHeadDim + 64 * grp);
+    if (!wait_warp(kBarXchg, 1u)) { ok = false; break; }
 #pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
-        uint32_t o[32];
-        tmem_ld32(tO + 64u * uint32_t(grp) + 32u * uint32_t(c), o);
-        tmem_wait_ld();
-        if (stored) {
+    for (int c = 0; c < 2; ++c) {
+      uint32_t o[32];
+      tmem_ld32(tO + 64u * uint32_t(grp) + 32u * uint32_t(c), o);
+      tmem_wait_ld();
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            uint32_t h[4];
+      for (int u = 0; u < 4; ++u) {
+        uint32_t h[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              h[i] = pack_h2(__uint_as_float(o[8 * u + 2 * i]) * inv_l, __uint_as_float(o[8 * u + 2 * i + 1]) * inv_l);
-            dst[4 * c + u] = make_uint4(h[0], h[1], h[2], h[3]);
-          }
-        }
+        for (int i = 0; i < 4; ++i)
+          h[i] = pack_h2(__uint_as_float(o[8 * u + 2 * i]) * inv_l, __uint_as_float(o[8 * u + 2 * i + 1]) * inv_l);
+        const int gu = 8 * grp + 4 * c + u;  // 16-byte unit of the 256-byte output row
+        st_shared_v4(sQ + uint32_t(gu >> 3) * kQHalfBytes + uint32_t(row) * 128 + (uint32_t((gu & 7) ^ (row & 7)) << 4), h[0],
+                     h[1], h[2], h[3]);
       }
     }
     tc_fence_before();
+    fence_proxy_async_smem();
     arrive_local(kBarOStaged);
   }
 #else
@@ -1288,6 +1278,40 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
   }
 }
 
+#if B200FA_WINDOW
+// One thread of a warp with no other role (rank 0: warp 11, rank 1: warp 10):
+// stores each item's staged output and then frees its Q tile.  It polls with a
+// long time hint, so that it takes no issue slots from the softmax.
+__device__ __forceinline__ void store_role(const FwdParams& p, const Smem& sm, const Waiter& w, uint32_t rank, uint32_t warp) {
+  const uint32_t site = (rank << 16) | (warp << 8);
+  for (int item = int(cluster_id_x()), it = 0; item < p.num_items; item += int(num_clusters_x()), ++it) {
+    int bh, qb, cnt;
+    plan_decode<int>(p.nqb, p.unit_begin, p.unit_end, item, bh, qb, cnt);
+    const int orow = (qb + int(rank)) * kBlockM;
+    const uint32_t sQ = sm.q(it & 1);
+    // Bounded (2^25 probes of 2 us), but loosely: an item may be long, and the
+    // roles it waits for have closer bounds of their own.
+    uint32_t probes = 1u << 25;
+    while (!mbar_test_long(sm.bar(kBarOStaged), uint32_t(it) & 1u)) {
+      if (ld_volatile_shared(sm.abort_slot()) != 0u) return;
+      if (--probes == 0u) {
+        w.fail(site | uint32_t(kBarOStaged));
+        return;
+      }
+    }
+    if (int(rank) < cnt) {
+      if (!w.check(orow >= 0 && orow < p.nqb * kBlockM && bh >= 0 && bh < p.heads, site | (kCheckSite + 4u))) return;
+      tma_store_3d(&p.tm_o, sQ, 0, orow, bh);
+      tma_store_3d(&p.tm_o, sQ + kQHalfBytes, 64, orow, bh);
+      bulk_commit_group();
+      bulk_wait_group_read0();
+    }
+    mbar_arrive(sm.bar(kBarQEmpty + (it & 1)));
+  }
+  bulk_wait_group0();
+}
+#endif
+
 __device__ __forceinline__ Smem smem_of(uint8_t* smem_raw) { return Smem{(smem_addr(smem_raw) + 1023u) & ~1023u}; }
 
 __device__ __forceinline__ Waiter waiter_of(const FwdParams& p, const Smem& sm) { return Waiter{sm.abort_slot(), &p}; }
@@ -1305,7 +1329,7 @@ __device__ __forceinline__ void setup_phase(const FwdParams& p, uint8_t* smem_ra
     const uint32_t fed = rank == 0 ? 2u : 1u;  // rank 0's full barriers also count rank 1's forward
     for (int t = 0; t < 2; ++t) {
       mbar_init(sm.bar(kBarQFull + t), fed);
-      mbar_init(sm.bar(kBarQEmpty + t), B200FA_WINDOW ? 8 : 1);
+      mbar_init(sm.bar(kBarQEmpty + t), 1);
       mbar_init(sm.bar(kBarSFull + t), 1);
       mbar_init(sm.bar(kBarSFree + t), kGroupWarps);
       mbar_init(sm.bar(kBarPFull + t), kGroupWarps);
@@ -1377,8 +1401,11 @@ __device__ __forceinline__ void role_phase(const FwdParams& p, uint8_t* smem_raw
       else if (rank == 0 && warp == kPVIssuerWarp) pv_issuer_role(p, sm, tmem_base, w);
       else if (warp == kLoadWarp) load_role(p, sm, w, rank);
       else if (rank == 1 && warp == kForwardWarp) forward_role(p, sm, w);
+#if B200FA_WINDOW
+      else if (warp == (rank == 0 ? kForwardWarp : kPVIssuerWarp)) store_role(p, sm, w, rank, warp);
+#endif
     }
-    if (kTimeline && rank == 0 && warp == kForwardWarp) watch_role(p, sm, lane);
+    if (kTimeline && !B200FA_WINDOW && rank == 0 && warp == kForwardWarp) watch_role(p, sm, lane);
   }
   __syncwarp();
 }
