@@ -12,6 +12,8 @@ raise.
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import struct
 import threading
 
 from . import build as _build
@@ -81,6 +83,17 @@ class PagedArgs(C.Structure):
 Strides2, Strides3 = _i64 * 2, _i64 * 3
 _s = C.POINTER(_i64)
 
+
+@functools.lru_cache(maxsize=4096)
+def strides(*values):
+    """The values as a C array (one per set of values: making one costs more than a light kernel's launch)."""
+    return (_i64 * len(values))(*values)
+
+
+# PagedArgs' bytes from its fields in one call (natural alignment, as C lays it out).
+paged_args = struct.Struct("@Ii4P2q2q3q3qPqPPqqiiiiiifiiIPQ")
+assert paged_args.size == C.sizeof(PagedArgs)
+
 SIGNATURES = {
     "b200fa_num_units": (_i64, [_i64, _i64, _i64]),
     "b200fa_partition": (C.c_int, [_i64, _i32, _i32, C.POINTER(_i64), C.POINTER(_i64)]),
@@ -106,7 +119,7 @@ SIGNATURES = {
     "b200fa_append": (C.c_int, [_p, _s, _p, _s, _p, _s, _p, _s, _p, _s, _p, _s, _i64, _i32, _i32, _i32, _i64, _i32,
                                 _p, _p, _i32, C.POINTER(RotaryDesc), _i32, _p]),
     "b200fa_paged_workspace_size": (_i64, []),
-    "b200fa_paged_fwd": (C.c_int, [C.POINTER(PagedArgs), _p]),
+    "b200fa_paged_fwd": (C.c_int, [_p, _p]),  # a PagedArgs, or its bytes
 }
 
 _lock = threading.Lock()
@@ -124,6 +137,9 @@ class B200FAError(RuntimeError):
 def load(build_if_needed: bool = True, debug: bool = False) -> C.CDLL:
     """Load (building first if the sources changed) and bind the library;
     ``debug`` selects the checking build libb200fa_debug.so."""
+    lib = _libs.get(debug)
+    if lib is not None:
+        return lib
     with _lock:
         lib = _libs.get(debug)
         if lib is not None:

@@ -15,14 +15,13 @@ stay on the device, so a step can be captured into a CUDA graph.
 
 from __future__ import annotations
 
-import ctypes as C
 from dataclasses import dataclass
 
 import torch
 
 from . import lib
 from .ops import HEAD_DIM, _window
-from .rotary import DTYPES, Rotary, _position_bits
+from .rotary import DTYPES, Rotary, _position_bits, call
 
 
 def _int32(name, t, shape, device):
@@ -44,7 +43,7 @@ class StepTables:
     @staticmethod
     def empty(requests: int, num_tokens: int, device) -> "StepTables":
         ints = torch.empty(2 * requests + 3 + num_tokens, dtype=torch.int32, device=device)
-        cu, kv, left, status, pos = ints.split([requests + 1, requests, 1, 1, num_tokens])
+        cu, kv, left, status, pos = ints.split_with_sizes([requests + 1, requests, 1, 1, num_tokens])
         return StepTables(torch.empty(num_tokens, dtype=torch.int64, device=device), pos, cu, kv, left, status)
 
 
@@ -91,13 +90,10 @@ def build_tables(ctx_lens, new_lens, block_table, free_pages, free_count, *, pag
                 a, b = t.data_ptr(), u.data_ptr()
                 if a < b + u.numel() * 4 and b < a + t.numel() * t.element_size():
                     raise ValueError("an output overlaps an input: alternate between two StepTables")
-    with torch.cuda.device(dev):
-        lib.check(lib.load().b200fa_build_tables(
-            ctx_lens.data_ptr(), new_lens.data_ptr(), R, block_table.data_ptr(), block_table.stride(0),
-            block_table.shape[1], free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), page_size,
-            out.slots.data_ptr(), out.positions.data_ptr(), num_tokens, out.cu_q.data_ptr(), out.kv_lens.data_ptr(),
-            out.free_left.data_ptr(), out.status.data_ptr(), torch.cuda.current_stream(dev).cuda_stream),
-            "b200fa_build_tables")
+    call(dev, "b200fa_build_tables", ctx_lens.data_ptr(), new_lens.data_ptr(), R, block_table.data_ptr(),
+         block_table.stride(0), block_table.shape[1], free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
+         page_size, out.slots.data_ptr(), out.positions.data_ptr(), num_tokens, out.cu_q.data_ptr(),
+         out.kv_lens.data_ptr(), out.free_left.data_ptr(), out.status.data_ptr())
     return out
 
 
@@ -143,7 +139,7 @@ def append(k, v, k_pages, v_pages, slots, *, q=None, positions=None, rotary: Rot
         if rotary.dim != dim:
             raise ValueError(f"the rotary's dim is {rotary.dim}, the cache's {dim}")
         bits, pos_ptr = _position_bits(positions, dev), positions.data_ptr()
-        desc = C.byref(rotary.desc(dev))
+        desc = rotary.desc(dev)
     if q is not None:
         _rows("q", q, (T, None, dim), k_pages)
         if q_out is None:
@@ -151,16 +147,13 @@ def append(k, v, k_pages, v_pages, slots, *, q=None, positions=None, rotary: Rot
         elif q_out.shape != q.shape:
             raise ValueError("q_out must be shaped like q")
         _rows("q_out", q_out, (T, None, dim), k_pages)
-        qa = (q.data_ptr(), lib.Strides2(*q.stride()[:2]), q_out.data_ptr(), lib.Strides2(*q_out.stride()[:2]))
+        qa = (q.data_ptr(), lib.strides(*q.stride()[:2]), q_out.data_ptr(), lib.strides(*q_out.stride()[:2]))
     else:
         qa = (None, None, None, None)
-    with torch.cuda.device(dev):
-        lib.check(lib.load().b200fa_append(
-            *qa, k.data_ptr(), lib.Strides2(*k.stride()[:2]), v.data_ptr(), lib.Strides2(*v.stride()[:2]),
-            k_pages.data_ptr(), lib.Strides3(*k_pages.stride()[:3]), v_pages.data_ptr(),
-            lib.Strides3(*v_pages.stride()[:3]), T, 0 if q is None else q.shape[1], hkv, dim, pages, ps,
-            slots.data_ptr(), pos_ptr, bits, desc, DTYPES[k_pages.dtype], torch.cuda.current_stream(dev).cuda_stream),
-            "b200fa_append")
+    call(dev, "b200fa_append", *qa, k.data_ptr(), lib.strides(*k.stride()[:2]), v.data_ptr(),
+         lib.strides(*v.stride()[:2]), k_pages.data_ptr(), lib.strides(*k_pages.stride()[:3]), v_pages.data_ptr(),
+         lib.strides(*v_pages.stride()[:3]), T, 0 if q is None else q.shape[1], hkv, dim, pages, ps, slots.data_ptr(),
+         pos_ptr, bits, desc, DTYPES[k_pages.dtype])
     return q_out
 
 
@@ -233,15 +226,13 @@ class PagedOperator:
         ws = self.workspace(dev)
         qs, os = q.stride(), out.stride()
         ks, vs = k_pages.stride(), v_pages.stride()
-        args = lib.PagedArgs(
-            C.sizeof(lib.PagedArgs), DTYPES[q.dtype], q.data_ptr(), out.data_ptr(), k_pages.data_ptr(),
-            v_pages.data_ptr(), lib.Strides2(qs[0], qs[1]), lib.Strides2(os[0], os[1]), lib.Strides3(*ks[:3]),
-            lib.Strides3(*vs[:3]), block_table.data_ptr(), block_table.stride(0), kv_lens.data_ptr(), cu_q.data_ptr(), T,
-            pages, R, block_table.shape[1], ps, hq, hkv, min(int(max_q), 2**31 - 1),
-            HEAD_DIM ** -0.5 if scale is None else scale, window, sinks, self.timeout_us, ws.data_ptr(), ws.numel())
-        with torch.cuda.device(dev):
-            lib.check(lib.load().b200fa_paged_fwd(C.byref(args), torch.cuda.current_stream(dev).cuda_stream),
-                      "b200fa_paged_fwd")
+        args = lib.paged_args.pack(
+            lib.paged_args.size, DTYPES[q.dtype], q.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+            qs[0], qs[1], os[0], os[1], *ks[:3], *vs[:3], block_table.data_ptr(), block_table.stride(0),
+            kv_lens.data_ptr(), cu_q.data_ptr(), T, pages, R, block_table.shape[1], ps, hq, hkv,
+            max(0, min(int(max_q), 2**31 - 1)), HEAD_DIM ** -0.5 if scale is None else scale, window, sinks,
+            self.timeout_us, ws.data_ptr(), ws.numel())
+        call(dev, "b200fa_paged_fwd", args)
         return out
 
     def step(self, q, k, v, k_pages, v_pages, block_table, tables: StepTables, *, max_q: int,

@@ -81,9 +81,9 @@ class Rotary:
     def desc(self, device, inverse: bool = False) -> lib.RotaryDesc:
         d = self._descs.get((device, inverse))
         if d is None:
-            d = self._descs[(device, inverse)] = lib.RotaryDesc(
-                C.sizeof(lib.RotaryDesc), self.dim, self.rotary_dim, LAYOUTS[self.layout], int(inverse), self.magnitude,
-                self.table(device).data_ptr())
+            d = lib.RotaryDesc(C.sizeof(lib.RotaryDesc), self.dim, self.rotary_dim, LAYOUTS[self.layout], int(inverse),
+                               self.magnitude, self.table(device).data_ptr())
+            self._descs[(device, inverse)] = d
         return d
 
     def __call__(self, x: torch.Tensor, positions: torch.Tensor | None = None, *, out: torch.Tensor | None = None,
@@ -122,12 +122,25 @@ class Rotary:
             else:
                 raise ValueError("positions must be [N] or [B,N]")
             pos_ptr = positions.data_ptr()
-        with torch.cuda.device(x.device):
-            stream = torch.cuda.current_stream(x.device).cuda_stream
-            lib.check(lib.load().b200fa_rotary(
-                x.data_ptr(), out.data_ptr(), B, N, H, lib.Strides3(*xs[:3]), lib.Strides3(*os[:3]), pos_ptr, bits,
-                pos_stride, C.byref(self.desc(x.device, bool(inverse))), dtype, stream), "b200fa_rotary")
+        call(x.device, "b200fa_rotary", x.data_ptr(), out.data_ptr(), B, N, H, lib.strides(*xs[:3]),
+             lib.strides(*os[:3]), pos_ptr, bits, pos_stride, self.desc(x.device, bool(inverse)), dtype)
         return out
+
+
+def call(device, name: str, *args) -> None:
+    """Calls a C entry on the device's current stream (its last argument) with
+    the device current; raises on a nonzero status.  The device is switched
+    only when another one is current: the context manager takes longer than
+    the call."""
+    so = lib.load()
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        status = getattr(so, name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            status = getattr(so, name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        lib.check(status, name)
 
 
 def _position_bits(positions, device) -> int:
