@@ -18,39 +18,48 @@ __global__ void __launch_bounds__(kShortThreads, 1) b200_paged_short_kernel(cons
 }
 
 // Joins the parts of the item that begins in worker blockIdx.x's stretch and
-// goes on behind it, in worker order.  One warp per row at a time, four
-// columns per lane; rows are split over gridDim.y.  Reads 520 bytes per row
-// and part, from L2.
+// goes on behind it, in worker order.  A warp per row, four columns per lane,
+// the outputs of eight parts on their way before their weights are known: the
+// time is that of a few trips to L2 (520 bytes per row and part).  Launched so
+// that it is resident by the time the attention kernel ends.
 template <bool kBf16>
 __global__ void __launch_bounds__(256) b200_paged_combine_kernel(const __grid_constant__ PagedParams p) {
+  grid_wait();
   const int worker = int(blockIdx.x);
   const PagedRecord rec = *paged_record(p, worker);
-  if (rec.parts == 0) return;
-  const int lane = int(threadIdx.x & 31), warp = int(threadIdx.x >> 5);
-  const int rows = rec.tokens * p.group;
+  const int lane = int(threadIdx.x & 31), rows = rec.parts > 0 ? rec.tokens * p.group : 0;
   auto part = [&](int i) { return paged_partial(p, i == 0 ? 2 * worker + 1 : 2 * (worker + i)); };
-  for (int row = int(blockIdx.y) * 8 + warp; row < rows; row += int(gridDim.y) * 8) {
+  for (int row = int(blockIdx.y) * 8 + int(threadIdx.x >> 5); row < rows; row += int(gridDim.y) * 8) {
+    constexpr int kAhead = 8;
+    float4 v[kAhead];
+    auto fetch = [&](int i0) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (i0 + i < rec.parts) v[i] = __ldcg(reinterpret_cast<const float4*>(part(i0 + i) + row * 128 + lane * 4));
+    };
+    fetch(0);
     float top = -1e30f;
     for (int i = lane; i < rec.parts; i += 32) top = fmaxf(top, part(i)[p.part_rows * 128 + row]);
 #pragma unroll
     for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    float sum = 0.f;
+    float sum = 0.f, f = 0.f, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = 0; i0 < rec.parts; i0 += 32) {
-      float f = 0.f, l = 0.f;
-      if (i0 + lane < rec.parts) {
-        const float* tail = part(i0 + lane) + p.part_rows * 128;
-        f = ex2_approx(tail[row] - top);
-        l = tail[p.part_rows + row];
+    for (int i0 = 0; i0 < rec.parts; i0 += kAhead) {
+      if ((i0 & 31) == 0) {  // weights and sums of 32 parts, one per lane
+        f = l = 0.f;
+        if (i0 + lane < rec.parts) {
+          const float* tail = part(i0 + lane) + p.part_rows * 128;
+          f = ex2_approx(tail[row] - top);
+          l = tail[p.part_rows + row];
+        }
       }
-      const int n = min(32, rec.parts - i0);
-#pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const float fi = __shfl_sync(0xffffffffu, f, i);
-        sum += fi * __shfl_sync(0xffffffffu, l, i);
-        const float4 v = *reinterpret_cast<const float4*>(part(i0 + i) + row * 128 + lane * 4);
-        acc.x += fi * v.x, acc.y += fi * v.y, acc.z += fi * v.z, acc.w += fi * v.w;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const float fi = __shfl_sync(0xffffffffu, f, (i0 + i) & 31);
+        sum += fi * __shfl_sync(0xffffffffu, l, (i0 + i) & 31);
+        if (i0 + i < rec.parts) acc.x += fi * v[i].x, acc.y += fi * v[i].y, acc.z += fi * v[i].z, acc.w += fi * v[i].w;
       }
+      if (i0 + kAhead < rec.parts) fetch(i0 + kAhead);
     }
     const float inv = sum > 0.f ? 1.f / sum : 0.f;
     const int t = row / p.group, hd = row - t * p.group;
@@ -247,12 +256,10 @@ int b200fa_paged_fwd(const b200fa_paged_args* args, void* stream) {
   const bool bf16 = a.dtype == B200FA_DTYPE_BF16;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  unsigned row_blocks;
   if (chunk) {
     p.workers = d->pairs;
     p.tokens_per_tile = 2 * (128 / group);  // half of them per CTA of the pair
     p.part_rows = 256;
-    row_blocks = 8;
     if ((rc = encode_q(&p.tm_q, a, group, p.tokens_per_tile / 2)) != B200FA_OK) return rc;
     e = cudaError_t(paged_chunk_launch(p, bf16, st));
   } else {
@@ -260,15 +267,11 @@ int b200fa_paged_fwd(const b200fa_paged_args* args, void* stream) {
     p.workers = d->sms;
     p.tokens_per_tile = 16 * m / group;
     p.part_rows = 16 * m;
-    row_blocks = unsigned(m);
-    short_kernel(bf16, m)<<<p.workers, kShortThreads, kShortSmemBytes, st>>>(p);
-    e = cudaGetLastError();
+    e = launch_early(short_kernel(bf16, m), dim3(unsigned(p.workers)), dim3(kShortThreads), kShortSmemBytes, st, p);
   }
   if (e != cudaSuccess) return cuda_fail(e, "paged attention launch");
-  const dim3 grid(unsigned(p.workers), row_blocks);
-  if (bf16) b200_paged_combine_kernel<true><<<grid, 256, 0, st>>>(p);
-  else b200_paged_combine_kernel<false><<<grid, 256, 0, st>>>(p);
-  e = cudaGetLastError();
+  e = launch_early(bf16 ? b200_paged_combine_kernel<true> : b200_paged_combine_kernel<false>,
+                   dim3(unsigned(p.workers), unsigned(chunk ? 16 : p.part_rows / 8)), dim3(256), 0, st, p);
   return e == cudaSuccess ? B200FA_OK : cuda_fail(e, "combine kernel launch");
 }
 

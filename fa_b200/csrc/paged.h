@@ -161,9 +161,16 @@ __device__ __forceinline__ int64_t blocks_before(const PagedParams& p, const Pag
   return n;
 }
 
-__device__ __forceinline__ int64_t request_blocks(const PagedParams& p, int r) {
-  const PagedRequest q = paged_request(p, r);
-  return blocks_before(p, q, q.tiles(p)) * p.heads_kv;
+// Key blocks of a request for one key/value head.
+__device__ __forceinline__ int64_t head_blocks(const PagedParams& p, const PagedRequest& q) {
+  const int tiles = q.tiles(p);
+  return tiles == 1 ? paged_blocks(p, q, 0).n : blocks_before(p, q, tiles);
+}
+
+// a / b for a >= 0, b > 0: in 32 bits where it fits (a 64-bit division takes
+// some hundred cycles, and a worker's start is on every call's path).
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? int64_t(uint32_t(a) / uint32_t(b)) : a / b;
 }
 
 // A worker's place in the line of blocks.
@@ -171,19 +178,24 @@ struct PagedStart {
   int r, h, tile, off;   // first item and the block of it to begin with
   int64_t count;         // blocks of the stretch
   int64_t total;         // blocks of all
-  int workers;           // stretches they are cut into: no more than blocks
+  int64_t per;           // total / workers
+  int workers, rest;     // stretches they are cut into, no more than blocks; total % workers
+
+  // First block of stretch w: floor(total w / workers).
+  __device__ __forceinline__ int64_t begin(int w) const { return per * w + int64_t(uint32_t(rest) * uint32_t(w) / uint32_t(workers)); }
+  // The stretch that holds block x: the last w with begin(w) <= x.
+  __device__ __forceinline__ int owner(int64_t x) const { return int(((x + 1) * workers - 1) / total); }
 };
+static_assert(kMaxWorkers <= 512, "rest * w stays below 2^32");
 
-__device__ __forceinline__ int64_t stretch_begin(int64_t total, int w, int n) { return total / n * w + total % n * w / n; }
-
-// The same for every worker; all threads of the block call it.  `scratch`:
-// blockDim.x / 32 + 1 shared int64; `start`: shared.
+// The start of worker `worker`; all threads of the block call it.  `scratch`:
+// blockDim.x / 32 shared int64; `start`: shared.
 __device__ __forceinline__ void find_start(const PagedParams& p, int worker, int64_t* scratch, PagedStart* start) {
   const int tid = int(threadIdx.x), nt = int(blockDim.x), warps = nt / 32;
   const int per = (p.requests + nt - 1) / nt;
   const int r0 = min(p.requests, tid * per), r1 = min(p.requests, r0 + per);
   int64_t sum = 0;
-  for (int r = r0; r < r1; ++r) sum += request_blocks(p, r);
+  for (int r = r0; r < r1; ++r) sum += head_blocks(p, paged_request(p, r)) * p.heads_kv;
   int64_t inc = sum;
   for (int d = 1; d < 32; d <<= 1) {
     const int64_t a = __shfl_up_sync(0xffffffffu, inc, d);
@@ -196,28 +208,41 @@ __device__ __forceinline__ void find_start(const PagedParams& p, int worker, int
     if (w < (tid >> 5)) inc += scratch[w];
     total += scratch[w];
   }
-  const int workers = total < p.workers ? int(total) : p.workers;
-  int64_t begin = 0, end = 0;
-  if (worker < workers) begin = stretch_begin(total, worker, workers), end = stretch_begin(total, worker + 1, workers);
+  PagedStart s{0, 0, 0, 0, 0, total, 0, total < p.workers ? int(total) : p.workers, 0};
+  int64_t begin = 0;
+  if (worker < s.workers) {
+    s.per = divide(total, s.workers);
+    s.rest = int(total - s.per * s.workers);
+    begin = s.begin(worker);
+    s.count = s.begin(worker + 1) - begin;
+  }
+  __syncthreads();  // scratch has been read
+  if (s.count == 0) {
+    if (tid == 0) *start = s;
+    __syncthreads();
+    return;
+  }
   int64_t at = inc - sum;
-  if (tid == 0) *start = PagedStart{0, 0, 0, 0, end - begin, total, workers};
-  __syncthreads();
-  if (end > begin && at <= begin && begin < inc) {
+  if (at <= begin && begin < inc) {  // one thread
     for (int r = r0; r < r1; ++r) {
-      const int64_t n = request_blocks(p, r);
+      const PagedRequest q = paged_request(p, r);
+      const int64_t head = head_blocks(p, q), n = head * p.heads_kv;
       if (begin >= at + n) {
         at += n;
         continue;
       }
-      const int64_t head = n / p.heads_kv, x = begin - at;
-      start->r = r;
-      start->h = int(x / head);
-      scratch[0] = x % head;
+      const int64_t x = begin - at, h = divide(x, head);
+      s.r = r;
+      s.h = int(h);
+      s.tile = q.tiles(p) == 1 ? 0 : -1;  // -1: still to be found
+      scratch[0] = x - h * head;
+      s.off = int(scratch[0]);
+      *start = s;
       break;
     }
   }
   __syncthreads();
-  if (end <= begin) return;
+  if (start->tile == 0) return;
   // The tile: every thread looks at the beginning of one in `step`.
   const PagedRequest q = paged_request(p, start->r);
   const int64_t rest = scratch[0];
@@ -294,18 +319,23 @@ __device__ __forceinline__ PagedRecord* paged_record(const PagedParams& p, int w
   return reinterpret_cast<PagedRecord*>(p.ws + kPagedHeader) + worker;
 }
 
+// One thread of a warp with no other role: the worker's record.
+__device__ __forceinline__ void write_record(const PagedParams& p, const PagedStart& s, int worker) {
+  PagedRecord rec{0, 0, 0, 0, {0, 0, 0, 0}};
+  for (PagedWalk w(p, s); w.more(); w.next(p)) {
+    if (!w.begins() || w.ends()) continue;
+    const int t0 = w.tile * p.tokens_per_tile, left = w.req.len - t0;
+    rec.parts = s.owner(s.begin(worker + 1) + (w.blocks.n - (w.off + w.take)) - 1) - worker + 1;
+    rec.row0 = w.req.q0 + t0;
+    rec.tokens = left < p.tokens_per_tile ? left : p.tokens_per_tile;
+    rec.h = w.h;
+  }
+  *paged_record(p, worker) = rec;
+}
+
 // Partial slot s: [rows][128] outputs, then [rows] maxima, then [rows] sums.
 __device__ __forceinline__ float* paged_partial(const PagedParams& p, int slot) {
   return reinterpret_cast<float*>(p.ws + kPagedPartials) + size_t(slot) * size_t(p.part_rows) * 130u;
-}
-
-// Stretches covered by an item that begins in `worker` and has `rest` blocks
-// behind that worker's end.
-__device__ __forceinline__ int paged_parts(const PagedStart& s, int worker, int64_t rest) {
-  const int64_t end = stretch_begin(s.total, worker + 1, s.workers) + rest;
-  int w = worker + 1;
-  while (w < s.workers && stretch_begin(s.total, w, s.workers) < end) ++w;
-  return w - worker;
 }
 
 __device__ __forceinline__ void paged_status(const PagedParams& p, uint32_t code, uint32_t site) {
@@ -314,6 +344,24 @@ __device__ __forceinline__ void paged_status(const PagedParams& p, uint32_t code
     ws[1] = site;
     ws[2] = blockIdx.x;
   }
+}
+
+// A launch that may begin before the work ahead of it in the stream has ended:
+// the kernel waits for that itself (grid_wait) before it touches memory, and
+// what can be done before -- barriers, tensor memory, descriptors -- is done.
+inline cudaError_t launch_early(void (*kernel)(PagedParams), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                                const PagedParams& p) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
 // The chunk kernel (paged_chunk.cu): workers are CTA pairs.  0 or a CUDA error.

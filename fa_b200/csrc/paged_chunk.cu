@@ -545,8 +545,6 @@ __device__ __forceinline__ void softmax(const PagedParams& p, const PagedStart& 
         part[p.part_rows * 128 + prow] = m_final;
         part[p.part_rows * 129 + prow] = l;
       }
-      if (w.begins() && rank == 0 && warp == 0 && lane == 0)
-        *paged_record(p, worker) = PagedRecord{paged_parts(start, worker, w.blocks.n - (w.off + w.take)), w.req.q0 + t0, toks, w.h, {0, 0, 0, 0}};
     }
     tc_fence_before();
     arrive_local(kBarOStaged);
@@ -584,11 +582,12 @@ __device__ __forceinline__ void setup(const PagedParams& p, uint8_t* raw) {
     tma_prefetch_map(&p.tm_q);
     tma_prefetch_map(&p.tm_k);
     tma_prefetch_map(&p.tm_v);
-    if (rank == 0) paged_record(p, int(cluster_id_x()))->parts = 0;
   }
   // Rows of a Q tile that no box covers stay zeros.
   for (uint32_t i = tid; i < 2 * kQTileBytes / 16; i += kThreads) st_shared_v4(sm.base + kSmemQ + i * 16u, 0, 0, 0, 0);
   fence_proxy_async_smem();
+  grid_wait();
+  grid_release();
   find_start(p, int(cluster_id_x()), reinterpret_cast<int64_t*>(smem + kSmScan), reinterpret_cast<PagedStart*>(smem + kSmStart));
   if ((tid >> 5) == 0) {
     __syncwarp();
@@ -617,6 +616,7 @@ __device__ __forceinline__ void roles(const PagedParams& p, uint8_t* raw) {
       load(p, start, sm, wait, rank, lane);
     } else if (warp == kForwardWarp) {
       if (rank == 1) forward(p, start, sm, wait, lane);
+      else if (lane == 0) write_record(p, start, int(cluster_id_x()));
     } else if (rank == 0) {
       const uint32_t tmem = ld_volatile_shared(sm.tmem_slot());
       if (warp == kPVIssuerWarp) pv_issuer<kBf16>(p, start, sm, tmem, wait);
@@ -681,8 +681,7 @@ int paged_chunk_setup(int* pairs) {
 }
 
 int paged_chunk_launch(const PagedParams& p, bool bf16, cudaStream_t stream) {
-  paged_chunk_kernel(bf16)<<<2 * p.workers, kThreads, chunk::kBytes, stream>>>(p);
-  return int(cudaGetLastError());
+  return int(launch_early(paged_chunk_kernel(bf16), dim3(unsigned(2 * p.workers)), dim3(kThreads), chunk::kBytes, stream, p));
 }
 
 }  // namespace b200fa

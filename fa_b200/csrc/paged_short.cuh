@@ -159,7 +159,6 @@ __device__ __forceinline__ void short_rows(const PagedParams& p, const PagedStar
   auto bar_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kShortWarps * 32) : "memory"); };
   uint32_t g = 0;
   bool ok = true;
-  if (warp == 0 && lane == 0) paged_record(p, worker)->parts = 0;
 
   for (PagedWalk w(p, s); w.more(); w.next(p)) {
     const int t0 = w.tile * p.tokens_per_tile;
@@ -377,10 +376,6 @@ __device__ __forceinline__ void short_rows(const PagedParams& p, const PagedStar
           tail[p.part_rows + ra] = la_sum;
           tail[p.part_rows + rb] = lb_sum;
         }
-        if (w.begins() && warp == 0 && lane == 0) {
-          const int rest = w.blocks.n - (w.off + w.take);
-          *paged_record(p, worker) = PagedRecord{paged_parts(s, worker, rest), w.req.q0 + t0, tok, w.h, {0, 0, 0, 0}};
-        }
       }
     }
     // One decision for all eight warps: a warp that went on alone would wait
@@ -411,6 +406,8 @@ __device__ __forceinline__ void paged_short_body(const PagedParams& p) {
     tma_prefetch_map(&p.tm_k);
     tma_prefetch_map(&p.tm_v);
   }
+  grid_wait();
+  grid_release();
   PagedStart* start = reinterpret_cast<PagedStart*>(smem + kSmStart);
   find_start(p, int(blockIdx.x), reinterpret_cast<int64_t*>(smem + kSmScan), start);
   if (warp < kShortWarps) {
@@ -419,6 +416,7 @@ __device__ __forceinline__ void paged_short_body(const PagedParams& p) {
   } else {
     regs_decrease<kShortLoadRegs>();
     if (warp == kShortWarps) short_load(p, *start, sm, lane);
+    else if (threadIdx.x == kShortThreads - 1) write_record(p, *start, int(blockIdx.x));
   }
 }
 
