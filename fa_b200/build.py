@@ -39,6 +39,11 @@ DEBUG_LIB_NAME = "libb200fa_debug.so"
 DEBUG_LIB_PATH = BUILD_DIR / DEBUG_LIB_NAME
 DEBUG_MANIFEST = BUILD_DIR / "build_debug.json"
 DEBUG_FLAGS = ["-DB200FA_DEBUG"]
+CALLS_LIB_NAME = "fa_b200_calls.so"
+CALLS_LIB_PATH = BUILD_DIR / CALLS_LIB_NAME
+CALLS_MANIFEST = BUILD_DIR / "build_calls.json"
+CALLS_SOURCE = "torch_calls.cpp"
+CALLS_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH_FLAGS + [
@@ -135,6 +140,52 @@ def build(force: bool = False, verbose: bool = False, debug: bool = False) -> Pa
         return lib_path
 
 
+def build_calls(force: bool = False) -> Path:
+    """Compile the serving operators' Python module (``torch_calls.cpp``, host
+    code against torch's headers) when its source, the public header, torch or
+    Python changed; return its path."""
+    import sysconfig
+
+    import torch
+
+    source, header = CSRC / CALLS_SOURCE, INCLUDE / "b200fa.h"
+    h = hashlib.sha256()
+    for part in (source.read_bytes(), header.read_bytes(), torch.__version__.encode(),
+                 sysconfig.get_python_version().encode(), " ".join(CALLS_FLAGS).encode()):
+        h.update(part)
+    identity = h.hexdigest()
+
+    def current() -> bool:
+        try:
+            manifest = json.loads(CALLS_MANIFEST.read_text())
+            return manifest.get("identity") == identity and manifest.get("artifact_sha256") == _file_hash(CALLS_LIB_PATH)
+        except (OSError, ValueError):
+            return False
+
+    BUILD_DIR.mkdir(parents=True, exist_ok=True)
+    with open(BUILD_DIR / ".lock_calls", "a") as lock:
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        if not force and current():
+            return CALLS_LIB_PATH
+        root = Path(torch.__file__).resolve().parent
+        cuda_include = Path(nvcc_path()).resolve().parent.parent / "include"
+        with tempfile.TemporaryDirectory(dir=BUILD_DIR) as tmp:
+            out = Path(tmp) / CALLS_LIB_NAME
+            cmd = [os.environ.get("CXX", "g++"), *CALLS_FLAGS,
+                   *[f"-I{p}" for p in (INCLUDE, root / "include", root / "include/torch/csrc/api/include",
+                                        sysconfig.get_paths()["include"], cuda_include)],
+                   "-o", str(out), str(source), f"-L{root / 'lib'}", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda"]
+            res = subprocess.run(cmd, capture_output=True, text=True)
+            (BUILD_DIR / "build_calls.log").write_text(" ".join(cmd) + "\n" + res.stdout + res.stderr)
+            if res.returncode != 0:
+                raise RuntimeError(f"{cmd[0]} failed ({res.returncode}):\n{res.stderr[-4000:]}")
+            os.replace(out, CALLS_LIB_PATH)
+        CALLS_MANIFEST.write_text(json.dumps({"identity": identity, "artifact_sha256": _file_hash(CALLS_LIB_PATH),
+                                              "flags": CALLS_FLAGS, "sources": [CALLS_SOURCE]}, indent=2))
+        return CALLS_LIB_PATH
+
+
 if __name__ == "__main__":
     print(build(force=True, verbose=True))
+    print(build_calls(force=True))
     print(build(force=True, verbose=True, debug=True))

@@ -12,8 +12,6 @@ raise.
 from __future__ import annotations
 
 import ctypes as C
-import functools
-import struct
 import threading
 
 from . import build as _build
@@ -83,17 +81,6 @@ class PagedArgs(C.Structure):
 Strides2, Strides3 = _i64 * 2, _i64 * 3
 _s = C.POINTER(_i64)
 
-
-@functools.lru_cache(maxsize=4096)
-def strides(*values):
-    """The values as a C array (one per set of values: making one costs more than a light kernel's launch)."""
-    return (_i64 * len(values))(*values)
-
-
-# PagedArgs' bytes from its fields in one call (natural alignment, as C lays it out).
-paged_args = struct.Struct("@Ii4P2q2q3q3qPqPPqqiiiiiifiiIPQ")
-assert paged_args.size == C.sizeof(PagedArgs)
-
 SIGNATURES = {
     "b200fa_num_units": (_i64, [_i64, _i64, _i64]),
     "b200fa_partition": (C.c_int, [_i64, _i32, _i32, C.POINTER(_i64), C.POINTER(_i64)]),
@@ -119,7 +106,7 @@ SIGNATURES = {
     "b200fa_append": (C.c_int, [_p, _s, _p, _s, _p, _s, _p, _s, _p, _s, _p, _s, _i64, _i32, _i32, _i32, _i64, _i32,
                                 _p, _p, _i32, C.POINTER(RotaryDesc), _i32, _p]),
     "b200fa_paged_workspace_size": (_i64, []),
-    "b200fa_paged_fwd": (C.c_int, [_p, _p]),  # a PagedArgs, or its bytes
+    "b200fa_paged_fwd": (C.c_int, [C.POINTER(PagedArgs), _p]),
 }
 
 _lock = threading.Lock()

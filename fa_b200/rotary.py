@@ -22,10 +22,9 @@ import math
 
 import torch
 
-from . import lib
+from . import calls, lib
 
 LAYOUTS = {"half": 0, "interleaved": 1}
-DTYPES = {torch.float16: lib.DTYPE_FP16, torch.bfloat16: lib.DTYPE_BF16, torch.float32: lib.DTYPE_FP32}
 
 
 class Rotary:
@@ -69,6 +68,9 @@ class Rotary:
 
     def table(self, device) -> torch.Tensor:
         """The frequencies on ``device`` (made at its first use: outside a stream capture)."""
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError("a Rotary works on CUDA devices")
         t = self._tables.get(device)
         if t is None:
             if torch.cuda.is_current_stream_capturing():
@@ -78,13 +80,14 @@ class Rotary:
             self._tables[device] = t
         return t
 
-    def desc(self, device, inverse: bool = False) -> lib.RotaryDesc:
+    def desc(self, device, inverse: bool = False) -> int:
+        """Address of the C description (b200fa_rotary_desc) for ``device``."""
         d = self._descs.get((device, inverse))
         if d is None:
             d = lib.RotaryDesc(C.sizeof(lib.RotaryDesc), self.dim, self.rotary_dim, LAYOUTS[self.layout], int(inverse),
                                self.magnitude, self.table(device).data_ptr())
-            self._descs[(device, inverse)] = d
-        return d
+            d = self._descs[(device, inverse)] = (d, C.addressof(d))
+        return d[1]
 
     def __call__(self, x: torch.Tensor, positions: torch.Tensor | None = None, *, out: torch.Tensor | None = None,
                  inverse: bool = False) -> torch.Tensor:
@@ -94,56 +97,4 @@ class Rotary:
         int64 on x's device; None is 0 .. N-1.  out may be x.  ``inverse``
         turns back; with the magnitude it is the transposed map, so it carries
         a gradient of y to x."""
-        if x.ndim not in (3, 4) or x.shape[-1] != self.dim:
-            raise ValueError(f"x must be [B,H,N,{self.dim}] or [N,H,{self.dim}]")
-        dtype = DTYPES.get(x.dtype)
-        if dtype is None or x.device.type != "cuda":
-            raise ValueError("x must be FP16, BF16 or FP32 on a CUDA device")
-        if out is None:
-            out = torch.empty_like(x, memory_format=torch.contiguous_format)
-        elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
-            raise ValueError("out must be shaped and typed like x, on its device")
-        if x.ndim == 4:
-            B, H, N, _ = x.shape
-            xs, os = x.stride(), out.stride()
-            xs, os = (xs[0], xs[2], xs[1], xs[3]), (os[0], os[2], os[1], os[3])
-        else:
-            B, (N, H, _) = 1, x.shape
-            xs, os = (0, *x.stride()), (0, *out.stride())
-        if xs[3] != 1 or os[3] != 1:
-            raise ValueError("the last dimension of x and out must be contiguous")
-        bits, pos_ptr, pos_stride = 32, None, 0
-        if positions is not None:
-            bits = _position_bits(positions, x.device)
-            if positions.shape == (N,):
-                pass
-            elif positions.shape == (B, N):
-                pos_stride = N
-            else:
-                raise ValueError("positions must be [N] or [B,N]")
-            pos_ptr = positions.data_ptr()
-        call(x.device, "b200fa_rotary", x.data_ptr(), out.data_ptr(), B, N, H, lib.strides(*xs[:3]),
-             lib.strides(*os[:3]), pos_ptr, bits, pos_stride, self.desc(x.device, bool(inverse)), dtype)
-        return out
-
-
-def call(device, name: str, *args) -> None:
-    """Calls a C entry on the device's current stream (its last argument) with
-    the device current; raises on a nonzero status.  The device is switched
-    only when another one is current: the context manager takes longer than
-    the call."""
-    so = lib.load()
-    index = device.index
-    if torch._C._cuda_getDevice() == index:
-        status = getattr(so, name)(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(device):
-            status = getattr(so, name)(*args, torch._C._cuda_getCurrentRawStream(index))
-    if status:
-        lib.check(status, name)
-
-
-def _position_bits(positions, device) -> int:
-    if positions.dtype not in (torch.int32, torch.int64) or positions.device != device or not positions.is_contiguous():
-        raise ValueError("positions must be contiguous int32 or int64 on the same device")
-    return 64 if positions.dtype == torch.int64 else 32
+        return calls.load().rotary(x, positions, out, self.desc(x.device, bool(inverse)))
