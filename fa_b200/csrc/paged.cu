@@ -164,8 +164,9 @@ int check_paged(const b200fa_paged_args& a) {
   const int64_t most = (int64_t(1) << 31) - 1;
   if (a.page_size < 8 || a.page_size > (1 << 20) || (a.page_size & (a.page_size - 1)))
     return fail(B200FA_ERR_PAGE_SIZE, "page size must be a power of two in [8, 2^20], got %d", a.page_size);
-  if (a.tokens > most || a.num_pages >= most || a.requests > B200FA_MAX_REQUESTS || int64_t(a.width) * a.page_size > most)
-    return fail(B200FA_ERR_TOO_LARGE, "tokens, pages and keys of a request must be below 2^31, requests at most %d", B200FA_MAX_REQUESTS);
+  if (a.tokens > most || a.num_pages >= most || a.requests > B200FA_MAX_REQUESTS || int64_t(a.width) * a.page_size > most - 1023)  // key indices run up to a block past the last key
+    return fail(B200FA_ERR_TOO_LARGE, "tokens and pages must be below 2^31, keys of a table row below 2^31 - 1023, requests at most %d",
+                B200FA_MAX_REQUESTS);
   if (a.window < 0 || a.sinks < 0 || (a.sinks > 0 && a.window == 0))
     return fail(B200FA_ERR_OPTIONS, "window %d, sinks %d: both at least 0, sinks only with a window", a.window, a.sinks);
   if (!std::isfinite(a.scale) || !(a.scale > 0.f)) return fail(B200FA_ERR_SCALE, "scale must be finite and positive");

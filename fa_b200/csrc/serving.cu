@@ -330,6 +330,13 @@ int check_strides(const int64_t* s, int count, int64_t unit, const char* what) {
   return B200FA_OK;
 }
 
+// A written tensor's rows must not share memory.
+int check_distinct(const int64_t* s, const int64_t* sizes, int count, const char* what) {
+  for (int i = 0; i < count; ++i)
+    if (s[i] == 0 && sizes[i] > 1) return fail(B200FA_ERR_STRIDE, "%s is written and must not be expanded", what);
+  return B200FA_OK;
+}
+
 // Tokens of a block: one where there are few (the shortest chain), else enough
 // for about 288 rows, within 16 KiB of angles.
 int launch_rotary(RotaryParams& p, const b200fa_rotary_desc* r, int32_t dim, int32_t dtype, void* stream) {
@@ -420,6 +427,8 @@ int b200fa_rotary(const void* x, void* out, int64_t batch, int64_t n, int64_t he
   const int64_t unit = 16 / element_size(dtype);
   if ((rc = check_strides(x_strides, 3, unit, "x")) != B200FA_OK) return rc;
   if ((rc = check_strides(out_strides, 3, unit, "out")) != B200FA_OK) return rc;
+  const int64_t sizes[3] = {batch, n, heads};
+  if ((rc = check_distinct(out_strides, sizes, 3, "out")) != B200FA_OK) return rc;
   RotaryParams p{};
   p.seg[0] = Segment{x, out, x_strides[0], x_strides[1], x_strides[2], out_strides[0], out_strides[1], out_strides[2],
                      int32_t(heads), 1, 0};
@@ -461,6 +470,10 @@ int b200fa_append(const void* q, const int64_t* q_strides, void* q_out, const in
   if ((q && ((rc = check_strides(q_strides, 2, 8, "q")) || (rc = check_strides(q_out_strides, 2, 8, "q_out")))) ||
       (rc = check_strides(k_strides, 2, 8, "k")) || (rc = check_strides(v_strides, 2, 8, "v")) ||
       (rc = check_strides(k_page_strides, 3, 8, "k_pages")) || (rc = check_strides(v_page_strides, 3, 8, "v_pages")))
+    return rc;
+  const int64_t rows[2] = {tokens, heads_q}, pages[3] = {num_pages, page_size, heads_kv};
+  if ((q && (rc = check_distinct(q_out_strides, rows, 2, "q_out"))) || (rc = check_distinct(k_page_strides, pages, 3, "k_pages")) ||
+      (rc = check_distinct(v_page_strides, pages, 3, "v_pages")))
     return rc;
   RotaryParams p{};
   int n = 0;

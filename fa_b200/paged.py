@@ -115,7 +115,7 @@ class PagedOperator:
         as the host knows: it picks the kernel, a longer one is still right.
 
         Rows that see no key become zeros; rows of no request (behind
-        cu_q[R]) are left as they were in ``out``.  A page that holds no key
+        cu_q[R]) are left as they were in ``out``, and undefined without it.  A page that holds no key
         any row of its work item sees is not read.  Where the table ends early
         or names a page outside the cache, zeros are read and
         ``status(device)`` says so.  A NaN or infinity in V at a key that some

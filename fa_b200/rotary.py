@@ -27,6 +27,22 @@ from . import calls, lib
 LAYOUTS = {"half": 0, "interleaved": 1}
 
 
+class _Turn(torch.autograd.Function):
+    """The rotation for autograd: its backward pass is the other direction."""
+
+    @staticmethod
+    def forward(ctx, x, positions, rotary, inverse):
+        ctx.save_for_backward(*([] if positions is None else [positions]))
+        ctx.rotary, ctx.inverse = rotary, inverse
+        return calls.load().rotary(x, positions, None, rotary.desc(x.device, inverse))
+
+    @staticmethod
+    def backward(ctx, grad):
+        # A gradient may come expanded or transposed; the kernel reads rows of whole 16 bytes.
+        saved = ctx.saved_tensors
+        return ctx.rotary(grad.contiguous(), saved[0] if saved else None, inverse=not ctx.inverse), None, None, None
+
+
 class Rotary:
     """``rotary(x, positions) -> y`` with y shaped like x.
 
@@ -96,5 +112,10 @@ class Rotary:
         other strides of whole 16 bytes.  positions: [N] or [B,N], int32 or
         int64 on x's device; None is 0 .. N-1.  out may be x.  ``inverse``
         turns back; with the magnitude it is the transposed map, so it carries
-        a gradient of y to x."""
+        a gradient of y to x: that is what autograd runs when x requires a
+        gradient (out must then be None)."""
+        if x.requires_grad and torch.is_grad_enabled():
+            if out is not None:
+                raise ValueError("out cannot be given when x requires a gradient")
+            return _Turn.apply(x, positions, self, bool(inverse))
         return calls.load().rotary(x, positions, out, self.desc(x.device, bool(inverse)))

@@ -189,6 +189,42 @@ def test_rotary_inverse_is_the_gradient(layout):
 
 
 @gpu
+@pytest.mark.parametrize("inverse", [False, True])
+def test_rotary_under_autograd(inverse):
+    rotary, freq, _ = _rotary(32, 32, "half", SCALINGS[2])
+    x = torch.randn((2, 3, 7, 32), device="cuda", requires_grad=True)
+    pos = torch.arange(7, device="cuda") * 37
+    for grad in (torch.randn_like(x), torch.ones((1,), device="cuda").expand(2, 3, 7, 32)):
+        y = rotary(x, pos, inverse=inverse)
+        assert torch.equal(y.detach(), rotary(x.detach(), pos, inverse=inverse))
+        (got,) = torch.autograd.grad(y, x, grad)
+        assert torch.equal(got, rotary(grad.contiguous(), pos, inverse=not inverse))
+        xx = x.detach().transpose(1, 2).contiguous().transpose(1, 2).requires_grad_()
+        rotary(xx).sum().backward()
+        assert torch.equal(xx.grad, rotary(torch.ones_like(x).detach(), inverse=True))
+    with pytest.raises(ValueError):
+        rotary(x, pos, out=torch.empty_like(x))
+    with torch.no_grad():
+        rotary(x, pos, out=torch.empty_like(x))
+
+
+@gpu
+def test_written_tensors_must_not_be_expanded():
+    from fa_b200 import lib
+    from fa_b200.paged import append
+
+    rotary, _, _ = _rotary(128, 128, "half", {})
+    x = torch.randn((2, 3, 4, 128), device="cuda").half()
+    with pytest.raises(lib.B200FAError):
+        rotary(x, out=torch.empty((1, 3, 4, 128), dtype=F16, device="cuda").expand(2, -1, -1, -1))
+    assert torch.equal(rotary(x[:1].expand(2, -1, -1, -1)), rotary(x[:1].repeat(2, 1, 1, 1)))
+    k = torch.randn((4, 2, 128), device="cuda").half()
+    pages = torch.zeros((1, 8, 2, 128), dtype=F16, device="cuda").expand(3, -1, -1, -1)
+    with pytest.raises(lib.B200FAError):
+        append(k, k, pages, pages, torch.arange(4, device="cuda"))
+
+
+@gpu
 def test_rotary_inside_the_dense_operator():
     from fa_b200.ops import Operator
 
@@ -325,6 +361,17 @@ LENGTHS = {
     "rows_before_the_cache": [(9, 4), (3, 0), (2, 50)],
     "many": [(1 + i % 3, 10 + 37 * i) for i in range(40)],
 }
+
+
+@gpu
+@pytest.mark.parametrize("lens,hq,hkv,ps,window", [
+    ([(1, 1 + 7 * i % 400) for i in range(1500)], 4, 4, 16, 0),           # more requests than threads of a block
+    ([(2 if i % 3 else 0, 3 + i % 90) for i in range(900)], 6, 1, 8, 50),
+    ([(3, 700), (1, 40), (9, 2000)], 128, 1, 32, 0),                      # one token per tile and CTA
+    ([(3, 700), (1, 40), (9, 2000)], 100, 1, 16, 129),
+    ([(5, 600), (200, 900)], 65, 65, 64, 0)])
+def test_paged_many_requests_and_wide_groups(lens, hq, hkv, ps, window):
+    _check_paged(_paged_case(lens, hq, hkv, ps, F16, 31, spare_rows=1), window, 3 if window else 0)
 
 
 @gpu
@@ -552,7 +599,7 @@ def _args(**kw):
 @pytest.mark.parametrize("kw,code", [
     ({"struct_size": 8}, -11), ({"dtype": 2}, -14), ({"requests": -1}, -3), ({"width": 0}, -3), ({"heads_kv": 3}, -4),
     ({"heads_q": 512}, -4), ({"page_size": 24}, -15), ({"page_size": 4}, -15), ({"tokens": 2**31}, -5),
-    ({"requests": 5000}, -5), ({"width": 2**30}, -5), ({"window": -1}, -11), ({"sinks": 3}, -11), ({"scale": 0.0}, -10),
+    ({"requests": 5000}, -5), ({"width": 2**30}, -5), ({"width": 2**27}, -5), ({"window": -1}, -11), ({"sinks": 3}, -11), ({"scale": 0.0}, -10),
     ({"q": None}, -1), ({"kv_lens": None}, -1), ({"o": 8}, -7), ({"table_stride": 3}, -16), ({"q_strides": (100, 128)}, -16),
     ({"k_strides": (2048, 0, 128)}, -16), ({"workspace": None}, -8), ({"workspace": 128}, -8)])
 def test_paged_validation_codes_without_gpu(kw, code):
