@@ -324,9 +324,25 @@ int fill_params(const void* q, const void* k, const void* v, void* o, int64_t B,
 }
 
 int launch(int32_t variant, const FwdParams& p, int grid, void* stream, const char* where) {
-  kernel_for(variant, p.capture != nullptr, (p.flags & kFlagCausal) != 0, (p.flags & kFlagWindow) != 0)
-      <<<grid, kThreads, kSmemBytes, static_cast<cudaStream_t>(stream)>>>(p);
-  const cudaError_t e = cudaGetLastError();
+  cudaError_t e;
+  if (p.flags & kFlagWindow) {
+    // Its setup may overlap the end of the work before it; it waits inside.
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(unsigned(grid));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmemBytes;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, b200_fa_window_kernel, p);
+  } else {
+    kernel_for(variant, p.capture != nullptr, (p.flags & kFlagCausal) != 0)<<<grid, kThreads, kSmemBytes,
+                                                                            static_cast<cudaStream_t>(stream)>>>(p);
+    e = cudaGetLastError();
+  }
   if (e != cudaSuccess) return cuda_fail(e, where);
   return B200FA_OK;
 }

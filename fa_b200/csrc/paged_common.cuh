@@ -24,12 +24,6 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-// All work ahead of this grid in the stream is done and its writes are seen.
-__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-// The next grid in the stream may start (it waits for this one's end itself).
-__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // Two floats rounded to the cache's type (lo in bits 0..15).
 template <bool kBf16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {

@@ -102,7 +102,8 @@ class Operator:
         ``causal``): only keys i - window < j <= i of those, and the first
         ``sinks`` keys; a row that sees no key (Nq > Nk) gets zeros, and key
         blocks that no row of a work item sees are not read; softmax sums are
-        FP32 in both variants.  ``rotary`` (a
+        FP32 in both variants.  (A NaN or infinity in V at a key that some row
+        of a work item of 256 rows sees can reach all of them.)  ``rotary`` (a
         ``fa_b200.rotary.Rotary``): Q and K are turned by it first, into new
         tensors, by ``positions`` ([N] or [B, N]; None: 0 .. N-1; given
         positions need Nq == Nk).  ``capture`` (FP32, at least
