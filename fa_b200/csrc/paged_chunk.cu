@@ -12,7 +12,8 @@
 //     pair.  A Q tile is one box of the [tokens][heads_kv][group][128] view,
 //     so its rows land in the order token * group + head.
 //   * K and V come page by page, a box (K: one per 64 columns) for each page
-//     of a block; the producer warp reads the block table 32 entries ahead.
+//     of a block, K and V by a warp each, which read the block table 32
+//     entries ahead.
 //   * V rows behind the last key that any row sees are cleared in shared
 //     memory before the product (0 * NaN is no 0), in an item's last
 //     stage: by the PV issuer's warp for rank 0, by the forwarding warp for
@@ -46,8 +47,8 @@ constexpr int kSmXchg = kSmBar + kBars * 8;             // float [2][128]
 constexpr int kSmTmem = kSmXchg + 2 * kBlockM * 4;      // TMEM base, abort flag
 constexpr int kSmStart = kSmTmem + 16;                  // PagedStart
 constexpr int kSmScan = kSmStart + 64;                  // int64 [12]
-constexpr int kSmPages = kSmScan + (kThreads / 32) * 8;  // 32 page numbers
-constexpr int kSmUsed = kSmPages + 128;
+constexpr int kSmPages = kSmScan + (kThreads / 32) * 8;  // 32 page numbers for each producer
+constexpr int kSmUsed = kSmPages + 256;
 constexpr int kBytes = kSmUsed + 1024;
 static_assert(kBytes <= 232448, "shared memory budget exceeded");
 static_assert(kSmBar % 8 == 0 && kSmStart % 8 == 0 && kSmScan % 8 == 0 && sizeof(PagedStart) <= 64, "layout");
@@ -61,7 +62,7 @@ struct Sm {
   __device__ __forceinline__ uint32_t xchg(uint32_t slot, int row) const { return base + kSmXchg + (slot * kBlockM + uint32_t(row)) * 4u; }
   __device__ __forceinline__ uint32_t tmem_slot() const { return base + kSmTmem; }
   __device__ __forceinline__ uint32_t abort_slot() const { return base + kSmTmem + 4; }
-  __device__ __forceinline__ uint32_t pages() const { return base + kSmPages; }
+  __device__ __forceinline__ uint32_t pages(bool v) const { return base + kSmPages + (v ? 128 : 0); }
 };
 
 __device__ __forceinline__ Sm sm_of(uint8_t* raw) { return Sm{(smem_addr(raw) + 1023u) & ~1023u}; }
@@ -235,15 +236,20 @@ __device__ __forceinline__ void forward(const PagedParams& p, const PagedStart& 
   }
 }
 
-// Both ranks, a whole warp: this CTA's Q tiles and its halves of every block.
+// Both ranks, a warp each for Q and K and for V: this CTA's Q tiles and its
+// halves of every block.  Two warps because a block of small pages is many
+// copies (16-token pages: 8 of K, 8 of V), which one thread issued in more time
+// than the products take (1.36 us a block of 16-token pages against 1.07 of
+// 64-token ones).
+template <bool kV>
 __device__ __forceinline__ void load(const PagedParams& p, const PagedStart& start, const Sm& sm, const Wait& wait,
-                                     uint32_t rank, uint32_t lane) {
-  const uint32_t site = (rank << 16) | (uint32_t(kLoadWarp) << 8);
+                                     uint32_t rank, uint32_t warp, uint32_t lane) {
+  const uint32_t site = (rank << 16) | (warp << 8);
   const int half_tok = p.tokens_per_tile / 2;
   const uint32_t q_bytes = uint32_t(half_tok * p.group) * 256u;
   const int size_mask = (1 << p.page_shift) - 1;
   const int k_rows = p.page_shift < 6 ? 1 << p.page_shift : kPairKeys;  // of a K box: this rank's keys of a page
-  uint32_t g0 = 0, issued_k = 0, issued_v = 0, q_issued = 0;  // issued_*: in the issuing lane
+  uint32_t g0 = 0, issued = 0, q_issued = 0;  // issued, q_issued: in the issuing lane
   bool ok = true;
   int it = 0;
   // Bounded wait for a free stage, then the announcement of its bytes.
@@ -252,12 +258,12 @@ __device__ __forceinline__ void load(const PagedParams& p, const PagedStart& sta
     mbar_arrive_expect_tx(sm.bar(full), bytes);
     return true;
   };
-  PageFeed feed(p, sm.pages());
+  PageFeed feed(p, sm.pages(kV));
   const int k_first = feed.per > 1 ? int(rank) * (feed.per / 2) : 0, k_pages = kPairKeys / k_rows;
   for (PagedWalk w(p, start); ok && w.more(); w.next(p), ++it) {
-    const int qt = it & 1;
     feed.begin(w, lane);
-    if (elect_one()) {
+    if (!kV && elect_one()) {
+      const int qt = it & 1;
       if ((ok = claim(kBarQEmpty + qt, (uint32_t(it >> 1) & 1u) ^ 1u, kBarQFull + qt, q_bytes))) {
         const int tok = w.req.q0 + w.tile * p.tokens_per_tile + int(rank) * half_tok;
         tma_load_4d(sm.q(qt), &p.tm_q, sm.bar(kBarQFull + qt), 0, 0, w.h, tok);
@@ -272,25 +278,26 @@ __device__ __forceinline__ void load(const PagedParams& p, const PagedStart& sta
       if (elect_one()) {
         for (int j = 0; j < n; ++j) {
           const uint32_t g = g0 + uint32_t(j), e = ring_entry(g);
-          const int key0 = w.blocks.key_block(w.off + j0 + j) * kPagedBlock;
-          // Rank 1's V is handed over by its warp 11; rank 0's where it needs clearing.
-          const bool hand = rank == 1 || w.blocks.end_key < key0 + kPagedBlock;
-          const int v_bar = (hand ? kBarVLand : kBarVFull) + int(e);
-          if (!(ok = claim(kBarKEmpty + int(e), ring_parity(g) ^ 1u, kBarKFull + int(e), kStageBytes))) break;
-          uint32_t dst = sm.k(e);
-          int key = key0 + int(rank) * kPairKeys;
-          for (int i = 0; i < k_pages; ++i, dst += uint32_t(k_rows) * 128u, key += k_rows) {
-            const int page = feed(j, k_first + i);
-            tma_load_4d(dst, &p.tm_k, sm.bar(kBarKFull + int(e)), 0, key & size_mask, w.h, page);
-            tma_load_4d(dst + kKBoxBytes, &p.tm_k, sm.bar(kBarKFull + int(e)), 64, key & size_mask, w.h, page);
+          int key = w.blocks.key_block(w.off + j0 + j) * kPagedBlock;
+          if constexpr (!kV) {
+            if (!(ok = claim(kBarKEmpty + int(e), ring_parity(g) ^ 1u, kBarKFull + int(e), kStageBytes))) break;
+            uint32_t dst = sm.k(e);
+            key += int(rank) * kPairKeys;
+            for (int i = 0; i < k_pages; ++i, dst += uint32_t(k_rows) * 128u, key += k_rows) {
+              const int page = feed(j, k_first + i);
+              tma_load_4d(dst, &p.tm_k, sm.bar(kBarKFull + int(e)), 0, key & size_mask, w.h, page);
+              tma_load_4d(dst + kKBoxBytes, &p.tm_k, sm.bar(kBarKFull + int(e)), 64, key & size_mask, w.h, page);
+            }
+          } else {
+            // Rank 1's V is handed over by its warp 11; rank 0's where it needs clearing.
+            const bool hand = rank == 1 || w.blocks.end_key < key + kPagedBlock;
+            const int bar = (hand ? kBarVLand : kBarVFull) + int(e);
+            if (!(ok = claim(kBarVEmpty + int(e), ring_parity(g) ^ 1u, bar, kStageBytes))) break;
+            uint32_t dst = sm.v(e);
+            for (int i = 0; i < feed.per; ++i, dst += uint32_t(feed.rows) * 128u, key += feed.rows)
+              tma_load_4d(dst, &p.tm_v, sm.bar(bar), int(rank) * kPairDims, key & size_mask, w.h, feed(j, i));
           }
-          ++issued_k;
-          if (!(ok = claim(kBarVEmpty + int(e), ring_parity(g) ^ 1u, v_bar, kStageBytes))) break;
-          dst = sm.v(e);
-          key = key0;
-          for (int i = 0; i < feed.per; ++i, dst += uint32_t(feed.rows) * 128u, key += feed.rows)
-            tma_load_4d(dst, &p.tm_v, sm.bar(v_bar), int(rank) * kPairDims, key & size_mask, w.h, feed(j, i));
-          ++issued_v;
+          ++issued;
         }
       }
       ok = __all_sync(0xffffffffu, ok);
@@ -299,12 +306,9 @@ __device__ __forceinline__ void load(const PagedParams& p, const PagedStart& sta
   }
   // The last copies land before the CTA exits, also when a role gave up.
   if (elect_one()) {
-    for (uint32_t i = issued_k > kRing ? issued_k - kRing : 0; i < issued_k; ++i)
-      wait.drain(sm.bar(kBarKFull + int(ring_entry(i))), ring_parity(i));
-    for (uint32_t i = issued_v > kRing ? issued_v - kRing : 0; i < issued_v; ++i)
-      wait.drain(sm.bar((rank == 1 ? kBarVLand : kBarVFull) + int(ring_entry(i))), ring_parity(i));
-    for (uint32_t i = q_issued > 2 ? q_issued - 2 : 0; i < q_issued; ++i)
-      wait.drain(sm.bar(kBarQFull + int(i & 1u)), (i >> 1) & 1u);
+    const int full = kV ? (rank == 1 ? kBarVLand : kBarVFull) : kBarKFull;
+    for (uint32_t i = issued > kRing ? issued - kRing : 0; i < issued; ++i) wait.drain(sm.bar(full + int(ring_entry(i))), ring_parity(i));
+    for (uint32_t i = q_issued > 2 ? q_issued - 2 : 0; i < q_issued; ++i) wait.drain(sm.bar(kBarQFull + int(i & 1u)), (i >> 1) & 1u);
   }
   __syncwarp();
 }
@@ -613,11 +617,14 @@ __device__ __forceinline__ void roles(const PagedParams& p, uint8_t* raw) {
     const Wait wait{sm.abort_slot(), &p};
     const PagedStart& start = *start_of(raw);
     if (warp == kLoadWarp) {
-      load(p, start, sm, wait, rank, lane);
+      load<false>(p, start, sm, wait, rank, warp, lane);
+    } else if (warp == (rank == 0 ? kForwardWarp : kPVIssuerWarp)) {
+      load<true>(p, start, sm, wait, rank, warp, lane);
     } else if (warp == kForwardWarp) {
-      if (rank == 1) forward(p, start, sm, wait, lane);
-      else if (lane == 0) write_record(p, start, int(cluster_id_x()));
-    } else if (rank == 0) {
+      forward(p, start, sm, wait, lane);
+    } else if (rank == 1) {
+      if (lane == 0) write_record(p, start, int(cluster_id_x()));
+    } else {
       const uint32_t tmem = ld_volatile_shared(sm.tmem_slot());
       if (warp == kPVIssuerWarp) pv_issuer<kBf16>(p, start, sm, tmem, wait);
       else if (elect_one()) s_issuer<kBf16>(p, start, sm, tmem, wait);
