@@ -154,10 +154,12 @@ __global__ void __launch_bounds__(kTableThreads) b200_build_tables_kernel(const 
 // the position, where a 32-bit product of position and frequency is off by
 // position * 2^-24 radians (0.008 at 131072).
 struct Segment {  // a run of heads: rows [batch][n][heads][dim] -> the same, or the cache
-  const void* src;
-  void* dst;
-  int64_t src_b, src_n, src_h;
-  int64_t dst_b, dst_n, dst_h;  // scattered: page, token, head
+  const uint4* src;
+  uint4* dst;
+  // In units of 16 bytes: 32 bits reach 32 GB, and index times stride is one
+  // instruction (the kernel is close to its issue rate).
+  int32_t src_b, src_n, src_h;
+  int32_t dst_b, dst_n, dst_h;  // scattered: page, token, head
   int32_t heads;
   int32_t rotate, scatter;
 };
@@ -189,12 +191,21 @@ struct Sixteen {  // 16 elements as 16-byte pieces
   uint4 v[kPieces];
 };
 
-__device__ __forceinline__ void to_float(float x, float& o) { o = x; }
-__device__ __forceinline__ void to_float(__half x, float& o) { o = __half2float(x); }
-__device__ __forceinline__ void to_float(__nv_bfloat16 x, float& o) { o = __bfloat162float(x); }
-__device__ __forceinline__ void from_float(float x, float& o) { o = x; }
-__device__ __forceinline__ void from_float(float x, __half& o) { o = __float2half_rn(x); }
-__device__ __forceinline__ void from_float(float x, __nv_bfloat16& o) { o = __float2bfloat16_rn(x); }
+template <typename T>
+struct Two;
+template <>
+struct Two<float> { using type = float2; };
+template <>
+struct Two<__half> { using type = __half2; };
+template <>
+struct Two<__nv_bfloat16> { using type = __nv_bfloat162; };
+
+__device__ __forceinline__ float2 to_float2(float2 x) { return x; }
+__device__ __forceinline__ float2 to_float2(__half2 x) { return __half22float2(x); }
+__device__ __forceinline__ float2 to_float2(__nv_bfloat162 x) { return __bfloat1622float2(x); }
+__device__ __forceinline__ void from_float2(float2 x, float2& o) { o = x; }
+__device__ __forceinline__ void from_float2(float2 x, __half2& o) { o = __float22half2_rn(x); }
+__device__ __forceinline__ void from_float2(float2 x, __nv_bfloat162& o) { o = __float22bfloat162_rn(x); }
 
 // kLayout 0: a thread's pairs are elements (8 c + i, rot/2 + 8 c + i); 1:
 // (16 c + 2 i, 16 c + 2 i + 1).  Lanes at or behind rot copy elements 16 c ...
@@ -218,12 +229,12 @@ __global__ void __launch_bounds__(256) b200_rotary_kernel(const RotaryParams p) 
   // the tokens first where those are closer in memory than the heads.
   const int c = int(threadIdx.x) % p.lanes, step = 256 / p.lanes;
   const bool turn = 16 * c < p.rot, active = int(threadIdx.x) / p.lanes < step;
-  // Element offsets of the thread's first and second eight elements.
-  const int lo = (turn && kLayout == 0) ? 8 * c : 16 * c;
-  const int hi = (turn && kLayout == 0) ? pairs + 8 * c : 16 * c + 8;
+  // Where the thread's first and second eight elements are, in 16 bytes.
+  const int lo = ((turn && kLayout == 0) ? 8 * c : 16 * c) / kPer;
+  const int hi = ((turn && kLayout == 0) ? pairs + 8 * c : 16 * c + 8) / kPer;
   const int inners = p.tokens_first ? tokens : p.heads, outers = p.tokens_first ? p.heads : tokens;
   struct Row {
-    T* dst;  // NULL: none, or skipped
+    uint4* dst;  // NULL: none, or skipped
     int t;
     bool turned;
     Sixteen<T> x;
@@ -238,27 +249,26 @@ __global__ void __launch_bounds__(256) b200_rotary_kernel(const RotaryParams p) 
     inner += step;
     while (k + 1 < p.segments && hh >= p.seg[k].heads) hh -= p.seg[k++].heads;
     const Segment& s = p.seg[k];
-    int64_t b = tok_b[row.t];
-    const int64_t n = tok_n[row.t];
+    int b = tok_b[row.t];
+    const int n = tok_n[row.t];
     if (p.batched) {  // a token of all sequences: heads run over (sequence, head)
       b = hh / s.heads;
-      hh -= int(b) * s.heads;
+      hh -= b * s.heads;
     }
-    T* dst = static_cast<T*>(s.dst);
     row.dst = nullptr;
+    uint4* dst = s.dst;
     if (s.scatter) {
       const int64_t slot = tok_slot[row.t];
       if (slot < 0 || slot >= p.num_slots) return true;
-      dst += (slot >> p.shift) * s.dst_b + (slot & ((int64_t(1) << p.shift) - 1)) * s.dst_n + hh * s.dst_h;
+      dst += int64_t(int32_t(slot >> p.shift)) * s.dst_b + int64_t(int32_t(slot) & ((1 << p.shift) - 1)) * s.dst_n + int64_t(hh) * s.dst_h;
     } else {
-      dst += b * s.dst_b + n * s.dst_n + hh * s.dst_h;
+      dst += int64_t(b) * s.dst_b + int64_t(n) * s.dst_n + int64_t(hh) * s.dst_h;
     }
     row.dst = dst;
     row.turned = s.rotate && turn;
-    const T* src = static_cast<const T*>(s.src) + b * s.src_b + n * s.src_n + hh * s.src_h;
+    const uint4* src = s.src + int64_t(b) * s.src_b + int64_t(n) * s.src_n + int64_t(hh) * s.src_h;
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u)
-      row.x.v[u] = __ldcs(reinterpret_cast<const uint4*>(src + (u < kPieces / 2 ? lo + u * kPer : hi + (u - kPieces / 2) * kPer)));
+    for (int u = 0; u < kPieces; ++u) row.x.v[u] = __ldcs(src + (u < kPieces / 2 ? lo + u : hi + (u - kPieces / 2)));
     return true;
   };
   Row row;
@@ -284,27 +294,26 @@ __global__ void __launch_bounds__(256) b200_rotary_kernel(const RotaryParams p) 
     have = load(row);  // the next row's loads before this one's stores
     if (cur.dst == nullptr) continue;
     if (cur.turned) {
-      T* e = reinterpret_cast<T*>(cur.x.v);
+      using T2 = typename Two<T>::type;
+      T2* e = reinterpret_cast<T2*>(cur.x.v);
       const float4* a4 = reinterpret_cast<const float4*>(angles + cur.t * pairs + 8 * c);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const float4 a = a4[u];  // two pairs
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const float cs = w ? a.z : a.x, sn = w ? a.w : a.y;
-          T& y = e[kLayout == 0 ? 2 * u + w : 4 * u + 2 * w];
-          T& z = e[kLayout == 0 ? 8 + 2 * u + w : 4 * u + 2 * w + 1];
-          float f, g;
-          to_float(y, f);
-          to_float(z, g);
-          from_float(f * cs - g * sn, y);
-          from_float(g * cs + f * sn, z);
+        const float4 a = a4[u];  // cos, sin of two pairs
+        if constexpr (kLayout == 0) {
+          const float2 f = to_float2(e[u]), g = to_float2(e[4 + u]);
+          from_float2(make_float2(f.x * a.x - g.x * a.y, f.y * a.z - g.y * a.w), e[u]);
+          from_float2(make_float2(g.x * a.x + f.x * a.y, g.y * a.z + f.y * a.w), e[4 + u]);
+        } else {
+          const float2 f = to_float2(e[2 * u]), g = to_float2(e[2 * u + 1]);
+          from_float2(make_float2(f.x * a.x - f.y * a.y, f.y * a.x + f.x * a.y), e[2 * u]);
+          from_float2(make_float2(g.x * a.z - g.y * a.w, g.y * a.z + g.x * a.w), e[2 * u + 1]);
         }
       }
     }
 #pragma unroll
     for (int u = 0; u < kPieces; ++u)
-      __stcs(reinterpret_cast<uint4*>(cur.dst + (u < kPieces / 2 ? lo + u * kPer : hi + (u - kPieces / 2) * kPer)), cur.x.v[u]);
+      __stcs(cur.dst + (u < kPieces / 2 ? lo + u : hi + (u - kPieces / 2)), cur.x.v[u]);
   }
 }
 
@@ -325,9 +334,17 @@ int check_rotary(const b200fa_rotary_desc* r, int32_t dim) {
 
 int check_strides(const int64_t* s, int count, int64_t unit, const char* what) {
   for (int i = 0; i < count; ++i)
-    if (s[i] < 0 || s[i] % unit)
-      return fail(B200FA_ERR_STRIDE, "%s: stride %lld is not a non-negative multiple of 16 bytes", what, (long long)s[i]);
+    if (s[i] < 0 || s[i] % unit || s[i] / unit > kInt32Max)
+      return fail(B200FA_ERR_STRIDE, "%s: stride %lld is not a multiple of 16 bytes from 0 to 32 GB", what, (long long)s[i]);
   return B200FA_OK;
+}
+
+// Strides (batch, n, heads) or (page, token, head) in elements of 16 / unit bytes.
+Segment segment(const void* src, void* dst, const int64_t (&s)[3], const int64_t (&d)[3], int64_t unit, int64_t heads, bool rotate,
+                bool scatter) {
+  return Segment{static_cast<const uint4*>(src), static_cast<uint4*>(dst), int32_t(s[0] / unit), int32_t(s[1] / unit),
+                 int32_t(s[2] / unit), int32_t(d[0] / unit), int32_t(d[1] / unit), int32_t(d[2] / unit), int32_t(heads),
+                 int32_t(rotate), int32_t(scatter)};
 }
 
 // A written tensor's rows must not share memory.
@@ -430,8 +447,8 @@ int b200fa_rotary(const void* x, void* out, int64_t batch, int64_t n, int64_t he
   const int64_t sizes[3] = {batch, n, heads};
   if ((rc = check_distinct(out_strides, sizes, 3, "out")) != B200FA_OK) return rc;
   RotaryParams p{};
-  p.seg[0] = Segment{x, out, x_strides[0], x_strides[1], x_strides[2], out_strides[0], out_strides[1], out_strides[2],
-                     int32_t(heads), 1, 0};
+  p.seg[0] = segment(x, out, {x_strides[0], x_strides[1], x_strides[2]}, {out_strides[0], out_strides[1], out_strides[2]}, unit,
+                     heads, true, false);
   p.segments = 1;
   // Sequences with the same positions share the angles.
   p.batched = (!positions || pos_stride == 0) && batch > 1 && batch * heads <= kInt32Max;
@@ -477,12 +494,13 @@ int b200fa_append(const void* q, const int64_t* q_strides, void* q_out, const in
     return rc;
   RotaryParams p{};
   int n = 0;
-  p.seg[n++] = Segment{k, k_pages, 0, k_strides[0], k_strides[1], k_page_strides[0], k_page_strides[1],
-                       k_page_strides[2], heads_kv, rotary != nullptr, 1};
-  p.seg[n++] = Segment{v, v_pages, 0, v_strides[0], v_strides[1], v_page_strides[0], v_page_strides[1],
-                       v_page_strides[2], heads_kv, 0, 1};
-  if (q) p.seg[n++] = Segment{q, q_out, 0, q_strides[0], q_strides[1], 0, q_out_strides[0], q_out_strides[1], heads_q,
-                              rotary != nullptr, 0};
+  const int64_t unit = 8;  // elements of 16 bytes
+  p.seg[n++] = segment(k, k_pages, {0, k_strides[0], k_strides[1]}, {k_page_strides[0], k_page_strides[1], k_page_strides[2]}, unit,
+                       heads_kv, rotary != nullptr, true);
+  p.seg[n++] = segment(v, v_pages, {0, v_strides[0], v_strides[1]}, {v_page_strides[0], v_page_strides[1], v_page_strides[2]}, unit,
+                       heads_kv, false, true);
+  if (q) p.seg[n++] = segment(q, q_out, {0, q_strides[0], q_strides[1]}, {0, q_out_strides[0], q_out_strides[1]}, unit, heads_q,
+                              rotary != nullptr, false);
   p.segments = n;
   p.heads = 2 * heads_kv + (q ? heads_q : 0);
   p.n = tokens;
