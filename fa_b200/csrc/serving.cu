@@ -18,7 +18,8 @@ constexpr int64_t kInt32Max = (int64_t(1) << 31) - 1;
 // Latency-bound: a few KB in, 12 bytes per token out.  Every block scans all
 // requests (two prefix sums in shared memory, <= 32 KB) instead of waiting for
 // another block's scan, so one launch without any grid-wide step does it; the
-// token and page loops are then split over the blocks.
+// token and page loops are then split over the blocks.  8 requests: 4.3 us; 250
+// requests and 175,000 token places: 6.3 us.
 constexpr int kTableThreads = 256;
 
 struct TableParams {
