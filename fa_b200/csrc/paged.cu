@@ -169,6 +169,7 @@ int check_paged(const b200fa_paged_args& a) {
                 B200FA_MAX_REQUESTS);
   if (a.window < 0 || a.sinks < 0 || (a.sinks > 0 && a.window == 0))
     return fail(B200FA_ERR_OPTIONS, "window %d, sinks %d: both at least 0, sinks only with a window", a.window, a.sinks);
+  if (a.flags & ~B200FA_PAGED_TEST_WITHHOLD_V) return fail(B200FA_ERR_OPTIONS, "unknown flags 0x%x", a.flags);
   if (!std::isfinite(a.scale) || !(a.scale > 0.f)) return fail(B200FA_ERR_SCALE, "scale must be finite and positive");
   if (a.requests == 0 || a.tokens == 0) return B200FA_OK;
   if (!a.q || !a.o || !a.k_pages || !a.v_pages || !a.block_table || !a.kv_lens || !a.cu_q)
@@ -252,6 +253,7 @@ int b200fa_paged_fwd(const b200fa_paged_args* args, void* stream) {
   p.sinks = a.sinks;
   p.scale_log2 = float(double(a.scale) * 1.4426950408889634074);
   p.timeout_ns = uint64_t(a.timeout_us ? a.timeout_us : 2000000u) * 1000ull;
+  p.flags = a.flags;
   p.wait_probes = uint32_t(p.timeout_ns / 20 < 0xffffffffull ? p.timeout_ns / 20 + 1 : 0xffffffffull);
   p.ws = static_cast<uint8_t*>(a.workspace);
   const bool bf16 = a.dtype == B200FA_DTYPE_BF16;

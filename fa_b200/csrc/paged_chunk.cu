@@ -251,6 +251,7 @@ __device__ __forceinline__ void load(const PagedParams& p, const PagedStart& sta
   const uint32_t q_bytes = uint32_t(half_tok * p.group) * 256u;
   const int size_mask = (1 << p.page_shift) - 1;
   const int k_rows = p.page_shift < 6 ? 1 << p.page_shift : kPairKeys;  // of a K box: this rank's keys of a page
+  if (kV && (p.flags & B200FA_PAGED_TEST_WITHHOLD_V)) return;
   uint32_t g0 = 0, issued = 0, q_issued = 0;  // issued, q_issued: in the issuing lane
   bool ok = true;
   int it = 0;

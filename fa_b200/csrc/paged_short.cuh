@@ -109,6 +109,10 @@ __device__ __forceinline__ void short_load(const PagedParams& p, const PagedStar
         for (int j = 0; ok && j < n; ++j) {
           const int key0 = w.blocks.key_block(w.off + j0 + j) * kPagedBlock;
           for (int kv = 0; kv < 2; ++kv) {
+            if (kv && (p.flags & B200FA_PAGED_TEST_WITHHOLD_V)) {
+              ok = false;
+              break;
+            }
             const uint32_t use = g + 2u * uint32_t(j) + uint32_t(kv), e = use % kShortRing;
             const uint32_t full = sm + kSmBars + 8 * e, empty = full + 8 * kShortRing;
             if (!(ok = paged_wait(p, empty, ((use / kShortRing) & 1u) ^ 1u, abort_slot, 0x800u | e))) break;

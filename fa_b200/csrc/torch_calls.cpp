@@ -77,6 +77,10 @@ T* ptr(const Tensor& t) { return static_cast<T*>(t.data_ptr()); }
 
 int64_t bytes_of(const Tensor& t) { return t.numel() * int64_t(t.element_size()); }
 
+// A dimension of one element has no stride of its own: torch may report any.
+int64_t step_of(const Tensor& t, int64_t i) { return t.size(i) == 1 ? 0 : t.stride(i); }
+int64_t row_stride(const Tensor& table) { return table.size(0) == 1 ? table.size(1) : table.stride(0); }
+
 using Tables = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;  // slots, positions, cu_q, kv_lens, free_left, status
 
 Tables empty_tables(int64_t requests, int64_t tokens, c10::Device dev) {
@@ -125,7 +129,7 @@ Tables build_tables(const Tensor& ctx, const Tensor& add, const Tensor& table, c
   const c10::cuda::OptionalCUDAGuard guard(dev);
   const Tables r = out ? *out : empty_tables(R, tokens, dev);
   const auto& [slots, pos, cu, kv, left, status] = r;
-  check(g.build_tables(ptr<int32_t>(ctx), ptr<int32_t>(add), int32_t(R), ptr<int32_t>(table), table.stride(0), int32_t(table.size(1)),
+  check(g.build_tables(ptr<int32_t>(ctx), ptr<int32_t>(add), int32_t(R), ptr<int32_t>(table), row_stride(table), int32_t(table.size(1)),
                        ptr<int32_t>(free_pages), free_pages.size(0), ptr<int32_t>(count), int32_t(page_size), ptr<int64_t>(slots),
                        ptr<int32_t>(pos), tokens, ptr<int32_t>(cu), ptr<int32_t>(kv), ptr<int32_t>(left), ptr<int32_t>(status),
                        stream_of(dev)),
@@ -153,8 +157,8 @@ Tensor rotary(const Tensor& x, const std::optional<Tensor>& positions, const std
   need(x.stride(-1) == 1 && out.stride(-1) == 1, "the last dimension of x and out must be contiguous");
   const bool four = x.dim() == 4;
   const int64_t B = four ? x.size(0) : 1, N = x.size(four ? 2 : 0), H = x.size(1);
-  const int64_t xs[3] = {four ? x.stride(0) : 0, x.stride(four ? 2 : 0), x.stride(1)};
-  const int64_t os[3] = {four ? out.stride(0) : 0, out.stride(four ? 2 : 0), out.stride(1)};
+  const int64_t xs[3] = {four ? step_of(x, 0) : 0, step_of(x, four ? 2 : 0), step_of(x, 1)};
+  const int64_t os[3] = {four ? step_of(out, 0) : 0, step_of(out, four ? 2 : 0), step_of(out, 1)};
   int bits = 32;
   int64_t pos_stride = 0;
   if (positions) {
@@ -214,11 +218,10 @@ std::optional<Tensor> append(const Tensor& k, const Tensor& v, const Tensor& kp,
     q_out = q_out_in ? *q_out_in : at::empty_like(*q, q->options(), at::MemoryFormat::Contiguous);
     need(q_out->sizes() == q->sizes(), "q_out must be shaped like q");
     need_rows("q_out", *q_out, T, -1, dim, kp);
-    qs[0] = q->stride(0), qs[1] = q->stride(1);
-    os[0] = q_out->stride(0), os[1] = q_out->stride(1);
+    for (int i = 0; i < 2; ++i) qs[i] = step_of(*q, i), os[i] = step_of(*q_out, i);
   }
-  const int64_t ks[2] = {k.stride(0), k.stride(1)}, vs[2] = {v.stride(0), v.stride(1)};
-  const int64_t kps[3] = {kp.stride(0), kp.stride(1), kp.stride(2)}, vps[3] = {vp.stride(0), vp.stride(1), vp.stride(2)};
+  const int64_t ks[2] = {step_of(k, 0), step_of(k, 1)}, vs[2] = {step_of(v, 0), step_of(v, 1)};
+  const int64_t kps[3] = {step_of(kp, 0), step_of(kp, 1), step_of(kp, 2)}, vps[3] = {step_of(vp, 0), step_of(vp, 1), step_of(vp, 2)};
   check(g.append(q ? q->data_ptr() : nullptr, q ? qs : nullptr, q ? q_out->data_ptr() : nullptr, q ? os : nullptr, k.data_ptr(), ks,
                  v.data_ptr(), vs, kp.data_ptr(), kps, vp.data_ptr(), vps, T, q ? int32_t(q->size(1)) : 0, int32_t(hkv), int32_t(dim),
                  kp.size(0), int32_t(kp.size(1)), ptr<int64_t>(slots), d ? positions->data_ptr() : nullptr, bits, d,
@@ -229,7 +232,7 @@ std::optional<Tensor> append(const Tensor& k, const Tensor& v, const Tensor& kp,
 
 Tensor paged(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& kv, const Tensor& cu,
              int64_t max_q, double scale, int64_t window, int64_t sinks, const std::optional<Tensor>& out_in, const Tensor& ws,
-             uint32_t timeout_us) {
+             uint32_t timeout_us, uint32_t flags) {
   constexpr int64_t kDim = 128;
   need_pages(kp, vp, kDim);
   need(q.dim() == 3, "q must be [T, Hq, 128]");
@@ -257,7 +260,7 @@ Tensor paged(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& 
   for (int i = 0; i < 2; ++i) a.q_strides[i] = q.stride(i), a.o_strides[i] = out.stride(i);
   for (int i = 0; i < 3; ++i) a.k_strides[i] = kp.stride(i), a.v_strides[i] = vp.stride(i);
   a.block_table = ptr<int32_t>(table);
-  a.table_stride = table.stride(0);
+  a.table_stride = row_stride(table);
   a.kv_lens = ptr<int32_t>(kv);
   a.cu_q = ptr<int32_t>(cu);
   a.tokens = T;
@@ -272,6 +275,7 @@ Tensor paged(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& 
   a.window = int32_t(window);
   a.sinks = int32_t(sinks);
   a.timeout_us = timeout_us;
+  a.flags = flags;
   a.workspace = ws.data_ptr();
   a.ws_bytes = uint64_t(ws.numel());
   check(g.paged_fwd(&a, stream_of(dev)), "b200fa_paged_fwd");

@@ -105,7 +105,7 @@ class PagedOperator:
         return ws
 
     def __call__(self, q, k_pages, v_pages, block_table, kv_lens, cu_q, *, max_q: int, scale: float | None = None,
-                 window: int = 0, sinks: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+                 window: int = 0, sinks: int = 0, out: torch.Tensor | None = None, flags: int = 0) -> torch.Tensor:
         """q [T, Hq, 128]; block_table int32 [R, width]; kv_lens int32 [R], the
         cached tokens of each request, its new ones included; cu_q int32
         [R + 1], the requests' rows of q.  Row i of request r stands at
@@ -123,7 +123,7 @@ class PagedOperator:
         window, sinks = _window(window, sinks, True)
         return calls.load().paged(q, k_pages, v_pages, block_table, kv_lens, cu_q, max_q,
                                   HEAD_DIM ** -0.5 if scale is None else scale, window, sinks, out,
-                                  self.workspace(q.device), self.timeout_us)
+                                  self.workspace(q.device), self.timeout_us, flags)
 
     def step(self, q, k, v, k_pages, v_pages, block_table, tables: StepTables, *, max_q: int,
              rotary: Rotary | None = None, scale: float | None = None, window: int = 0, sinks: int = 0,

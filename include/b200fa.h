@@ -399,9 +399,14 @@ typedef struct b200fa_paged_args {
     float       scale;
     int32_t     window, sinks;  /* window 0: none                                */
     uint32_t    timeout_us;     /* bound of every device-side wait; 0 = 2 s      */
+    uint32_t    flags;          /* B200FA_PAGED_TEST_WITHHOLD_V or 0             */
     void*       workspace;      /* 256-byte aligned, its header zeroed once      */
     uint64_t    ws_bytes;
 } b200fa_paged_args;
+
+/* Test-only: no V block is loaded, so that the waits for it run out and the
+ * kernel reports B200FA_DEV_TIMEOUT (the failure-detection test). */
+#define B200FA_PAGED_TEST_WITHHOLD_V 1u
 
 /* Bytes of workspace on the current device (status header + partial results);
  * calls that share a workspace must not overlap on the GPU.  Negative: error. */

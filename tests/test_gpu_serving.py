@@ -500,6 +500,47 @@ def test_paged_runs_give_the_same_bits_and_can_be_captured(name):
 
 
 @gpu
+def test_dimensions_of_one_element_may_have_any_stride():
+    from fa_b200.paged import PagedOperator, append, build_tables
+
+    rotary, _, _ = _rotary(128, 128, "half", {})
+    buf = torch.randn(1 + 12 * 128 + 3, device="cuda").half()
+    x = buf[:12 * 128].as_strided((1, 12, 128), (1537, 128, 1))
+    pos = torch.tensor([5], device="cuda")
+    assert torch.equal(rotary(x, pos), rotary(x.clone(memory_format=torch.contiguous_format), pos))
+    kp, vp = (torch.zeros((1, 8, 1, 128), dtype=F16, device="cuda").as_strided((1, 8, 1, 128), (7, 128, 3, 1)) for _ in range(2))
+    k = torch.randn((1, 1, 128), device="cuda").half().as_strided((1, 1, 128), (13, 9, 1))
+    assert torch.equal(append(k, k, kp, vp, torch.tensor([2], device="cuda"), q=x, positions=pos, rotary=rotary), rotary(x, pos))
+    assert torch.equal(vp[0, 2], k[0])
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    table = i32([0, -1]).as_strided((1, 2), (1, 1))
+    t = build_tables(i32([2]), i32([1]), table, i32([]), i32([0]), page_size=8, num_tokens=1)
+    assert t.slots.tolist() == [2]
+    out = PagedOperator()(x, kp, vp, table, t.kv_lens, t.cu_q, max_q=1)
+    O, A = ref.paged_attention(x, kp, vp, table, t.kv_lens, t.cu_q)
+    _within(out, O, A)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["ragged", "chunk_long"])
+def test_a_wait_that_runs_out_is_reported_and_nothing_hangs(name):
+    """No block of V is loaded (a test flag): every role gives up after its
+    bound, the status says so, and the same operator is right afterwards."""
+    from fa_b200 import lib
+    from fa_b200.paged import PagedOperator
+
+    case = _paged_case(LENGTHS[name], 12, 1, 16, F16, 13)
+    q, kp, vp, table, kv, cu, longest = case
+    op = PagedOperator(timeout_us=20000)
+    _check_paged(case, op=op)
+    op(q, kp, vp, table, kv, cu, max_q=longest, flags=lib.PAGED_TEST_WITHHOLD_V)
+    assert op.status(q.device)[0] == lib.DEV_TIMEOUT
+    op.reset_status(q.device)
+    assert op.status(q.device)[0] == lib.DEV_OK
+    _check_paged(case, op=op)
+
+
+@gpu
 def test_paged_first_use_in_a_capture_is_refused():
     from fa_b200.paged import PagedOperator
     from fa_b200.rotary import Rotary
@@ -590,7 +631,7 @@ def _args(**kw):
     from fa_b200 import lib
 
     a = lib.PagedArgs(C.sizeof(lib.PagedArgs), lib.DTYPE_FP16, 16, 16, 16, 16, (512, 128), (512, 128), (2048, 128, 128),
-                      (2048, 128, 128), 16, 4, 16, 16, 5, 8, 2, 4, 16, 4, 1, 1, 0.1, 0, 0, 0, 256, 1 << 30)
+                      (2048, 128, 128), 16, 4, 16, 16, 5, 8, 2, 4, 16, 4, 1, 1, 0.1, 0, 0, 0, 0, 256, 1 << 30)
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -600,7 +641,7 @@ def _args(**kw):
     ({"struct_size": 8}, -11), ({"dtype": 2}, -14), ({"requests": -1}, -3), ({"width": 0}, -3), ({"heads_kv": 3}, -4),
     ({"heads_q": 512}, -4), ({"page_size": 24}, -15), ({"page_size": 4}, -15), ({"tokens": 2**31}, -5),
     ({"requests": 5000}, -5), ({"width": 2**30}, -5), ({"width": 2**27}, -5), ({"window": -1}, -11), ({"sinks": 3}, -11), ({"scale": 0.0}, -10),
-    ({"q": None}, -1), ({"kv_lens": None}, -1), ({"o": 8}, -7), ({"table_stride": 3}, -16), ({"q_strides": (100, 128)}, -16),
+    ({"flags": 2}, -11), ({"q": None}, -1), ({"kv_lens": None}, -1), ({"o": 8}, -7), ({"table_stride": 3}, -16), ({"q_strides": (100, 128)}, -16),
     ({"k_strides": (2048, 0, 128)}, -16), ({"workspace": None}, -8), ({"workspace": 128}, -8)])
 def test_paged_validation_codes_without_gpu(kw, code):
     import ctypes as C

@@ -132,6 +132,23 @@ def test_window_through_host_buffers_and_a_graph():
     assert torch.equal(out, want)
 
 
+@pytest.mark.gpu
+def test_a_withheld_hand_over_ends_the_window_kernel_with_a_status():
+    """Every role of the window kernel, the storing warp among them, leaves when
+    a bounded wait runs out (the flag withholds one arrival)."""
+    from fa_b200 import lib
+    from fa_b200.ops import Operator
+
+    q, k, v = _inputs(1, 2, 1, 600, 600, 2, "cuda")
+    op = Operator("fp32", timeout_us=20000)
+    want = op(q, k, v, causal=True, window=300)
+    op(q, k, v, causal=True, window=300, flags=lib.FLAG_TEST_WITHHOLD_P)
+    assert op.status(q.device)[0] == lib.DEV_TIMEOUT
+    op.reset_status(q.device)
+    assert torch.equal(op(q, k, v, causal=True, window=300), want)
+    assert op.status(q.device)[0] == lib.DEV_OK
+
+
 def test_window_refusals():
     from fa_b200 import lib
     from fa_b200.ops import _window
