@@ -19,8 +19,8 @@
 //     stage: by the PV issuer's warp for rank 0, by the forwarding warp for
 //     rank 1.
 //   * scores are masked in tensor memory before the softmax loads them.
-//   * 4096 + 1024 tokens over 32768 + 20480 keys, 12 heads on 1: 830 us in short
-//     bursts, 906 under the power cap, 990 TFLOP/s of visible products.
+//   * 4096 + 1024 tokens over 32768 + 20480 keys, 12 heads on 1: 826 us in short
+//     bursts, 935 under the power cap, 961 TFLOP/s of visible products.
 //   * an item that lies in the stretch is normalised and stored; one that a
 //     stretch's end cuts leaves FP32 partial results, joined by
 //     b200_paged_combine_kernel.
