@@ -6,6 +6,9 @@ Layout:
   build.py   hash-keyed nvcc build of libb200fa.so
   lib.py     ctypes binding of the C ABI (include/b200fa.h)
   ops.py     torch-facing Operator (reference binding.py semantics)
+  paged.py   serving: page tables, cache append, attention over a paged cache
+  rotary.py  rotary positions
+  calls.py   the serving calls' host side in C++ (csrc/torch_calls.cpp)
   shard.py   multi-GPU partition of the (b, hq, q-block) unit grid
   core/      harness mirror: contract, registry, drivers, bench, runner,
              schedule, profiler (reference core/*)

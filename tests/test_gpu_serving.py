@@ -596,6 +596,48 @@ def test_a_serving_loop(dtype, hq, hkv, ps, window, sinks):
     assert int(count) == pages - sum(-(-sum(s[r] for s in steps) // ps) for r in range(R))
 
 
+@gpu
+def test_a_captured_generation_step_follows_the_device():
+    """One step -- tables, append with rotary, attention, and the lengths' and
+    the count's update -- as a graph, replayed with other new lengths."""
+    from fa_b200.paged import PagedOperator, StepTables, append, build_tables
+
+    dev, g, R, ps, width, T = "cuda", torch.Generator(device="cuda").manual_seed(2), 5, 16, 40, 24
+    rotary, _, _ = _rotary(128, 128, "half", {})
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    lens, new, count = i32([100, 0, 33, 250, 16]), i32([1, 1, 1, 1, 1]), i32([R * width])
+    table, free = torch.full((R, width), -1, dtype=torch.int32, device=dev), torch.randperm(R * width, device=dev).int()
+    kp, vp = (torch.full((R * width, ps, 2, 128), float("nan"), dtype=BF16, device=dev) for _ in range(2))
+    q, k, v = (torch.zeros((T, h, 128), dtype=BF16, device=dev) for h in (8, 2, 2))
+    # What is cached already, written as a step of its own.
+    t0 = build_tables(torch.zeros_like(lens), lens, table, free, count, page_size=ps, num_tokens=399)
+    append(torch.randn((399, 2, 128), generator=g, device=dev).to(BF16), torch.randn((399, 2, 128), generator=g, device=dev).to(BF16),
+           kp, vp, t0.slots)
+    count.copy_(t0.free_left)
+    op, t, out = PagedOperator(), StepTables.empty(R, T, dev), torch.zeros_like(q)
+    op.workspace(q.device)
+    rotary.table(q.device)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        build_tables(lens, new, table, free, count, page_size=ps, num_tokens=T, out=t)
+        op.step(q, k, v, kp, vp, table, t, max_q=4, rotary=rotary, out=out)
+        lens.copy_(t.kv_lens)
+        count.copy_(t.free_left)
+    for step in ([1, 1, 1, 1, 1], [1, 3, 0, 1, 16], [0, 1, 1, 4, 1], [1, 1, 1, 1, 1]):
+        new.copy_(i32(step))
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, generator=g, device=dev))
+        had = lens.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(t.status) == 0 and op.status(dev)[0] == 0
+        assert lens.tolist() == [a + b for a, b in zip(had.tolist(), step)]
+        n = sum(step)
+        O, A = ref.paged_attention(rotary(q, t.positions), kp, vp, table, t.kv_lens, t.cu_q)
+        _within(out[:n], O[:n], A[:n])
+
+
 # ----------------------------------------------------------------- refusals
 def test_rotary_refusals():
     from fa_b200.rotary import Rotary
