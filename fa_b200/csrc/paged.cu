@@ -254,7 +254,6 @@ int b200fa_paged_fwd(const b200fa_paged_args* args, void* stream) {
   p.scale_log2 = float(double(a.scale) * 1.4426950408889634074);
   p.timeout_ns = uint64_t(a.timeout_us ? a.timeout_us : 2000000u) * 1000ull;
   p.flags = a.flags;
-  p.wait_probes = uint32_t(p.timeout_ns / 20 < 0xffffffffull ? p.timeout_ns / 20 + 1 : 0xffffffffull);
   p.ws = static_cast<uint8_t*>(a.workspace);
   const bool bf16 = a.dtype == B200FA_DTYPE_BF16;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -56,7 +56,6 @@ struct PagedParams {
   int32_t part_rows;        // rows of a partial result
   uint64_t timeout_ns;
   uint32_t flags;           // B200FA_PAGED_TEST_WITHHOLD_V
-  uint32_t wait_probes;     // chunk kernel: bound of a wait, in probes of at least 20 ns
   uint8_t* ws;
 };
 

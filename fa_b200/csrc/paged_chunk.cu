@@ -72,26 +72,40 @@ __device__ __forceinline__ const PagedStart* start_of(uint8_t* raw) {
   return reinterpret_cast<const PagedStart*>(raw + (sm_of(raw).base - smem_addr(raw)) + kSmStart);
 }
 
-// Bounded waits: a number of probes, each of which may suspend the thread for
-// the probe's time hint.  A wait that runs out leaves its site in the abort
-// slot, which the teardown reports; the roles behind it run out in turn.  The
-// loop is kept this short on purpose: it is inlined at every wait of every
-// role, the hot loops of an SM sub-partition share a small instruction cache,
-// and with clock reads and an abort check in each, chunks ran slower.
+// What a wait does every thousand probes: the time of the first such look (`t0`,
+// 0 before it); a wait that runs out raises both CTAs' abort flags with its site,
+// which it then finds.  Out of line: these few instructions at every wait of the
+// hot loops cost 13 to 18 % of a chunk's time (4096 + 1024 tokens over 32768 +
+// 20480 keys: 987 against 836 us; called like this: within 2 % of a count alone).
+__device__ __noinline__ uint64_t wait_look(uint64_t t0, uint32_t abort_slot, uint64_t limit_ns, uint32_t site) {
+  const uint64_t now = global_timer_ns();
+  if (t0 == 0u) return now;
+  if (now - t0 <= limit_ns) return t0;
+  st_volatile_shared(abort_slot, site | 0x80000000u);
+  st_cluster_u32(map_shared(abort_slot, cluster_rank() ^ 1u), site | 0x80000000u);
+  return t0;
+}
+
+// Bounded waits.  A probe may suspend the thread, for about a microsecond, so a
+// wait ends within its bound and some milliseconds; the other roles of the pair
+// end with the one that gave up, and the teardown reports its site.
 struct Wait {
   uint32_t abort_slot;
   const PagedParams* p;
   template <bool kCluster = false>
   __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity, uint32_t site) const {
+    uint64_t t0 = 0;
 #pragma unroll 1
-    for (uint32_t n = p->wait_probes; n != 0u; --n)
+    for (uint32_t n = 0;; ++n) {
       if (kCluster ? mbar_test_cluster(bar, parity) : mbar_test(bar, parity)) return true;
-    st_volatile_shared(abort_slot, site | 0x80000000u);
-    return false;
+      if (ld_volatile_shared(abort_slot) != 0u) return false;
+      if ((n & 1023u) == 1023u) t0 = wait_look(t0, abort_slot, p->timeout_ns, site);
+    }
   }
-  __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) const {
-#pragma unroll 1
-    for (uint32_t n = 1u << 20; n != 0u && !mbar_test_cluster(bar, parity); --n) {}
+  // Exit-path wait for copies and products under way; it ignores the abort slot
+  // and gives up 100 ms after `t0`.
+  __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity, uint64_t t0) const {
+    while (!mbar_test_cluster(bar, parity) && global_timer_ns() - t0 < 100000000ull) {}
   }
 };
 
@@ -129,7 +143,7 @@ __device__ __forceinline__ void s_issuer(const PagedParams& p, const PagedStart&
     }
   }
   mma_commit_pair(sm.bar(kBarDrain + 0));
-  wait.drain(sm.bar(kBarDrain + 0), 0u);
+  wait.drain(sm.bar(kBarDrain + 0), 0u, global_timer_ns());
 }
 
 // V rows from key `from` of the block on, which no row of the item sees, become
@@ -198,7 +212,7 @@ __device__ __forceinline__ void pv_issuer(const PagedParams& p, const PagedStart
   // Issued by the lane that issued the products: commits follow a thread's own.
   if (elect_one()) {
     mma_commit_pair(sm.bar(kBarDrain + 1));
-    wait.drain(sm.bar(kBarDrain + 1), 0u);
+    wait.drain(sm.bar(kBarDrain + 1), 0u, global_timer_ns());
   }
 }
 
@@ -309,9 +323,10 @@ __device__ __forceinline__ void load(const PagedParams& p, const PagedStart& sta
   }
   // The last copies land before the CTA exits, also when a role gave up.
   if (elect_one()) {
+    const uint64_t t0 = global_timer_ns();
     const int full = kV ? (rank == 1 ? kBarVLand : kBarVFull) : kBarKFull;
-    for (uint32_t i = issued > kRing ? issued - kRing : 0; i < issued; ++i) wait.drain(sm.bar(full + int(ring_entry(i))), ring_parity(i));
-    for (uint32_t i = q_issued > 2 ? q_issued - 2 : 0; i < q_issued; ++i) wait.drain(sm.bar(kBarQFull + int(i & 1u)), (i >> 1) & 1u);
+    for (uint32_t i = issued > kRing ? issued - kRing : 0; i < issued; ++i) wait.drain(sm.bar(full + int(ring_entry(i))), ring_parity(i), t0);
+    for (uint32_t i = q_issued > 2 ? q_issued - 2 : 0; i < q_issued; ++i) wait.drain(sm.bar(kBarQFull + int(i & 1u)), (i >> 1) & 1u, t0);
   }
   __syncwarp();
 }

@@ -398,7 +398,8 @@ typedef struct b200fa_paged_args {
     int32_t     max_q;          /* the longest chunk (a hint: picks the kernel)  */
     float       scale;
     int32_t     window, sinks;  /* window 0: none                                */
-    uint32_t    timeout_us;     /* bound of every device-side wait; 0 = 2 s      */
+    uint32_t    timeout_us;     /* bound of every device-side wait (to some
+                                   milliseconds); 0 = 2 s                        */
     uint32_t    flags;          /* B200FA_PAGED_TEST_WITHHOLD_V or 0             */
     void*       workspace;      /* 256-byte aligned, its header zeroed once      */
     uint64_t    ws_bytes;
