@@ -14,7 +14,8 @@ import torch  # noqa: F401  (the module links against torch's libraries)
 from . import build as _build
 from . import lib
 
-ENTRIES = ("b200fa_build_tables", "b200fa_rotary", "b200fa_append", "b200fa_paged_fwd", "b200fa_last_error_string")
+ENTRIES = ("b200fa_build_tables", "b200fa_rotary", "b200fa_append", "b200fa_paged_workspace_size", "b200fa_paged_fwd",
+           "b200fa_last_error_string")
 
 _lock = threading.Lock()
 _module = None

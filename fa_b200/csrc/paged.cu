@@ -2,6 +2,7 @@
 // checks, tensor maps, the choice of kernel, and the kernel that joins the
 // parts of items cut by a worker's end.
 #include <cmath>
+#include <cstddef>
 #include <cstring>
 #include <mutex>
 
@@ -205,12 +206,16 @@ int64_t b200fa_paged_workspace_size(void) {
 int b200fa_paged_fwd(const b200fa_paged_args* args, void* stream) {
   clear_error();
   if (!args) return fail(B200FA_ERR_NULL, "args must not be NULL");
-  if (args->struct_size != sizeof(b200fa_paged_args)) return fail(B200FA_ERR_OPTIONS, "b200fa_paged_args.struct_size mismatch");
-  const b200fa_paged_args& a = *args;
+  b200fa_paged_args a = {};
+  constexpr uint32_t kArgsV1Bytes = offsetof(b200fa_paged_args, status);  // without the status pointer
+  if (args->struct_size != sizeof(a) && args->struct_size != kArgsV1Bytes)
+    return fail(B200FA_ERR_OPTIONS, "b200fa_paged_args.struct_size mismatch");
+  std::memcpy(&a, args, args->struct_size);
   int rc = check_paged(a);
   if (rc != B200FA_OK) return rc;
   if (!a.workspace || (reinterpret_cast<uintptr_t>(a.workspace) & 255u))
     return fail(B200FA_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  if (reinterpret_cast<uintptr_t>(a.status) & 3u) return fail(B200FA_ERR_ALIGNMENT, "status must be 4-byte aligned");
   if (a.requests == 0 || a.tokens == 0) return B200FA_OK;
   const PagedDevice* d = nullptr;
   if ((rc = paged_device(&d)) != B200FA_OK) return rc;
@@ -255,6 +260,7 @@ int b200fa_paged_fwd(const b200fa_paged_args* args, void* stream) {
   p.timeout_ns = uint64_t(a.timeout_us ? a.timeout_us : 2000000u) * 1000ull;
   p.flags = a.flags;
   p.ws = static_cast<uint8_t*>(a.workspace);
+  p.status = a.status ? a.status : static_cast<uint32_t*>(a.workspace);
   const bool bf16 = a.dtype == B200FA_DTYPE_BF16;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;

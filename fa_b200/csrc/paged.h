@@ -57,6 +57,7 @@ struct PagedParams {
   uint64_t timeout_ns;
   uint32_t flags;           // B200FA_PAGED_TEST_WITHHOLD_V
   uint8_t* ws;
+  uint32_t* status;
 };
 
 struct PagedRequest {
@@ -339,10 +340,9 @@ __device__ __forceinline__ float* paged_partial(const PagedParams& p, int slot) 
 }
 
 __device__ __forceinline__ void paged_status(const PagedParams& p, uint32_t code, uint32_t site) {
-  uint32_t* ws = reinterpret_cast<uint32_t*>(p.ws);
-  if (atomicCAS(&ws[0], 0u, code) == 0u) {
-    ws[1] = site;
-    ws[2] = blockIdx.x;
+  if (atomicCAS(&p.status[0], 0u, code) == 0u) {
+    p.status[1] = site;
+    p.status[2] = blockIdx.x;
   }
 }
 

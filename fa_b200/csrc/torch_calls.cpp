@@ -28,6 +28,7 @@ struct Abi {
   decltype(&b200fa_build_tables) build_tables = nullptr;
   decltype(&b200fa_rotary) rotary = nullptr;
   decltype(&b200fa_append) append = nullptr;
+  decltype(&b200fa_paged_workspace_size) paged_workspace_size = nullptr;
   decltype(&b200fa_paged_fwd) paged_fwd = nullptr;
   decltype(&b200fa_last_error_string) last_error = nullptr;
   PyObject* error = nullptr;  // B200FAError(where, status, message)
@@ -38,6 +39,7 @@ void bind(const py::dict& addresses, const py::object& error) {
   g.build_tables = reinterpret_cast<decltype(g.build_tables)>(at("b200fa_build_tables"));
   g.rotary = reinterpret_cast<decltype(g.rotary)>(at("b200fa_rotary"));
   g.append = reinterpret_cast<decltype(g.append)>(at("b200fa_append"));
+  g.paged_workspace_size = reinterpret_cast<decltype(g.paged_workspace_size)>(at("b200fa_paged_workspace_size"));
   g.paged_fwd = reinterpret_cast<decltype(g.paged_fwd)>(at("b200fa_paged_fwd"));
   g.last_error = reinterpret_cast<decltype(g.last_error)>(at("b200fa_last_error_string"));
   Py_XDECREF(g.error);
@@ -231,7 +233,7 @@ std::optional<Tensor> append(const Tensor& k, const Tensor& v, const Tensor& kp,
 }
 
 Tensor paged(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& kv, const Tensor& cu,
-             int64_t max_q, double scale, int64_t window, int64_t sinks, const std::optional<Tensor>& out_in, const Tensor& ws,
+             int64_t max_q, double scale, int64_t window, int64_t sinks, const std::optional<Tensor>& out_in, const Tensor& status,
              uint32_t timeout_us, uint32_t flags) {
   constexpr int64_t kDim = 128;
   need_pages(kp, vp, kDim);
@@ -250,6 +252,12 @@ Tensor paged(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& 
   const c10::cuda::OptionalCUDAGuard guard(dev);
   const Tensor out = out_in ? *out_in : at::empty({T, hq, kDim}, q.options());
   if (out_in) need_rows("out", out, T, hq, kDim, kp);
+  // Partial results live for this call: a block of torch's allocator belongs to
+  // the call's stream, or to the graph that is being captured, so calls that
+  // overlap never share one (the join finds its rows by what is written there).
+  const int64_t bytes = g.paged_workspace_size();
+  check(int(bytes < 0 ? bytes : 0), "b200fa_paged_workspace_size");
+  const Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
   b200fa_paged_args a = {};
   a.struct_size = sizeof(a);
   a.dtype = dtype_of(q.scalar_type());
@@ -278,6 +286,7 @@ Tensor paged(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& 
   a.flags = flags;
   a.workspace = ws.data_ptr();
   a.ws_bytes = uint64_t(ws.numel());
+  a.status = static_cast<uint32_t*>(status.data_ptr());
   check(g.paged_fwd(&a, stream_of(dev)), "b200fa_paged_fwd");
   return out;
 }

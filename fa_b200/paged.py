@@ -15,6 +15,7 @@ stay on the device, so a step can be captured into a CUDA graph.
 
 from __future__ import annotations
 
+import threading
 from dataclasses import dataclass
 
 import torch
@@ -22,6 +23,8 @@ import torch
 from . import calls, lib
 from .ops import HEAD_DIM, _window
 from .rotary import Rotary
+
+_first_use = threading.Lock()  # of an operator on a device
 
 
 @dataclass
@@ -79,29 +82,35 @@ class PagedOperator:
     """``op(q, k_pages, v_pages, block_table, kv_lens, cu_q, max_q=n) -> O``:
     attention of a step's new tokens over a paged cache, FP16 or BF16.
 
-    The operator owns a workspace per device; its calls must not overlap on
-    the GPU (one operator per stream, and per graph of graphs that may run at
-    the same time).  The first call on a device allocates it and cannot be
-    captured."""
+    The operator owns the status words of each device, made by its first call
+    there, which cannot be captured.  Everything else lives for one call, so
+    calls may overlap: on any streams, in any graphs.  Keep the operator as long
+    as a graph that captured a call of it."""
 
     def __init__(self, *, timeout_us: int = 0):
         self.timeout_us = int(timeout_us)
-        self.workspaces = {}  # device -> uint8 tensor
+        self.workspaces = {}  # device -> its status words
         lib.load()
 
     def workspace(self, device) -> torch.Tensor:
+        """The status words on ``device``, which must exist before a capture."""
         ws = self.workspaces.get(device)
         if ws is None:
-            if device.type != "cuda":
-                raise ValueError("the paged operator works on CUDA devices")
+            with _first_use:
+                ws = self.workspaces.get(device)
+                if ws is None:
+                    ws = self.workspaces[device] = self._new_workspace(device)
+        return ws
+
+    @staticmethod
+    def _new_workspace(device) -> torch.Tensor:
+        if device.type != "cuda":
+            raise ValueError("the paged operator works on CUDA devices")
+        with torch.cuda.device(device):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("the first call on a device cannot be captured: call workspace(device) before")
-            with torch.cuda.device(device):
-                n = int(lib.load().b200fa_paged_workspace_size())
-                lib.check(n if n < 0 else 0, "b200fa_paged_workspace_size")
-                ws = torch.zeros(n, dtype=torch.uint8, device=device)
-                torch.cuda.current_stream(device).synchronize()  # calls on other streams find it zeroed
-            self.workspaces[device] = ws
+            ws = torch.zeros(lib.WS_HEADER_BYTES, dtype=torch.uint8, device=device)
+            torch.cuda.current_stream(device).synchronize()  # calls on other streams find them zeroed
         return ws
 
     def __call__(self, q, k_pages, v_pages, block_table, kv_lens, cu_q, *, max_q: int, scale: float | None = None,
@@ -137,8 +146,9 @@ class PagedOperator:
                     max_q=max_q, scale=scale, window=window, sinks=sinks, out=out)
 
     def status(self, device) -> tuple[int, int, int, int]:
-        """Synchronize and read the device status header {status, site, block, 0}."""
+        """Synchronize the device and read the status words {status, site, block, 0}."""
         ws = self.workspace(_indexed(device))
+        torch.cuda.synchronize(ws.device)
         with torch.cuda.device(ws.device):
             return lib.read_status(ws.data_ptr(), torch.cuda.current_stream(ws.device).cuda_stream)
 

@@ -401,16 +401,24 @@ typedef struct b200fa_paged_args {
     uint32_t    timeout_us;     /* bound of every device-side wait (to some
                                    milliseconds); 0 = 2 s                        */
     uint32_t    flags;          /* B200FA_PAGED_TEST_WITHHOLD_V or 0             */
-    void*       workspace;      /* 256-byte aligned, its header zeroed once      */
+    void*       workspace;      /* 256-byte aligned; with status NULL, its first
+                                   256 bytes zeroed once                         */
     uint64_t    ws_bytes;
+    uint32_t*   status;         /* 256 bytes, zeroed once, kept between calls and
+                                   shared by any of them (b200fa_read_status,
+                                   b200fa_reset_status); NULL: the first ones of
+                                   the workspace.  A struct that ends before this
+                                   field is accepted too.                        */
 } b200fa_paged_args;
 
 /* Test-only: no V block is loaded, so that the waits for it run out and the
  * kernel reports B200FA_DEV_TIMEOUT (the failure-detection test). */
 #define B200FA_PAGED_TEST_WITHHOLD_V 1u
 
-/* Bytes of workspace on the current device (status header + partial results);
- * calls that share a workspace must not overlap on the GPU.  Negative: error. */
+/* Bytes of workspace on the current device (status header + partial results,
+ * which live for one call).  Calls that share a workspace must not overlap on
+ * the GPU: where streams or graphs may, each call takes one from an allocator
+ * that knows its stream, and `status` points elsewhere.  Negative: error. */
 int64_t b200fa_paged_workspace_size(void);
 int b200fa_paged_fwd(const b200fa_paged_args* args, void* stream);
 

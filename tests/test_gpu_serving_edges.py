@@ -3,12 +3,35 @@ forward-mode derivatives, values that no row sees, steps that could not be met,
 bounds of waits, ends of the number ranges.  Tolerances as in
 test_gpu_serving.py; most checks here are for equality."""
 
+import threading
+import time
+
 import pytest
 import torch
 
 F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
 gpu = pytest.mark.gpu
 i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+
+
+def _in_two_threads(a, b):
+    """a() and b() begun together; their results."""
+    gate, out, errors = threading.Barrier(2), [None, None], []
+
+    def run(i, f):
+        try:
+            gate.wait()
+            out[i] = f()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i, f)) for i, f in enumerate((a, b))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not errors, errors
+    return out
 
 
 def _cache(lens, hq, hkv, ps, dtype, seed):
@@ -52,3 +75,80 @@ def test_the_bound_of_a_wait_is_the_one_asked_for(lens):
     assert 290.0 <= begin.elapsed_time(end) <= 500.0, begin.elapsed_time(end)
     op.reset_status("cuda")
     assert torch.equal(op(q, kp, vp, table, kv, cu, max_q=n), want) and op.status("cuda")[0] == 0
+
+
+# ------------------------------------------------------------ calls that overlap
+@gpu
+def test_calls_of_one_operator_may_overlap():
+    """Single tokens on one stream, a chunk on another, both split over many
+    workers: eagerly, and as two graphs replayed at the same time."""
+    from fa_b200.paged import PagedOperator
+
+    op = PagedOperator()
+    cases = [_cache([(1, 30000), (1, 777)], 12, 1, 16, F16, 20), _cache([(300, 9000)], 12, 1, 64, F16, 21)]
+    longest = [1, 300]
+    wants = [op(*c, max_q=n) for c, n in zip(cases, longest)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    outs = [[torch.zeros_like(w) for _ in range(20)] for w in wants]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for c, n, s, o in zip(cases, longest, streams, outs):
+            with torch.cuda.stream(s):
+                op(*c, max_q=n, out=o[i])
+    torch.cuda.synchronize()
+    assert op.status("cuda")[0] == 0
+    for w, o in zip(wants, outs):
+        assert all(torch.equal(x, w) for x in o)
+    graphs = [torch.cuda.CUDAGraph() for _ in cases]
+    for graph, c, n, o in zip(graphs, cases, longest, outs):
+        with torch.cuda.graph(graph):
+            for x in o:
+                op(*c, max_q=n, out=x)
+    for o in outs:
+        for x in o:
+            x.zero_()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert op.status("cuda")[0] == 0
+    for w, o in zip(wants, outs):
+        assert all(torch.equal(x, w) for x in o)
+
+
+@gpu
+def test_an_operator_first_used_by_two_threads_has_one_status(monkeypatch):
+    from fa_b200.paged import PagedOperator
+
+    zeros = torch.zeros
+
+    def slowly(*args, **kw):
+        time.sleep(0.02)
+        return zeros(*args, **kw)
+
+    monkeypatch.setattr(torch, "zeros", slowly)
+    dev = torch.device("cuda", 0)
+    for _ in range(3):
+        op = PagedOperator()
+        a, b = _in_two_threads(lambda: op.workspace(dev), lambda: op.workspace(dev))
+        assert a is b is op.workspace(dev)
+
+
+def test_a_paged_call_without_the_status_pointer_is_still_accepted():
+    import ctypes as C
+
+    from fa_b200 import lib
+
+    a = lib.PagedArgs(lib.PagedArgs.status.offset, lib.DTYPE_FP16)
+    a.width = a.num_pages = a.heads_q = a.heads_kv = 1
+    a.page_size, a.scale, a.workspace = 16, 1.0, 256
+    assert lib.load().b200fa_paged_fwd(C.byref(a), None) == 0  # no requests
+    a.struct_size = C.sizeof(lib.PagedArgs)
+    assert lib.load().b200fa_paged_fwd(C.byref(a), None) == 0
+    a.status = 2
+    assert lib.load().b200fa_paged_fwd(C.byref(a), None) == -7
+    a.struct_size += 8
+    assert lib.load().b200fa_paged_fwd(C.byref(a), None) == -11
