@@ -19,12 +19,15 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import threading
 
 import torch
 
 from . import calls, lib
 
 LAYOUTS = {"half": 0, "interleaved": 1}
+
+_first_use = threading.RLock()  # of a Rotary on a device
 
 
 class _Turn(torch.autograd.Function):
@@ -80,29 +83,34 @@ class Rotary:
                 f = f * keep + f / factor * (1.0 - keep)
             self.frequencies.append(f)
         self._tables = {}  # device -> int64 tensor of 0.64 fixed-point turns
-        self._descs = {}   # (device, inverse) -> RotaryDesc
+        self._descs = {}   # (device, inverse) -> (RotaryDesc, its address, its table)
 
     def table(self, device) -> torch.Tensor:
         """The frequencies on ``device`` (made at its first use: outside a stream capture)."""
         device = torch.device(device)
         if device.type != "cuda":
             raise ValueError("a Rotary works on CUDA devices")
-        t = self._tables.get(device)
-        if t is None:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("the first use of a Rotary on a device cannot be captured: call table(device) before")
-            turns = [round(f / (2.0 * math.pi) * 2.0**64) % 2**64 for f in self.frequencies]
-            t = torch.tensor([x - 2**64 if x >= 2**63 else x for x in turns], dtype=torch.int64).to(device)
-            self._tables[device] = t
+        with _first_use:  # the copy below lets other threads run
+            t = self._tables.get(device)
+            if t is None:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("the first use of a Rotary on a device cannot be captured: call table(device) before")
+                turns = [round(f / (2.0 * math.pi) * 2.0**64) % 2**64 for f in self.frequencies]
+                t = torch.tensor([x - 2**64 if x >= 2**63 else x for x in turns], dtype=torch.int64).to(device)
+                self._tables[device] = t
         return t
 
     def desc(self, device, inverse: bool = False) -> int:
         """Address of the C description (b200fa_rotary_desc) for ``device``."""
         d = self._descs.get((device, inverse))
         if d is None:
-            d = lib.RotaryDesc(C.sizeof(lib.RotaryDesc), self.dim, self.rotary_dim, LAYOUTS[self.layout], int(inverse),
-                               self.magnitude, self.table(device).data_ptr())
-            d = self._descs[(device, inverse)] = (d, C.addressof(d))
+            with _first_use:
+                d = self._descs.get((device, inverse))
+                if d is None:
+                    table = self.table(device)
+                    c = lib.RotaryDesc(C.sizeof(lib.RotaryDesc), self.dim, self.rotary_dim, LAYOUTS[self.layout],
+                                       int(inverse), self.magnitude, table.data_ptr())
+                    d = self._descs[(device, inverse)] = (c, C.addressof(c), table)
         return d[1]
 
     def __call__(self, x: torch.Tensor, positions: torch.Tensor | None = None, *, out: torch.Tensor | None = None,

@@ -152,3 +152,26 @@ def test_a_paged_call_without_the_status_pointer_is_still_accepted():
     assert lib.load().b200fa_paged_fwd(C.byref(a), None) == -7
     a.struct_size += 8
     assert lib.load().b200fa_paged_fwd(C.byref(a), None) == -11
+
+
+# ------------------------------------------------- first use by two threads
+@pytest.mark.parametrize("directions", [(False, True), (False, False)], ids=["both_directions", "one_direction"])
+def test_a_rotary_first_used_by_two_threads_has_one_table(directions, monkeypatch):
+    """A stand-in takes the place of the copy to the device and lets the other
+    thread run, as the copy does."""
+    from fa_b200 import rotary as module
+
+    def to(self, *args, **kw):
+        time.sleep(0.02)
+        return self.clone()
+
+    monkeypatch.setattr(torch.Tensor, "to", to)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    dev = torch.device("cuda", 0)
+    for _ in range(5):
+        r = module.Rotary(64)
+        got = _in_two_threads(*[lambda inv=inv: r.desc(dev, inv) for inv in directions])
+        assert got == [r.desc(dev, inv) for inv in directions]  # neither was replaced behind its reader's back
+        for inv in directions:
+            d = module.lib.RotaryDesc.from_address(r.desc(dev, inv))
+            assert d.freq == r.table(dev).data_ptr()
