@@ -22,7 +22,7 @@ import torch
 
 from . import calls, lib
 from .ops import HEAD_DIM, _window
-from .rotary import Rotary
+from .rotary import Rotary, indexed
 
 _first_use = threading.Lock()  # of an operator on a device
 
@@ -96,6 +96,7 @@ class PagedOperator:
         """The status words on ``device``, which must exist before a capture."""
         ws = self.workspaces.get(device)
         if ws is None:
+            device = indexed(device)
             with _first_use:
                 ws = self.workspaces.get(device)
                 if ws is None:
@@ -147,17 +148,12 @@ class PagedOperator:
 
     def status(self, device) -> tuple[int, int, int, int]:
         """Synchronize the device and read the status words {status, site, block, 0}."""
-        ws = self.workspace(_indexed(device))
+        ws = self.workspace(device)
         torch.cuda.synchronize(ws.device)
         with torch.cuda.device(ws.device):
             return lib.read_status(ws.data_ptr(), torch.cuda.current_stream(ws.device).cuda_stream)
 
     def reset_status(self, device) -> None:
-        ws = self.workspace(_indexed(device))
+        ws = self.workspace(device)
         with torch.cuda.device(ws.device):
             lib.reset_status(ws.data_ptr(), torch.cuda.current_stream(ws.device).cuda_stream)
-
-
-def _indexed(device) -> torch.device:
-    device = torch.device(device)
-    return torch.device("cuda", torch.cuda.current_device()) if device.index is None else device

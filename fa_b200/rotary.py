@@ -30,6 +30,14 @@ LAYOUTS = {"half": 0, "interleaved": 1}
 _first_use = threading.RLock()  # of a Rotary on a device
 
 
+def indexed(device) -> torch.device:
+    """The device with its number: what is kept per device is found by it."""
+    device = torch.device(device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    return device
+
+
 class _Turn(torch.autograd.Function):
     """The rotation for autograd: its backward pass is the other direction."""
 
@@ -87,7 +95,7 @@ class Rotary:
 
     def table(self, device) -> torch.Tensor:
         """The frequencies on ``device`` (made at its first use: outside a stream capture)."""
-        device = torch.device(device)
+        device = indexed(device)
         if device.type != "cuda":
             raise ValueError("a Rotary works on CUDA devices")
         with _first_use:  # the copy below lets other threads run

@@ -175,3 +175,22 @@ def test_a_rotary_first_used_by_two_threads_has_one_table(directions, monkeypatc
         for inv in directions:
             d = module.lib.RotaryDesc.from_address(r.desc(dev, inv))
             assert d.freq == r.table(dev).data_ptr()
+
+
+# ------------------------------------------------------------- devices and copies
+@gpu
+def test_preparing_a_capture_with_the_device_without_its_number():
+    from fa_b200.paged import PagedOperator
+    from fa_b200.rotary import Rotary
+
+    q, kp, vp, table, kv, cu = _cache([(1, 40)], 4, 2, 16, F16, 12)
+    for device in ("cuda", torch.device("cuda"), "cuda:0"):
+        op, rotary = PagedOperator(), Rotary(128)
+        op.workspace(device)
+        rotary.table(device)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = op(rotary(q, torch.zeros(1, dtype=torch.int64, device="cuda")), kp, vp, table, kv, cu, max_q=1)
+        graph.replay()
+        assert torch.equal(out, op(q, kp, vp, table, kv, cu, max_q=1))
