@@ -93,6 +93,10 @@ class Rotary:
         self._tables = {}  # device -> int64 tensor of 0.64 fixed-point turns
         self._descs = {}   # (device, inverse) -> (RotaryDesc, its address, its table)
 
+    def __getstate__(self):
+        # Copies and pickles make tables of their own: a description is an address.
+        return {**self.__dict__, "_tables": {}, "_descs": {}}
+
     def table(self, device) -> torch.Tensor:
         """The frequencies on ``device`` (made at its first use: outside a stream capture)."""
         device = indexed(device)

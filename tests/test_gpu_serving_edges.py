@@ -3,6 +3,8 @@ forward-mode derivatives, values that no row sees, steps that could not be met,
 bounds of waits, ends of the number ranges.  Tolerances as in
 test_gpu_serving.py; most checks here are for equality."""
 
+import copy
+import pickle
 import threading
 import time
 
@@ -194,3 +196,14 @@ def test_preparing_a_capture_with_the_device_without_its_number():
             out = op(rotary(q, torch.zeros(1, dtype=torch.int64, device="cuda")), kp, vp, table, kv, cu, max_q=1)
         graph.replay()
         assert torch.equal(out, op(q, kp, vp, table, kv, cu, max_q=1))
+
+
+@gpu
+def test_a_used_rotary_can_be_copied_and_pickled():
+    from fa_b200.rotary import Rotary
+
+    rotary = Rotary(64, layout="interleaved", base=500.0)
+    x, pos = torch.randn((3, 2, 64), device="cuda"), torch.tensor([4, 9, 1], device="cuda")
+    want = rotary(x, pos)
+    for other in (copy.deepcopy(rotary), pickle.loads(pickle.dumps(rotary))):
+        assert torch.equal(other(x, pos), want)
