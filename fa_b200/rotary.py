@@ -22,6 +22,7 @@ import math
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import calls, lib
 
@@ -38,14 +39,29 @@ def indexed(device) -> torch.device:
     return device
 
 
+def differentiated(x: torch.Tensor) -> bool:
+    """Whether a derivative of either mode is being taken through x."""
+    if x.requires_grad and torch.is_grad_enabled():
+        return True
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None
+
+
 class _Turn(torch.autograd.Function):
-    """The rotation for autograd: its backward pass is the other direction."""
+    """The rotation for autograd: its backward pass is the other direction; it
+    is linear, so a tangent is turned as the value is."""
 
     @staticmethod
     def forward(ctx, x, positions, rotary, inverse):
-        ctx.save_for_backward(*([] if positions is None else [positions]))
+        saved = [] if positions is None else [positions]
+        ctx.save_for_backward(*saved)
+        ctx.save_for_forward(*saved)
         ctx.rotary, ctx.inverse = rotary, inverse
         return calls.load().rotary(x, positions, None, rotary.desc(x.device, inverse))
+
+    @staticmethod
+    def jvp(ctx, tangent, *_):
+        saved = ctx.saved_tensors
+        return ctx.rotary(tangent.contiguous(), saved[0] if saved else None, inverse=ctx.inverse)
 
     @staticmethod
     def backward(ctx, grad):
@@ -133,9 +149,9 @@ class Rotary:
         int64 on x's device; None is 0 .. N-1.  out may be x.  ``inverse``
         turns back; with the magnitude it is the transposed map, so it carries
         a gradient of y to x: that is what autograd runs when x requires a
-        gradient (out must then be None)."""
-        if x.requires_grad and torch.is_grad_enabled():
+        gradient or carries a tangent (out must then be None)."""
+        if differentiated(x):
             if out is not None:
-                raise ValueError("out cannot be given when x requires a gradient")
+                raise ValueError("out cannot be given when x requires a gradient or carries a tangent")
             return _Turn.apply(x, positions, self, bool(inverse))
         return calls.load().rotary(x, positions, out, self.desc(x.device, bool(inverse)))

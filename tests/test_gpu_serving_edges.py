@@ -207,3 +207,29 @@ def test_a_used_rotary_can_be_copied_and_pickled():
     want = rotary(x, pos)
     for other in (copy.deepcopy(rotary), pickle.loads(pickle.dumps(rotary))):
         assert torch.equal(other(x, pos), want)
+
+
+# ------------------------------------------------------ derivatives of a rotary
+@gpu
+@pytest.mark.parametrize("inverse", [False, True])
+def test_rotary_carries_forward_mode_derivatives(inverse):
+    import torch.autograd.forward_ad as fwd
+
+    from fa_b200.rotary import Rotary
+
+    rotary = Rotary(32, scaling="linear", factor=2.0, magnitude=1.5)
+    x, dx = torch.randn((2, 3, 7, 32), device="cuda"), torch.randn((2, 3, 7, 32), device="cuda")
+    pos = torch.arange(7, device="cuda") * 31
+    with fwd.dual_level():
+        y = fwd.unpack_dual(rotary(fwd.make_dual(x, dx), pos, inverse=inverse))
+        assert torch.equal(y.primal, rotary(x, pos, inverse=inverse))
+        assert y.tangent is not None and torch.equal(y.tangent, rotary(dx, pos, inverse=inverse))
+        plain = rotary(x, pos, inverse=inverse)  # no tangent in, none out
+        assert fwd.unpack_dual(plain).tangent is None
+        z = x.clone().requires_grad_()  # both modes at once
+        both = fwd.unpack_dual(rotary(fwd.make_dual(z, dx), pos, inverse=inverse))
+        assert torch.equal(both.tangent, rotary(dx, pos, inverse=inverse))
+        (grad,) = torch.autograd.grad(both.primal.sum(), z)
+        assert torch.equal(grad, rotary(torch.ones_like(x), pos, inverse=not inverse))
+        with pytest.raises(ValueError):
+            rotary(fwd.make_dual(x, dx), pos, out=torch.empty_like(x))
