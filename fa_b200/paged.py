@@ -22,7 +22,7 @@ import torch
 
 from . import calls, lib
 from .ops import HEAD_DIM, _window
-from .rotary import Rotary, indexed
+from .rotary import Rotary, differentiated, indexed
 
 _first_use = threading.Lock()  # of an operator on a device
 
@@ -73,14 +73,27 @@ def append(k, v, k_pages, v_pages, slots, *, q=None, positions=None, rotary: Rot
     skipped; the others are distinct).  With ``rotary``, K is turned by
     ``positions`` ([T], int32 or int64) on its way, and so is q [T, Hq, dim],
     which is returned (in q_out, which may be q).  One launch.  q, k and v may
-    be slices of one projection's output."""
+    be slices of one projection's output.
+
+    The cache holds values: derivatives of k and v end there.  The returned q
+    keeps its graph, or its tangent, when q has one (then a second launch, and
+    q_out must be None)."""
+    if q is not None and differentiated(q):
+        if q_out is not None:
+            raise ValueError("q_out cannot be given when q requires a gradient or carries a tangent")
+        if (q.ndim != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k_pages.shape[-1] or q.dtype != k_pages.dtype
+                or q.device != k_pages.device):
+            raise ValueError("q must be [T, heads, dim] of the cache's type and device")
+        append(k, v, k_pages, v_pages, slots, positions=positions, rotary=rotary)
+        return q.clone(memory_format=torch.contiguous_format) if rotary is None else rotary(q, positions)
     return calls.load().append(k, v, k_pages, v_pages, slots, q, positions if rotary is not None else None,
                                0 if rotary is None else rotary.desc(k_pages.device), q_out)
 
 
 class PagedOperator:
     """``op(q, k_pages, v_pages, block_table, kv_lens, cu_q, max_q=n) -> O``:
-    attention of a step's new tokens over a paged cache, FP16 or BF16.
+    attention of a step's new tokens over a paged cache, FP16 or BF16.  Forward
+    only: O has no graph.
 
     The operator owns the status words of each device, made by its first call
     there, which cannot be captured.  Everything else lives for one call, so
@@ -141,6 +154,8 @@ class PagedOperator:
         """The attention of one layer in a step: appends k and v to the cache
         at ``tables``' slots, rotated when ``rotary`` is given, and returns
         the attention of the (rotated) q over it."""
+        if q.requires_grad:
+            q = q.detach()  # the attention has no graph
         turned = append(k, v, k_pages, v_pages, tables.slots, q=q if rotary is not None else None,
                         positions=tables.positions if rotary is not None else None, rotary=rotary)
         return self(q if turned is None else turned, k_pages, v_pages, block_table, tables.kv_lens, tables.cu_q,

@@ -233,3 +233,41 @@ def test_rotary_carries_forward_mode_derivatives(inverse):
         assert torch.equal(grad, rotary(torch.ones_like(x), pos, inverse=not inverse))
         with pytest.raises(ValueError):
             rotary(fwd.make_dual(x, dx), pos, out=torch.empty_like(x))
+
+
+@gpu
+def test_the_rotated_q_of_an_append_keeps_its_graph():
+    """q's derivatives pass through append as through the rotary itself; the
+    cache holds values only."""
+    import torch.autograd.forward_ad as fwd
+
+    from fa_b200.paged import append
+    from fa_b200.rotary import Rotary
+
+    rotary = Rotary(128)
+    T, pos = 5, torch.arange(5, device="cuda") + 3
+    q, g = (torch.randn((T, 4, 128), device="cuda").half() for _ in range(2))
+    k, v = (torch.randn((T, 2, 128), device="cuda").half().requires_grad_() for _ in range(2))
+    kp, vp = (torch.zeros((1, 8, 2, 128), dtype=F16, device="cuda") for _ in range(2))
+    slots = torch.arange(T, device="cuda")
+    want = append(k.detach(), v.detach(), kp, vp, slots, q=q, positions=pos, rotary=rotary)
+    keys = kp.clone()
+    for turned in (rotary, None):
+        x = q.clone().requires_grad_()
+        kp.zero_(), vp.zero_()
+        y = append(k, v, kp, vp, slots, q=x, positions=pos, rotary=turned)
+        (grad,) = torch.autograd.grad(y, x, g)
+        assert torch.equal(grad, rotary(g, pos, inverse=True) if turned else g)
+        if turned:
+            assert torch.equal(y.detach(), want) and torch.equal(kp, keys) and torch.equal(vp[0, :T], v.detach())
+        assert not kp.requires_grad and not vp.requires_grad
+    with pytest.raises(ValueError):
+        append(k, v, kp, vp, slots, q=q.clone().requires_grad_(), positions=pos, rotary=rotary, q_out=torch.empty_like(q))
+    with torch.no_grad():
+        append(k, v, kp, vp, slots, q=q.clone().requires_grad_(), positions=pos, rotary=rotary, q_out=torch.empty_like(q))
+    for bad in (q[:4], q.float(), q[..., :64], q[0]):
+        with pytest.raises(ValueError):
+            append(k, v, kp, vp, slots, q=bad.clone().requires_grad_())
+    with fwd.dual_level():
+        y = fwd.unpack_dual(append(k, v, kp, vp, slots, q=fwd.make_dual(q, g), positions=pos, rotary=rotary))
+        assert torch.equal(y.primal, want) and torch.equal(y.tangent, rotary(g, pos))
