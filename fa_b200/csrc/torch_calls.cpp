@@ -83,6 +83,12 @@ int64_t bytes_of(const Tensor& t) { return t.numel() * int64_t(t.element_size())
 int64_t step_of(const Tensor& t, int64_t i) { return t.size(i) == 1 ? 0 : t.stride(i); }
 int64_t row_stride(const Tensor& table) { return table.size(0) == 1 ? table.size(1) : table.stride(0); }
 
+// A caller's tensor that a kernel writes: a backward pass that saved it must see
+// that it changed, as after torch's own in-place operations.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 using Tables = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;  // slots, positions, cu_q, kv_lens, free_left, status
 
 Tables empty_tables(int64_t requests, int64_t tokens, c10::Device dev) {
@@ -136,6 +142,9 @@ Tables build_tables(const Tensor& ctx, const Tensor& add, const Tensor& table, c
                        ptr<int32_t>(pos), tokens, ptr<int32_t>(cu), ptr<int32_t>(kv), ptr<int32_t>(left), ptr<int32_t>(status),
                        stream_of(dev)),
         "b200fa_build_tables");
+  written(table);
+  if (out)
+    for (const Tensor* t : {&slots, &pos, &cu, &kv, &left, &status}) written(*t);
   return r;
 }
 
@@ -171,6 +180,7 @@ Tensor rotary(const Tensor& x, const std::optional<Tensor>& positions, const std
   check(g.rotary(x.data_ptr(), out.data_ptr(), B, N, H, xs, os, positions ? positions->data_ptr() : nullptr, bits, pos_stride, d,
                  dtype, stream_of(dev)),
         "b200fa_rotary");
+  if (out_in) written(out);
   return out;
 }
 
@@ -229,6 +239,9 @@ std::optional<Tensor> append(const Tensor& k, const Tensor& v, const Tensor& kp,
                  kp.size(0), int32_t(kp.size(1)), ptr<int64_t>(slots), d ? positions->data_ptr() : nullptr, bits, d,
                  dtype_of(kp.scalar_type()), stream_of(dev)),
         "b200fa_append");
+  written(kp);
+  written(vp);
+  if (q && q_out_in) written(*q_out);
   return q_out;
 }
 
@@ -288,6 +301,7 @@ Tensor paged(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& 
   a.ws_bytes = uint64_t(ws.numel());
   a.status = static_cast<uint32_t*>(status.data_ptr());
   check(g.paged_fwd(&a, stream_of(dev)), "b200fa_paged_fwd");
+  if (out_in) written(out);
   return out;
 }
 

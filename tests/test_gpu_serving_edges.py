@@ -271,3 +271,39 @@ def test_the_rotated_q_of_an_append_keeps_its_graph():
     with fwd.dual_level():
         y = fwd.unpack_dual(append(k, v, kp, vp, slots, q=fwd.make_dual(q, g), positions=pos, rotary=rotary))
         assert torch.equal(y.primal, want) and torch.equal(y.tangent, rotary(g, pos))
+
+
+# ---------------------------------------------------------- in-place writes count
+@gpu
+def test_written_tensors_change_their_version():
+    """A tensor saved for a backward pass and written by an operator makes that
+    pass raise, as after torch's own in-place operations."""
+    from fa_b200.paged import PagedOperator, append, build_tables
+    from fa_b200.rotary import Rotary
+
+    rotary = Rotary(128)
+    q, kp, vp, table, kv, cu = _cache([(2, 40)], 4, 2, 16, F16, 7)
+    k, slots, pos = torch.randn((2, 2, 128), device="cuda").half(), torch.arange(2, device="cuda"), torch.arange(2, device="cuda")
+    q_out, x, out = torch.zeros_like(q), q.clone(), torch.zeros_like(q)
+
+    def bumped(call, *tensors):
+        before = [t._version for t in tensors]
+        call()
+        return all(t._version > b for t, b in zip(tensors, before))
+
+    assert bumped(lambda: append(k, k, kp, vp, slots, q=q, q_out=q_out, positions=pos, rotary=rotary), kp, vp, q_out)
+    assert bumped(lambda: rotary(x, pos, out=x), x)
+    assert bumped(lambda: PagedOperator()(q, kp, vp, table, kv, cu, max_q=2, out=out), out)
+    t = build_tables(kv, i32([1]), table, i32([]), i32([0]), page_size=16, num_tokens=2)
+    assert bumped(lambda: build_tables(kv, i32([1]), table, i32([]), i32([0]), page_size=16, num_tokens=2, out=t), table, *t.tensors())
+    w = torch.ones((), device="cuda", dtype=F16, requires_grad=True)
+    loss = (w * kp).sum()
+    append(k, k, kp, vp, slots)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        y = q.clone()
+        rotary(y, pos, out=y)
+    unchanged = q._version
+    rotary(q, pos)
+    assert q._version == unchanged
