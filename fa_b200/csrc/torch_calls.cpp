@@ -81,6 +81,7 @@ int64_t bytes_of(const Tensor& t) { return t.numel() * int64_t(t.element_size())
 
 // A dimension of one element has no stride of its own: torch may report any.
 int64_t step_of(const Tensor& t, int64_t i) { return t.size(i) == 1 ? 0 : t.stride(i); }
+bool rows_contiguous(const Tensor& table) { return table.size(1) == 1 || table.stride(1) == 1; }
 int64_t row_stride(const Tensor& table) { return table.size(0) == 1 ? table.size(1) : table.stride(0); }
 
 // A caller's tensor that a kernel writes: a backward pass that saved it must see
@@ -115,7 +116,7 @@ Tables build_tables(const Tensor& ctx, const Tensor& add, const Tensor& table, c
   need_int32("new_lens", add, R, dev);
   need(free_pages.dim() == 1 && int32s(free_pages, dev), "free_pages must be contiguous int32 [n] on the same CUDA device");
   need_int32("free_count", count, 1, dev);
-  need(table.scalar_type() == at::kInt && table.device() == dev && table.size(0) == R && table.stride(1) == 1,
+  need(table.scalar_type() == at::kInt && table.device() == dev && table.size(0) == R && rows_contiguous(table),
        "block_table must be int32 [R, width] with contiguous rows on the same CUDA device");
   need(tokens >= 0, "num_tokens must be at least 0");
   need(R <= INT32_MAX && table.size(1) <= INT32_MAX && page_size >= 0 && page_size <= INT32_MAX, "a size is out of range");
@@ -259,7 +260,7 @@ Tensor paged(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& 
   const int64_t R = kv.size(0);
   need_int32("kv_lens", kv, R, dev);
   need_int32("cu_q", cu, R + 1, dev);
-  need(table.dim() == 2 && table.scalar_type() == at::kInt && table.device() == dev && table.size(0) == R && table.stride(1) == 1,
+  need(table.dim() == 2 && table.scalar_type() == at::kInt && table.device() == dev && table.size(0) == R && rows_contiguous(table),
        "block_table must be int32 [R, width] with contiguous rows on the same CUDA device");
   need(R <= INT32_MAX && table.size(1) <= INT32_MAX, "a size is out of range");
   const c10::cuda::OptionalCUDAGuard guard(dev);

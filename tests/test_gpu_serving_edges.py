@@ -307,3 +307,16 @@ def test_written_tensors_change_their_version():
     unchanged = q._version
     rotary(q, pos)
     assert q._version == unchanged
+
+
+@gpu
+def test_a_table_of_one_column_may_have_any_stride():
+    from fa_b200.paged import PagedOperator, build_tables
+
+    q, kp, vp, table, kv, cu = _cache([(1, 5), (1, 9), (1, 2)], 4, 2, 16, F16, 11)
+    column = table.view(1, 3).t()  # [3, 1], strides (1, 3)
+    assert column.stride() == (1, 3)
+    want = PagedOperator()(q, kp, vp, table, kv, cu, max_q=1)
+    assert torch.equal(PagedOperator()(q, kp, vp, column, kv, cu, max_q=1), want)
+    t = build_tables(kv, i32([1, 1, 1]), column, i32([]), i32([0]), page_size=16, num_tokens=3)
+    assert t.status.tolist() == [0] and t.slots.tolist() == [int(p) * 16 + n for p, n in zip(table.view(-1).tolist(), (5, 9, 2))]
