@@ -9,13 +9,17 @@
 // included: tables of a step 22 -> 15 us, append 26 -> 16, one request's
 // attention 25 -> 15.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
+#include <array>
 #include <cmath>
 #include <optional>
 #include <string>
+#include <vector>
 
 #include "b200fa.h"
 
@@ -84,6 +88,61 @@ int64_t step_of(const Tensor& t, int64_t i) { return t.size(i) == 1 ? 0 : t.stri
 bool rows_contiguous(const Tensor& table) { return table.size(1) == 1 || table.stride(1) == 1; }
 int64_t row_stride(const Tensor& table) { return table.size(0) == 1 ? table.size(1) : table.stride(0); }
 
+// Whether indexes of two tensors of the same strides meet: `d`, the distance of
+// their starts, is a sum of (index in a - index in b) * stride.  `dims`: stride,
+// elements in a, elements in b, largest stride first and each above all the
+// smaller ones together, so that a dimension's difference is one of two values.
+bool meet(int64_t d, const std::vector<std::array<int64_t, 3>>& dims, size_t i = 0) {
+  if (i == dims.size()) return d == 0;
+  const auto [s, na, nb] = dims[i];
+  if (s == 0) return meet(d, dims, i + 1);
+  const int64_t q = d >= 0 ? d / s : -((-d + s - 1) / s);
+  for (int64_t x : {q, q + 1})
+    if (x < na && -x < nb && meet(d - x * s, dims, i + 1)) return true;
+  return false;
+}
+
+std::pair<const char*, const char*> extent(const Tensor& t) {
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  const char* p = static_cast<const char*>(t.data_ptr());
+  return {p, t.numel() == 0 ? p : p + (last + 1) * int64_t(t.element_size())};
+}
+
+// Whether a (written) and b share elements.  Slices of one buffer may lie
+// between each other; where that cannot be told, they are taken to be apart.
+bool overlap(const Tensor& a, const Tensor& b) {
+  const auto [a0, a1] = extent(a);
+  const auto [b0, b1] = extent(b);
+  if (a0 >= b1 || b0 >= a1) return false;
+  bool alike = a.dim() == b.dim() && a.element_size() == b.element_size();
+  std::vector<std::array<int64_t, 3>> dims;
+  for (int64_t i = 0; alike && i < a.dim(); ++i) {
+    const bool one_a = a.size(i) == 1, one_b = b.size(i) == 1;
+    alike = one_a || one_b || a.stride(i) == b.stride(i);
+    if (!(one_a && one_b)) dims.push_back({one_a ? b.stride(i) : a.stride(i), a.size(i), b.size(i)});
+  }
+  if (alike) {
+    std::sort(dims.begin(), dims.end(), [](const auto& x, const auto& y) { return x[0] > y[0]; });
+    return meet((b0 - a0) / int64_t(a.element_size()), dims);
+  }
+  const auto s = at::get_overlap_status(a, b);
+  return s == at::MemOverlapStatus::Partial || s == at::MemOverlapStatus::Full;
+}
+
+// The same elements at the same places: written where they are read.
+bool same(const Tensor& a, const Tensor& b) {
+  if (a.data_ptr() != b.data_ptr() || a.sizes() != b.sizes()) return false;
+  for (int64_t i = 0; i < a.dim(); ++i)
+    if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
+  return true;
+}
+
+void need_apart(const Tensor& to, const Tensor& from, const char* message) { need(!overlap(to, from), message); }
+void need_same_or_apart(const Tensor& to, const Tensor& from, const char* message) {
+  need(same(to, from) || !overlap(to, from), message);
+}
+
 // A caller's tensor that a kernel writes: a backward pass that saved it must see
 // that it changed, as after torch's own in-place operations.
 void written(const Tensor& t) {
@@ -105,6 +164,22 @@ Tables empty_tables(int64_t requests, int64_t tokens, c10::Device dev) {
   };
   Tensor cu = take(requests + 1), kv = take(requests), left = take(1), status = take(1);
   return {slots, take(tokens), cu, kv, left, status};
+}
+
+// Contiguous tensors' memory.
+bool ranges_meet(const Tensor& t, const Tensor& u) {
+  const char *a = ptr<char>(t), *b = ptr<char>(u);
+  return a < b + bytes_of(u) && b < a + bytes_of(t);
+}
+
+// A contiguous tensor and the rows of a table.
+bool meets_rows(const Tensor& table, const Tensor& u) {
+  const char *base = ptr<char>(table), *a = ptr<char>(u), *b = a + bytes_of(u);
+  const int64_t pitch = row_stride(table) * 4, row = table.size(1) * 4;
+  if (a == b || row == 0 || b <= base || pitch <= 0) return false;
+  // The first row that ends behind a's start.
+  const int64_t r = a < base + row ? 0 : (a - base - row) / pitch + 1;
+  return r < table.size(0) && base + r * pitch < b;
 }
 
 Tables build_tables(const Tensor& ctx, const Tensor& add, const Tensor& table, const Tensor& free_pages, const Tensor& count,
@@ -129,12 +204,15 @@ Tables build_tables(const Tensor& ctx, const Tensor& add, const Tensor& table, c
     need_int32("out.kv_lens", kv, R, dev);
     need_int32("out.free_left", left, 1, dev);
     need_int32("out.status", status, 1, dev);
-    for (const Tensor* t : {&slots, &pos, &cu, &kv, &left, &status})
-      for (const Tensor* u : {&ctx, &add, &free_pages, &count}) {
-        const char *a = ptr<char>(*t), *b = ptr<char>(*u);
-        need(!(a < b + bytes_of(*u) && b < a + bytes_of(*t)), "an output overlaps an input: alternate between two StepTables");
-      }
+    const std::array<const Tensor*, 6> outs = {&slots, &pos, &cu, &kv, &left, &status};
+    for (size_t i = 0; i < outs.size(); ++i) {
+      for (const Tensor* u : {&ctx, &add, &free_pages, &count})
+        need(!ranges_meet(*outs[i], *u), "an output overlaps an input: alternate between two StepTables");
+      need(!meets_rows(table, *outs[i]), "an output overlaps block_table");
+      for (size_t j = 0; j < i; ++j) need(!ranges_meet(*outs[i], *outs[j]), "two outputs overlap");
+    }
   }
+  for (const Tensor* u : {&ctx, &add, &free_pages, &count}) need(!meets_rows(table, *u), "block_table overlaps another input");
   const c10::cuda::OptionalCUDAGuard guard(dev);
   const Tables r = out ? *out : empty_tables(R, tokens, dev);
   const auto& [slots, pos, cu, kv, left, status] = r;
@@ -167,6 +245,7 @@ Tensor rotary(const Tensor& x, const std::optional<Tensor>& positions, const std
   need(out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type() && out.device() == dev,
        "out must be shaped and typed like x, on its device");
   need(x.stride(-1) == 1 && out.stride(-1) == 1, "the last dimension of x and out must be contiguous");
+  if (out_in) need_same_or_apart(out, x, "out must be x or lie apart from it");
   const bool four = x.dim() == 4;
   const int64_t B = four ? x.size(0) : 1, N = x.size(four ? 2 : 0), H = x.size(1);
   const int64_t xs[3] = {four ? step_of(x, 0) : 0, step_of(x, four ? 2 : 0), step_of(x, 1)};
@@ -223,6 +302,11 @@ std::optional<Tensor> append(const Tensor& k, const Tensor& v, const Tensor& kp,
       throw py::value_error("the rotary's dim is " + std::to_string(d->dim) + ", the cache's " + std::to_string(dim));
     bits = position_bits(*positions, dev);
   }
+  for (const Tensor* t : {&k, &v})
+    for (const Tensor* u : {&kp, &vp}) need_apart(*u, *t, "k or v overlaps the cache");
+  bool expanded = false;  // refused below, by its strides
+  for (int i = 0; i < 3; ++i) expanded |= kp.stride(i) == 0 && kp.size(i) > 1;
+  if (!expanded) need_apart(kp, vp, "k_pages and v_pages overlap");
   const c10::cuda::OptionalCUDAGuard guard(dev);
   std::optional<Tensor> q_out;
   int64_t qs[2] = {0, 0}, os[2] = {0, 0};
@@ -231,6 +315,11 @@ std::optional<Tensor> append(const Tensor& k, const Tensor& v, const Tensor& kp,
     q_out = q_out_in ? *q_out_in : at::empty_like(*q, q->options(), at::MemoryFormat::Contiguous);
     need(q_out->sizes() == q->sizes(), "q_out must be shaped like q");
     need_rows("q_out", *q_out, T, -1, dim, kp);
+    if (q_out_in) {
+      need_same_or_apart(*q_out, *q, "q_out must be q or lie apart from it");
+      for (const Tensor* t : {&k, &v, &kp, &vp}) need_apart(*q_out, *t, "q_out overlaps k, v or the cache");
+    }
+    for (const Tensor* t : {&kp, &vp}) need_apart(*t, *q, "q overlaps the cache");
     for (int i = 0; i < 2; ++i) qs[i] = step_of(*q, i), os[i] = step_of(*q_out, i);
   }
   const int64_t ks[2] = {step_of(k, 0), step_of(k, 1)}, vs[2] = {step_of(v, 0), step_of(v, 1)};
@@ -265,7 +354,11 @@ Tensor paged(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& 
   need(R <= INT32_MAX && table.size(1) <= INT32_MAX, "a size is out of range");
   const c10::cuda::OptionalCUDAGuard guard(dev);
   const Tensor out = out_in ? *out_in : at::empty({T, hq, kDim}, q.options());
-  if (out_in) need_rows("out", out, T, hq, kDim, kp);
+  if (out_in) {
+    need_rows("out", out, T, hq, kDim, kp);
+    need_same_or_apart(out, q, "out must be q or lie apart from it");
+    for (const Tensor* t : {&kp, &vp}) need_apart(out, *t, "out overlaps the cache");
+  }
   // Partial results live for this call: a block of torch's allocator belongs to
   // the call's stream, or to the graph that is being captured, so calls that
   // overlap never share one (the join finds its rows by what is written there).

@@ -59,8 +59,8 @@ def build_tables(ctx_lens, new_lens, block_table, free_pages, free_count, *, pag
     ``status`` (on the GPU) is 0, or 1: too few free pages, 2: a request
     outgrows its row of block_table, 3: more new tokens than num_tokens; then
     nothing is handed out, every slot is -1, kv_lens are ctx_lens and the table
-    is as it was.  The outputs must not overlap the inputs: a loop alternates
-    between two ``StepTables``.
+    is as it was.  The outputs must not overlap the inputs or one another: a
+    loop alternates between two ``StepTables``.
     """
     r = calls.load().build_tables(ctx_lens, new_lens, block_table, free_pages, free_count, page_size, num_tokens,
                                   None if out is None else out.tensors())

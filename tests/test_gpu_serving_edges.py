@@ -320,3 +320,45 @@ def test_a_table_of_one_column_may_have_any_stride():
     assert torch.equal(PagedOperator()(q, kp, vp, column, kv, cu, max_q=1), want)
     t = build_tables(kv, i32([1, 1, 1]), column, i32([]), i32([0]), page_size=16, num_tokens=3)
     assert t.status.tolist() == [0] and t.slots.tolist() == [int(p) * 16 + n for p, n in zip(table.view(-1).tolist(), (5, 9, 2))]
+
+
+# ------------------------------------------------------------------- overlaps
+@gpu
+def test_outputs_that_overlap_inputs_partly_are_refused():
+    from fa_b200.paged import PagedOperator, StepTables, append, build_tables
+    from fa_b200.rotary import Rotary
+
+    rotary, pos = Rotary(128), torch.arange(6, device="cuda")
+    buf = torch.randn((8, 4, 128), device="cuda").half()
+    with pytest.raises(ValueError):
+        rotary(buf[:6], pos, out=buf[1:7])
+    rotary(buf[:4], pos[:4], out=buf[4:])  # side by side in one buffer
+    square = torch.randn((6, 6, 128), device="cuda").half()
+    with pytest.raises(ValueError):
+        rotary(square, pos, out=square.transpose(0, 1))
+    k = torch.randn((6, 2, 128), device="cuda").half()
+    kp, vp = (torch.zeros((2, 8, 2, 128), dtype=F16, device="cuda") for _ in range(2))
+    slots = torch.arange(6, device="cuda")
+    with pytest.raises(ValueError):
+        append(k, k, kp, vp, slots, q=buf[:6], positions=pos, rotary=rotary, q_out=buf[1:7])
+    with pytest.raises(ValueError):
+        append(kp.view(16, 2, 128)[:6], k, kp, vp, slots + 2)  # moves within the cache
+    with pytest.raises(ValueError):
+        append(k, k, kp, kp, slots)  # one tensor for both
+    q, kp, vp, table, kv, cu = _cache([(2, 30)], 4, 2, 16, F16, 13)
+    op, wide = PagedOperator(), torch.zeros((3, 4, 128), dtype=F16, device="cuda")
+    wide[:2] = q
+    want = op(q, kp, vp, table, kv, cu, max_q=2)
+    with pytest.raises(ValueError):
+        op(wide[:2], kp, vp, table, kv, cu, max_q=2, out=wide[1:])
+    assert torch.equal(op(wide[:2], kp, vp, table, kv, cu, max_q=2, out=wide[:2]), want)  # the whole of q is fine
+    ints = torch.zeros(64, dtype=torch.int32, device="cuda")
+    args = dict(page_size=16, num_tokens=4)
+    t = StepTables.empty(1, 4, "cuda")
+    for out in (StepTables(t.slots, ints[:4], t.cu_q, t.kv_lens, t.free_left, t.status),       # on the table
+                StepTables(t.slots, t.positions, t.cu_q, t.kv_lens, t.status, t.status),       # two outputs in one
+                StepTables(t.slots, t.positions, ints[32:34], t.kv_lens, t.free_left, t.status)):  # on the free list
+        with pytest.raises(ValueError):
+            build_tables(i32([3]), i32([1]), ints[:8].view(1, 8), ints[32:40], i32([8]), out=out, **args)
+    with pytest.raises(ValueError):
+        build_tables(i32([3]), i32([1]), ints[:8].view(1, 8), ints[4:12], i32([8]), **args)  # the table on the free list
