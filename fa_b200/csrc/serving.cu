@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kTableThreads) b200_build_tables_kernel(const 
     const int64_t c = length(p.ctx[r]), n = length(p.add[r]);
     tok += n;
     page += pages(c + n) - pages(c);
-    wide |= pages(c + n) > p.width;
+    wide |= pages(c + n) > p.width || c + n > kInt32Max;  // lengths and positions are 32 bits
   }
   int64_t it = tok, ip = page;
   for (int d = 1; d < 32; d <<= 1) {

@@ -57,7 +57,7 @@ def build_tables(ctx_lens, new_lens, block_table, free_pages, free_count, *, pag
     token get slot -1 and position 0.
 
     ``status`` (on the GPU) is 0, or 1: too few free pages, 2: a request
-    outgrows its row of block_table, 3: more new tokens than num_tokens; then
+    outgrows its row of block_table or 2^31 - 1 tokens, 3: more new tokens than num_tokens; then
     nothing is handed out, every slot is -1, kv_lens are ctx_lens and the table
     is as it was.  The outputs must not overlap the inputs or one another: a
     loop alternates between two ``StepTables``.

@@ -362,3 +362,21 @@ def test_outputs_that_overlap_inputs_partly_are_refused():
             build_tables(i32([3]), i32([1]), ints[:8].view(1, 8), ints[32:40], i32([8]), out=out, **args)
     with pytest.raises(ValueError):
         build_tables(i32([3]), i32([1]), ints[:8].view(1, 8), ints[4:12], i32([8]), **args)  # the table on the free list
+
+
+@gpu
+def test_lengths_that_leave_32_bits_are_refused_by_the_tables():
+    """A row wide enough for more than 2^31 - 1 tokens: the length would wrap."""
+    from fa_b200.paged import build_tables
+
+    top = 2**31 - 1
+    table = torch.full((2, 4096), -1, dtype=torch.int32, device="cuda")
+    table[0, :2048] = torch.arange(2048, device="cuda").int()
+    ctx, free = i32([top - 4, 3]), torch.arange(2048, 2060, device="cuda").int()
+    before = table.clone()
+    t = build_tables(ctx, i32([5, 1]), table, free, i32([12]), page_size=1 << 20, num_tokens=8)
+    assert t.status.tolist() == [2] and t.kv_lens.tolist() == [top - 4, 3] and t.slots.tolist() == [-1] * 8
+    assert torch.equal(table, before) and t.free_left.tolist() == [12]
+    t = build_tables(ctx, i32([4, 0]), table, free, i32([12]), page_size=1 << 20, num_tokens=8)
+    assert t.status.tolist() == [0] and t.kv_lens.tolist() == [top, 3]
+    assert t.slots.tolist()[:4] == [top - 4 + i for i in range(4)] and t.positions.tolist()[:4] == [top - 4 + i for i in range(4)]
