@@ -664,9 +664,6 @@ __device__ void load_role(const FwdParams& p, const Smem& sm, const Waiter& w, u
   uint32_t g = 0;
   uint32_t issued = 0;       // bit e / kRing + e: K / V entry e has ever been loaded
   uint32_t last_par = 0;     // the same bits: parity of its last load
-#if B200FA_WINDOW
-  grid_wait();  // launched ahead of the end of the work before it, which may write Q, K and V
-#endif
   uint32_t q_issued = 0, q_par = 0;
   bool ok = true;
   for (int item = int(cluster_id_x()), it = 0; ok && item < p.num_items; item += int(num_clusters_x()), ++it) {
@@ -1287,7 +1284,6 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
 // long time hint, so that it takes no issue slots from the softmax.
 __device__ __forceinline__ void store_role(const FwdParams& p, const Smem& sm, const Waiter& w, uint32_t rank, uint32_t warp) {
   const uint32_t site = (rank << 16) | (warp << 8);
-  grid_wait();  // ... or read O
   for (int item = int(cluster_id_x()), it = 0; item < p.num_items; item += int(num_clusters_x()), ++it) {
     int bh, qb, cnt;
     plan_decode<int>(p.nqb, p.unit_begin, p.unit_end, item, bh, qb, cnt);
@@ -1366,6 +1362,12 @@ __device__ __forceinline__ void setup_phase(const FwdParams& p, uint8_t* smem_ra
     tmem_alloc_pair(sm.tmem_slot(), kTmemCols);
     tmem_relinquish_pair();
   }
+#if B200FA_WINDOW
+  // Launched ahead of the end of the work before it, which may write Q, K and V
+  // or read O.  All roles wait, so that none of their bounded waits begins
+  // before that end.
+  grid_wait();
+#endif
   // Barriers of both CTAs initialised and TMEM allocated before any
   // cross-CTA arrival or pair MMA.
   tc_fence_before();

@@ -319,9 +319,9 @@ int b200fa_fwd_noalloc(const void* q, const void* k, const void* v, void* o,
  *   cu_q [requests + 1]  prefix sums of new_lens
  *   kv_lens [requests]   ctx + new
  *   free_left, status    [1]: pages left; 0, or 1 the free list is too short,
- *                        2 a request outgrows its table row (width), or
-                        2^31 - 1 tokens, 3 more
- *                        new tokens than num_tokens.  With a status other
+ *                        2 a request outgrows its table row (width) or
+ *                        2^31 - 1 tokens, 3 more new tokens than
+ *                        num_tokens.  With a status other
  *                        than 0 nothing is handed out: every slot is -1,
  *                        kv_lens = ctx_lens, free_left = *free_count, the
  *                        table is untouched.

@@ -380,3 +380,43 @@ def test_lengths_that_leave_32_bits_are_refused_by_the_tables():
     t = build_tables(ctx, i32([4, 0]), table, free, i32([12]), page_size=1 << 20, num_tokens=8)
     assert t.status.tolist() == [0] and t.kv_lens.tolist() == [top, 3]
     assert t.slots.tolist()[:4] == [top - 4 + i for i in range(4)] and t.positions.tolist()[:4] == [top - 4 + i for i in range(4)]
+
+
+SLOW = r"""
+extern "C" __global__ void slow(unsigned long long ns) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  unsigned long long t0, t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
+  do {
+    __nanosleep(1000);
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  } while (t - t0 < ns);
+}
+"""
+
+
+@gpu
+def test_time_spent_waiting_for_the_kernel_before_is_no_timeout():
+    """A kernel that lets its dependents start early and runs longer than
+    timeout_us: what is launched behind it begins its waits after it."""
+    from fa_b200.ops import Operator
+    from fa_b200.paged import PagedOperator
+
+    slow = torch.cuda._compile_kernel(SLOW, "slow")
+    q, k, v = (torch.randn((1, h, 600, 128), device="cuda").half() for h in (4, 2, 2))
+    op = Operator("fp16", timeout_us=20000)
+    want = op(q, k, v, causal=True, window=100)
+    out = torch.zeros_like(want)
+    pq, kp, vp, table, kv, cu = _cache([(1, 900), (2, 300)], 4, 2, 16, F16, 8)
+    pop = PagedOperator(timeout_us=20000)
+    pwant = pop(pq, kp, vp, table, kv, cu, max_q=2)
+    pout = torch.zeros_like(pwant)
+    torch.cuda.synchronize()
+    slow((1, 1, 1), (32, 1, 1), (100_000_000,))
+    op(q, k, v, causal=True, window=100, out=out)
+    torch.cuda.synchronize()
+    assert op.status(q.device)[0] == 0 and torch.equal(out, want)
+    slow((1, 1, 1), (32, 1, 1), (100_000_000,))
+    pop(pq, kp, vp, table, kv, cu, max_q=2, out=pout)
+    torch.cuda.synchronize()
+    assert pop.status(q.device)[0] == 0 and torch.equal(pout, pwant)
