@@ -195,10 +195,11 @@ int validate_shape(int64_t B, int64_t Hq, int64_t Hkv, int64_t Nq, int64_t Nk, i
   return B200FA_OK;
 }
 
-int encode_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t planes, uint32_t box_rows) {
+// `height` (0: rows): rows from there on read as zeros.
+int encode_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t planes, uint32_t box_rows, int64_t height = 0) {
   PFN_cuTensorMapEncodeTiled_v12000 fn = encode_fn();
   if (!fn) return fail(B200FA_ERR_NO_DRIVER, "cuTensorMapEncodeTiled is not available from the driver");
-  const cuuint64_t dims[3] = {cuuint64_t(kHeadDim), cuuint64_t(rows), cuuint64_t(planes)};
+  const cuuint64_t dims[3] = {cuuint64_t(kHeadDim), cuuint64_t(height ? height : rows), cuuint64_t(planes)};
   const cuuint64_t strides[2] = {cuuint64_t(kHeadDim * 2), cuuint64_t(rows) * kHeadDim * 2};
   const cuuint32_t box[3] = {64, box_rows, 1};
   const cuuint32_t estr[3] = {1, 1, 1};
@@ -319,6 +320,11 @@ int fill_params(const void* q, const void* k, const void* v, void* o, int64_t B,
   if (opts.flags & B200FA_FLAG_WINDOW) {
     p->window = opts.window;
     p->sinks = opts.sinks < Nk ? opts.sinks : int32_t(Nk);
+    // V as the item's blocks may read it: no keys behind the last row, and in the
+    // sinks' blocks no others (window_blocks).
+    const int64_t seen = Nk < Nq ? Nk : Nq, sinks = p->sinks < seen ? p->sinks : seen;
+    if ((rc = encode_map(&p->tm_v, v, Nk, B * Hkv, kBlockN, seen)) != B200FA_OK) return rc;
+    if ((rc = encode_map(&p->tm_vs, v, Nk, B * Hkv, kBlockN, sinks > 0 ? sinks : 1)) != B200FA_OK) return rc;
   }
   return B200FA_OK;
 }

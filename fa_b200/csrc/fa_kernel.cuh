@@ -252,6 +252,7 @@ struct FwdParams {
   int32_t heads;            // B * Hq
   int32_t nq;               // query rows per head
   int32_t window, sinks;    // window kernels: keys behind a row that stay visible, first keys that always do
+  CUtensorMap tm_vs;        // window kernels: V of the sinks alone, (128, sinks, B*Hkv)
 };
 
 constexpr uint32_t kFlagTrace = 1u;
@@ -372,23 +373,35 @@ __host__ __device__ inline void plan_decode(I nqb, I ub, I ue, I x, I& bh, I& qb
 // block j of the item is key block j for j < sink, else j + skip.  At least
 // one, so that an item whose rows see no key (Nq > Nk, no sinks) still runs
 // the pipeline; its scores are then masked throughout.
+//
+// Keys that no row of the item sees are masked, but their V would still enter the
+// product as 0 times what may be an infinity or NaN.  So no such V is loaded: where
+// there are keys between the sinks and the first row's window, the sinks' blocks
+// read V through a tensor map that ends with the sinks (tm_vs), and the window's
+// first block begins at the first row's window rather than at a multiple of 128,
+// its last keys, which the next block holds, masked.  tm_v itself ends with the
+// last row's key.  (Sinks and window may share a key block; it is then read once
+// for each.)
 struct WindowBlocks {
   int n, sink, skip;
+  int first_key;  // of the window blocks; 0 when sinks and window leave no gap
   __device__ __forceinline__ int key_block(int j) const { return j < sink ? j : j + skip; }
+  // First key that is loaded for block j.
+  __device__ __forceinline__ int key_base(int j) const {
+    const int base = key_block(j) * kBlockN;
+    return j < sink || base > first_key ? base : first_key;
+  }
 };
 
 __device__ __forceinline__ WindowBlocks window_blocks(const FwdParams& p, int qb, int cnt) {
   const int end = qb + cnt < p.n_kv ? qb + cnt : p.n_kv;  // past the last row's diagonal block
   const int first_key = qb * kBlockM - p.window + 1;
-  const int first = first_key > 0 ? first_key / kBlockN : 0;
+  if (p.sinks >= first_key) return WindowBlocks{end, 0, 0, 0};
+  const int first = first_key / kBlockN;
   int sink = (p.sinks + kBlockN - 1) / kBlockN;
   if (sink > end) sink = end;
-  if (sink > first) sink = first;
-  WindowBlocks b;
-  b.n = sink + (end > first ? end - first : 0);
-  b.sink = sink;
-  b.skip = first - sink;
-  if (b.n == 0) b = WindowBlocks{1, 1, 0};
+  WindowBlocks b{sink + (end > first ? end - first : 0), sink, first - sink, first_key};
+  if (b.n == 0) b = WindowBlocks{1, 1, 0, 0};
   return b;
 }
 
@@ -711,12 +724,13 @@ __device__ void load_role(const FwdParams& p, const Smem& sm, const Waiter& w, u
       if (!w.wait(sm.bar(kBarKEmpty + int(e)), ph ^ 1u, site | (kBarKEmpty + e))) { ok = false; break; }
       tl.mark(9, j, 1);
 #if B200FA_WINDOW
-      const int kb = blocks.key_block(j);
+      // A block may begin inside a key block and end behind the keys, where zeros are read.
+      const int key0 = blocks.key_base(j), over = kBlockN - 1;
 #else
-      const int kb = j;
+      const int key0 = j * kBlockN, over = 0;
 #endif
-      const int krow = kb * kBlockN + int(rank) * kKBoxRows;
-      if (!w.check(krow >= 0 && krow + kKBoxRows <= key_end, site | (kCheckSite + 2u))) { ok = false; break; }
+      const int krow = key0 + int(rank) * kKBoxRows;
+      if (!w.check(krow >= 0 && krow + kKBoxRows <= key_end + over, site | (kCheckSite + 2u))) { ok = false; break; }
       mbar_arrive_expect_tx(sm.bar(kBarKFull + int(e)), kStageBytes);
       tma_load_3d(sm.k(e), &p.tm_k, sm.bar(kBarKFull + int(e)), 0, krow, kvh);
       tma_load_3d(sm.k(e) + kKBoxBytes, &p.tm_k, sm.bar(kBarKFull + int(e)), 64, krow, kvh);
@@ -727,13 +741,20 @@ __device__ void load_role(const FwdParams& p, const Smem& sm, const Waiter& w, u
       tl.mark(9, j, 2);
       if (!w.wait(sm.bar(kBarVEmpty + int(e)), ph ^ 1u, site | (kBarVEmpty + e))) { ok = false; break; }
       tl.mark(9, j, 3);
-      if (!w.check(kb * kBlockN + kBlockN <= key_end && int(rank) * kPairDims + kPairDims <= kHeadDim,
+      if (!w.check(key0 + kBlockN <= key_end + over && int(rank) * kPairDims + kPairDims <= kHeadDim,
                    site | (kCheckSite + 3u))) {
         ok = false;
         break;
       }
       mbar_arrive_expect_tx(sm.bar(kBarVFull + int(e)), kStageBytes);
-      tma_load_3d(sm.v(e), &p.tm_v, sm.bar(kBarVFull + int(e)), int(rank) * kPairDims, kb * kBlockN, kvh);
+#if B200FA_WINDOW
+      // An item whose rows see nothing reads its block of V behind the sinks: zeros.
+      const bool none = blocks.sink > 0 && p.sinks == 0;
+      tma_load_3d(sm.v(e), j < blocks.sink ? &p.tm_vs : &p.tm_v, sm.bar(kBarVFull + int(e)), int(rank) * kPairDims,
+                  none ? kBlockN : key0, kvh);
+#else
+      tma_load_3d(sm.v(e), &p.tm_v, sm.bar(kBarVFull + int(e)), int(rank) * kPairDims, key0, kvh);
+#endif
       issued |= 1u << (kRing + e);
       last_par = (last_par & ~(1u << (kRing + e))) | (ph << (kRing + e));
     }
@@ -1003,14 +1024,7 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
       tl.mark(int(warp), j, 7);
       tc_fence_after();
 #if B200FA_WINDOW
-      // Keys of the block that this row sees: c < valid (the end of the keys,
-      // the diagonal) and c >= lo (its window) or c < sink.
       const int kb = blocks.key_block(j);
-      const int ahead = qrow_g - kb * kBlockN;
-      int valid = kb == p.n_kv - 1 ? p.nk_tail : kBlockN;
-      if (ahead + 1 < valid) valid = ahead + 1;
-      const int lo = ahead - p.window + 1;
-      const int sink = p.sinks - kb * kBlockN;
 #elif B200FA_CAUSAL
       // Valid keys of the block for this row: the last block's key count
       // and the keys up to the row.
@@ -1058,7 +1072,16 @@ __device__ void softmax_role(const FwdParams& p, const Smem& sm, uint32_t tmem_b
 #endif
       arrive_rank0(kBarSFree + int(b));  // the S issuer may refill the buffer
 #if B200FA_WINDOW
-      if (kb >= kb_hi || kb <= kb_lo) mask_window(r, valid, lo, sink);
+      if (kb >= kb_hi || kb <= kb_lo) {
+        // Keys of the block that this row sees: c < valid (the end of the keys or
+        // of the key block, the diagonal) and c >= lo (its window) or c < sink; of
+        // the sinks' blocks before a gap, the sinks.
+        const int base = blocks.key_base(j), ahead = qrow_g - base, sink = p.sinks - base;
+        int valid = kb * kBlockN - base + (kb == p.n_kv - 1 ? p.nk_tail : kBlockN);
+        if (ahead + 1 < valid) valid = ahead + 1;
+        if (j < blocks.sink && sink < valid) valid = sink;
+        mask_window(r, valid, j < blocks.sink ? 0 : ahead - p.window + 1, sink);
+      }
 #endif
       const float mx = fmaxf(row_max64(r), row_max64(r + 64)) * sl2;
       tl.mark(int(warp), j, 2);
@@ -1357,6 +1380,9 @@ __device__ __forceinline__ void setup_phase(const FwdParams& p, uint8_t* smem_ra
     tma_prefetch_map(&p.tm_k);
     tma_prefetch_map(&p.tm_v);
     tma_prefetch_map(&p.tm_o);
+#if B200FA_WINDOW
+    tma_prefetch_map(&p.tm_vs);
+#endif
   }
   if (warp == 0) {
     tmem_alloc_pair(sm.tmem_slot(), kTmemCols);

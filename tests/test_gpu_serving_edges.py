@@ -11,8 +11,11 @@ import time
 import pytest
 import torch
 
+from oracle import serving_ref as ref
+
 F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
 gpu = pytest.mark.gpu
+HALF = {t: torch.finfo(t).eps / 2 for t in (F16, BF16, F32)}
 i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
 
 
@@ -420,3 +423,43 @@ def test_time_spent_waiting_for_the_kernel_before_is_no_timeout():
     pop(pq, kp, vp, table, kv, cu, max_q=2, out=pout)
     torch.cuda.synchronize()
     assert pop.status(q.device)[0] == 0 and torch.equal(pout, pwant)
+
+
+@gpu
+@pytest.mark.parametrize("value", [float("nan"), float("inf")], ids=["nan", "inf"])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 4), (64, 0), (64, 130), (100, 200), (128, 4), (200, 1), (200, 129), (255, 128), (300, 300),
+                                          (513, 20), (700, 0)])
+@pytest.mark.parametrize("debug", [False, True], ids=["product", "checking"])
+def test_dense_values_outside_every_window_may_be_anything(window, sinks, value, debug):
+    """Work items of 256 rows: the ones from row `at` on must not notice what is
+    planted at keys that none of their rows sees."""
+    from fa_b200.ops import Operator
+
+    B, Hq, Hkv, N = 1, 4, 2, 1300
+    g = torch.Generator(device="cuda").manual_seed(window)
+    q, k, v = (torch.randn((B, h, N, 128), generator=g, device="cuda").half() for h in (Hq, Hkv, Hkv))
+    op = Operator("fp16", debug=debug)
+    want = op(q, k, v, causal=True, window=window, sinks=sinks)
+    O, A = ref.window_attention(q, k, v, window, sinks)
+    over = (want.double() - O).abs() - (A * (HALF[F16] + 7.5e-5 + 2.0 ** -16 + 3e-4) + O.abs() * HALF[F16] + 2.0 ** -24)
+    assert bool((over <= 0).all()), float(over.max())
+    for at in (256, 512, 1024, 1280):
+        k2, v2 = k.clone(), v.clone()
+        end = max(sinks, at - window + 1)
+        k2[:, :, sinks:end], v2[:, :, sinks:end] = float("nan"), value
+        got = op(q, k2, v2, causal=True, window=window, sinks=sinks)
+        torch.cuda.synchronize()
+        assert op.status(q.device)[0] == 0
+        assert torch.equal(got[:, :, at:], want[:, :, at:])
+
+
+@gpu
+@pytest.mark.parametrize("nq,nk,window,sinks", [(130, 2000, 50, 10), (1, 300, 1, 0), (300, 301, 1000, 0), (257, 700, 20, 600)])
+def test_dense_values_behind_the_last_row_may_be_anything(nq, nk, window, sinks):
+    from fa_b200.ops import Operator
+
+    q, k, v = (torch.randn((1, h, n, 128), device="cuda").half() for h, n in ((4, nq), (2, nk), (2, nk)))
+    op = Operator("fp32")
+    want = op(q, k, v, causal=True, window=window, sinks=sinks)
+    k[:, :, nq:], v[:, :, nq:] = float("nan"), float("nan")
+    assert torch.equal(op(q, k, v, causal=True, window=window, sinks=sinks), want)
