@@ -233,6 +233,8 @@ int b200fa_paged_fwd(const b200fa_paged_args* args, void* stream) {
   if (chunk) {  // K: each CTA of a pair loads its half of a block's keys; V: its half of the columns
     if ((rc = encode_pages(&p.tm_k, a, a.k_pages, a.k_strides, kPagedBlock / 2, "k_pages")) != B200FA_OK) return rc;
     if ((rc = encode_pages(&p.tm_v, a, a.v_pages, a.v_strides, kPagedBlock, "v_pages")) != B200FA_OK) return rc;
+    if ((rc = encode_pages(&p.tm_v8, a, a.v_pages, a.v_strides, 8, "v_pages")) != B200FA_OK) return rc;
+    if ((rc = encode_pages(&p.tm_v1, a, a.v_pages, a.v_strides, 1, "v_pages")) != B200FA_OK) return rc;
   } else {
     if ((rc = encode_halves(&p.tm_k, a, a.k_pages, a.k_strides, "k_pages")) != B200FA_OK) return rc;
     if ((rc = encode_halves(&p.tm_v, a, a.v_pages, a.v_strides, "v_pages")) != B200FA_OK) return rc;

@@ -39,6 +39,7 @@ constexpr uint32_t kPagedPartials = kPagedHeader + kMaxWorkers * kPagedRecord;  
 struct PagedParams {
   CUtensorMap tm_k, tm_v;   // (128, page_size, heads_kv, num_pages), boxes of 64 columns; short kernel:
                             // (64, page_size, 2, heads_kv, num_pages), boxes of both halves of the head dim
+  CUtensorMap tm_v8, tm_v1; // chunk kernel: V in boxes of 64 columns by 8 tokens and by one
   CUtensorMap tm_q;         // chunk kernel: (128, group, heads_kv, tokens), box (64, group, 1, tokens_per_tile / 2)
   const void* q;
   void* o;
@@ -90,6 +91,19 @@ struct PagedBlocks {
   int first_key;   // first key of the first row's window
   int end_key;     // past the position of the last row
   __device__ __forceinline__ int key_block(int j) const { return j < sink ? j : j + skip; }
+  // Whether the key block at `key0` holds keys that no row of the tile sees and
+  // that come with its others: between the sinks and the first row's window, or
+  // behind the last row.  Of a tile's blocks only the last of the sinks', the
+  // first of the window's (block `sink`) and the last can.
+  __device__ __forceinline__ bool unseen(const PagedParams& p, int key0) const {
+    const int last = key0 + kPagedBlock;
+    return last > end_key || (last > p.sinks && key0 < first_key && p.sinks < first_key);
+  }
+  // Part 0 and 1 of them, [x, y) relative to the block; may be empty.
+  __device__ __forceinline__ int2 unseen_keys(const PagedParams& p, int key0, int part) const {
+    return part ? make_int2(max(end_key - key0, 0), kPagedBlock)
+                : make_int2(max(p.sinks - key0, 0), min(first_key - key0, kPagedBlock));
+  }
 };
 
 __device__ __forceinline__ PagedBlocks paged_blocks(const PagedParams& p, const PagedRequest& q, int tile) {

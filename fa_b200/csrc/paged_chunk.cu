@@ -14,10 +14,9 @@
 //   * K and V come page by page, a box (K: one per 64 columns) for each page
 //     of a block, K and V by a warp each, which read the block table 32
 //     entries ahead.
-//   * V rows behind the last key that any row sees are cleared in shared
-//     memory before the product (0 * NaN is no 0), in an item's last
-//     stage: by the PV issuer's warp for rank 0, by the forwarding warp for
-//     rank 1.
+//   * in a block that holds keys that no row of the item sees -- an item's
+//     last, the last of the sinks', the first of the window's -- V is loaded in
+//     smaller boxes, with zeros in those keys' places (load_seen_v).
 //   * scores are masked in tensor memory before the softmax loads them.
 //   * 4096 + 1024 tokens over 32768 + 20480 keys, 12 heads on 1: 826 us in short
 //     bursts, 935 under the power cap, 961 TFLOP/s of visible products.
@@ -40,12 +39,8 @@
 namespace b200fa {
 namespace chunk {
 
-// Barrier slots: the dense kernel's, and one per V stage between its landing
-// and its hand-over to the PV issuer.
-constexpr int kBarVLand = kNumBars;            // [kRing] V stage landed, local
-constexpr int kBars = kBarVLand + kRing;
-constexpr int kSmBar = kSmemV + kRing * kStageBytes;
-constexpr int kSmXchg = kSmBar + kBars * 8;             // float [2][128]
+constexpr int kSmBar = kSmemV + kRing * kStageBytes;    // the dense kernel's barriers
+constexpr int kSmXchg = kSmBar + kNumBars * 8;            // float [2][128]
 constexpr int kSmTmem = kSmXchg + 2 * kBlockM * 4;      // TMEM base, abort flag
 constexpr int kSmStart = kSmTmem + 16;                  // PagedStart
 constexpr int kSmScan = kSmStart + 64;                  // int64 [12]
@@ -146,40 +141,20 @@ __device__ __forceinline__ void s_issuer(const PagedParams& p, const PagedStart&
   wait.drain(sm.bar(kBarDrain + 0), 0u, global_timer_ns());
 }
 
-// V rows from key `from` of the block on, which no row of the item sees, become
-// zeros: by a whole warp whose lanes have all observed the copy.
-__device__ __forceinline__ void clear_rows(uint32_t stage, int from, uint32_t lane) {
-  for (int i = int(lane) + (from > 0 ? from : 0) * 8; i < kPagedBlock * 8; i += 32) st_shared_v4(stage + uint32_t(i) * 16u, 0, 0, 0, 0);
-  fence_proxy_async_smem();
-  __syncwarp();
-}
-
-// First key of the block that no row of the item sees, relative to the block:
-// below kPagedBlock only in an item's last block.
-__device__ __forceinline__ int clear_from(const PagedBlocks& b, int block) { return b.end_key - b.key_block(block) * kPagedBlock; }
-
-// Rank 0, one warp, of which one lane issues: O += P V of every block, in order.
-// Where an item's last V stage needs clearing the warp does it for rank 0's
-// half and hands it over itself; the idle lanes wait at the warp barrier, so
-// none of them polls beside the issuing one (a warp that watched for those
-// stages alone cost every other wait of the CTA issue slots).
+// Rank 0, one thread: O += P V of every block, in order.
 template <bool kBf16>
 __device__ __forceinline__ void pv_issuer(const PagedParams& p, const PagedStart& start, const Sm& sm, uint32_t tmem, const Wait& wait) {
   const uint32_t site = uint32_t(kPVIssuerWarp) << 8;
-  const uint32_t lane = tid_x() & 31u;
-  uint32_t g0 = 0, cleared = 0;  // bit e: parity of the next cleared stage in entry e
+  uint32_t g = 0;
   bool ok = true;
-  for (PagedWalk w(p, start); w.more(); w.next(p)) {
-    const int from = clear_from(w.blocks, w.off + w.take - 1);
-    const int plain = w.take - (from < kPagedBlock ? 1 : 0);
-    auto pv = [&](int j, bool cluster) -> bool {
-      const uint32_t g = g0 + uint32_t(j), b = buf(g), e = ring_entry(g);
-      const uint32_t bar = sm.bar(kBarVFull + int(e));
-      // Cluster scope where rank 1's rows of V were cleared by plain stores.
-      if (!(cluster ? wait.operator()<true>(bar, ring_parity(g), site | uint32_t(kBarVFull + int(e)))
-                    : wait(bar, ring_parity(g), site | uint32_t(kBarVFull + int(e)))) ||
-          !wait(sm.bar(kBarPFull + int(b)), buf_parity(g), site | uint32_t(kBarPFull + int(b))))
-        return false;
+  for (PagedWalk w(p, start); ok && w.more(); w.next(p)) {
+    for (int j = 0; j < w.take; ++j, ++g) {
+      const uint32_t b = buf(g), e = ring_entry(g);
+      if (!wait(sm.bar(kBarVFull + int(e)), ring_parity(g), site | uint32_t(kBarVFull + int(e))) ||
+          !wait(sm.bar(kBarPFull + int(b)), buf_parity(g), site | uint32_t(kBarPFull + int(b)))) {
+        ok = false;
+        break;
+      }
       tc_fence_after();
       const uint64_t v_desc = smem_desc(sm.v(e));
 #pragma unroll
@@ -188,66 +163,54 @@ __device__ __forceinline__ void pv_issuer(const PagedParams& p, const PagedStart
                     kk > 0 || j > 0 ? 1u : 0u);
       mma_commit_pair_both(sm.bar(kBarPVDone + int(b)));
       mma_commit_pair_both(sm.bar(kBarVEmpty + int(e)));
-      return true;
-    };
-    if (elect_one())
-      for (int j = 0; ok && j < plain; ++j) ok = pv(j, false);
-    ok = __all_sync(0xffffffffu, ok);
-    if (ok && plain < w.take) {
-      const uint32_t e = ring_entry(g0 + uint32_t(plain));
-      ok = __all_sync(0xffffffffu, wait(sm.bar(kBarVLand + int(e)), (cleared >> e) & 1u, site | uint32_t(kBarVLand + int(e))));
-      if (ok) {
-        clear_rows(sm.v(e), from, lane);
-        cleared ^= 1u << e;
-        if (elect_one()) {
-          mbar_arrive(sm.bar(kBarVFull + int(e)));
-          ok = pv(plain, true);
-        }
-        ok = __all_sync(0xffffffffu, ok);
-      }
     }
-    if (!ok) break;
-    g0 += uint32_t(w.take);
   }
-  // Issued by the lane that issued the products: commits follow a thread's own.
-  if (elect_one()) {
-    mma_commit_pair(sm.bar(kBarDrain + 1));
-    wait.drain(sm.bar(kBarDrain + 1), 0u, global_timer_ns());
+  mma_commit_pair(sm.bar(kBarDrain + 1));
+  wait.drain(sm.bar(kBarDrain + 1), 0u, global_timer_ns());
+}
+
+// Rank 1, one thread: passes its Q, K and V stages on to rank 0's barriers.
+__device__ __forceinline__ void forward(const PagedParams& p, const PagedStart& start, const Sm& sm, const Wait& wait) {
+  const uint32_t site = (1u << 16) | (uint32_t(kForwardWarp) << 8);
+  uint32_t g = 0;
+  int it = 0;
+  auto pass = [&](int bar, uint32_t parity) -> bool {
+    if (!wait(sm.bar(bar), parity, site | uint32_t(bar))) return false;
+    mbar_arrive_cluster_relaxed(map_shared(sm.bar(bar), 0));
+    return true;
+  };
+  for (PagedWalk w(p, start); w.more(); w.next(p), ++it) {
+    if (!pass(kBarQFull + (it & 1), uint32_t(it >> 1) & 1u)) return;
+    for (int j = 0; j < w.take; ++j, ++g) {
+      const int e = int(ring_entry(g));
+      if (!pass(kBarKFull + e, ring_parity(g)) || !pass(kBarVFull + e, ring_parity(g))) return;
+    }
   }
 }
 
-// Rank 1, one warp: passes its Q, K and V stages on to rank 0's barriers, and
-// clears V rows that no row of the item sees.
-__device__ __forceinline__ void forward(const PagedParams& p, const PagedStart& start, const Sm& sm, const Wait& wait, uint32_t lane) {
-  const uint32_t site = (1u << 16) | (uint32_t(kForwardWarp) << 8);
-  uint32_t g = 0;
-  bool ok = true;
-  int it = 0;
-  // Bounded wait of lane 0 with a warp-uniform outcome.
-  auto landed = [&](int bar, uint32_t parity) -> bool {
-    uint32_t got = 1;
-    if (lane == 0) got = wait(sm.bar(bar), parity, site | uint32_t(bar)) ? 1u : 0u;
-    return __shfl_sync(0xffffffffu, got, 0) != 0u;
-  };
-  auto pass = [&](int bar) {
-    if (lane == 0) mbar_arrive_cluster_relaxed(map_shared(sm.bar(bar), 0));
-  };
-  for (PagedWalk w(p, start); ok && w.more(); w.next(p), ++it) {
-    if (!(ok = landed(kBarQFull + (it & 1), uint32_t(it >> 1) & 1u))) break;
-    pass(kBarQFull + (it & 1));
-    for (int j = 0; j < w.take; ++j, ++g) {
-      const int e = int(ring_entry(g));
-      if (!(ok = landed(kBarKFull + e, ring_parity(g)))) break;
-      pass(kBarKFull + e);
-      if (!(ok = landed(kBarVLand + e, ring_parity(g)))) break;
-      const int from = clear_from(w.blocks, w.off + j);
-      if (from < kPagedBlock) {
-        mbar_test(sm.bar(kBarVLand + e), ring_parity(g));  // every lane observes the copy
-        clear_rows(sm.v(uint32_t(e)), from, lane);
-        if (lane == 0) mbar_arrive_cluster(map_shared(sm.bar(kBarVFull + e), 0));
-      } else {
-        pass(kBarVFull + e);
-      }
+// V of a block that holds keys that no row of the item sees: 0 times what may be
+// an infinity or NaN is no 0, so zeros take their place.  Boxes of 8 keys, of
+// single ones where a group of 8 is seen in part (a row's place in the swizzle
+// goes by its address); the unseen ones name the page behind the cache, for
+// which a copy delivers zeros.  At most 48 boxes, once to three times an item,
+// and nothing else in the kernel has to know.  (Cleared after the copy instead,
+// by warps between it and the products, chunks took up to 28 % longer: the loops
+// of the issuing warps grew.)
+// `pages`: shared memory, the block's page numbers; the keys before `end_key` and
+// not between the sinks and `first_key` are seen.
+__device__ __noinline__ void load_seen_v(const PagedParams& p, uint32_t pages, int end_key, int first_key, int key0, int h, int col,
+                                         uint32_t dst, uint32_t bar) {
+  const int size_mask = (1 << p.page_shift) - 1, shift = p.page_shift < 7 ? p.page_shift : 7;
+#pragma unroll 1
+  for (int c = 0; c < kPagedBlock; c += 8, dst += 1024u) {
+    const int page = int(ld_volatile_shared(pages + 4u * uint32_t(c >> shift))), key = key0 + c;
+    const uint32_t seen = bits_below(end_key - key) & (bits_below(p.sinks - key) | ~bits_below(first_key - key)) & 255u;
+    if (seen == 0u || seen == 255u) {
+      tma_load_4d(dst, &p.tm_v8, bar, col, key & size_mask, h, seen ? page : p.num_pages);
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i)
+        tma_load_4d(dst + uint32_t(i) * 128u, &p.tm_v1, bar, col, (key + i) & size_mask, h, (seen >> i) & 1u ? page : p.num_pages);
     }
   }
 }
@@ -306,13 +269,16 @@ __device__ __forceinline__ void load(const PagedParams& p, const PagedStart& sta
               tma_load_4d(dst + kKBoxBytes, &p.tm_k, sm.bar(kBarKFull + int(e)), 64, key & size_mask, w.h, page);
             }
           } else {
-            // Rank 1's V is handed over by its warp 11; rank 0's where it needs clearing.
-            const bool hand = rank == 1 || w.blocks.end_key < key + kPagedBlock;
-            const int bar = (hand ? kBarVLand : kBarVFull) + int(e);
+            const int bar = kBarVFull + int(e);
             if (!(ok = claim(kBarVEmpty + int(e), ring_parity(g) ^ 1u, bar, kStageBytes))) break;
             uint32_t dst = sm.v(e);
-            for (int i = 0; i < feed.per; ++i, dst += uint32_t(feed.rows) * 128u, key += feed.rows)
-              tma_load_4d(dst, &p.tm_v, sm.bar(bar), int(rank) * kPairDims, key & size_mask, w.h, feed(j, i));
+            if (w.blocks.unseen(p, key)) {
+              load_seen_v(p, feed.slots + 4u * uint32_t(j * feed.per), w.blocks.end_key, w.blocks.first_key, key, w.h,
+                          int(rank) * kPairDims, dst, sm.bar(bar));
+            } else {
+              for (int i = 0; i < feed.per; ++i, dst += uint32_t(feed.rows) * 128u, key += feed.rows)
+                tma_load_4d(dst, &p.tm_v, sm.bar(bar), int(rank) * kPairDims, key & size_mask, w.h, feed(j, i));
+            }
           }
           ++issued;
         }
@@ -324,7 +290,7 @@ __device__ __forceinline__ void load(const PagedParams& p, const PagedStart& sta
   // The last copies land before the CTA exits, also when a role gave up.
   if (elect_one()) {
     const uint64_t t0 = global_timer_ns();
-    const int full = kV ? (rank == 1 ? kBarVLand : kBarVFull) : kBarKFull;
+    const int full = kV ? kBarVFull : kBarKFull;
     for (uint32_t i = issued > kRing ? issued - kRing : 0; i < issued; ++i) wait.drain(sm.bar(full + int(ring_entry(i))), ring_parity(i), t0);
     for (uint32_t i = q_issued > 2 ? q_issued - 2 : 0; i < q_issued; ++i) wait.drain(sm.bar(kBarQFull + int(i & 1u)), (i >> 1) & 1u, t0);
   }
@@ -595,9 +561,8 @@ __device__ __forceinline__ void setup(const PagedParams& p, uint8_t* raw) {
     for (int e = 0; e < kRing; ++e) {
       mbar_init(sm.bar(kBarKFull + e), fed);
       mbar_init(sm.bar(kBarKEmpty + e), 1);
-      mbar_init(sm.bar(kBarVFull + e), 2);  // rank 0: both ranks' hand-overs
+      mbar_init(sm.bar(kBarVFull + e), fed);
       mbar_init(sm.bar(kBarVEmpty + e), 1);
-      mbar_init(sm.bar(kBarVLand + e), 1);
     }
     st_volatile_shared(sm.abort_slot(), 0u);
     fence_mbarrier_init();
@@ -639,13 +604,15 @@ __device__ __forceinline__ void roles(const PagedParams& p, uint8_t* raw) {
     } else if (warp == (rank == 0 ? kForwardWarp : kPVIssuerWarp)) {
       load<true>(p, start, sm, wait, rank, warp, lane);
     } else if (warp == kForwardWarp) {
-      forward(p, start, sm, wait, lane);
+      if (elect_one()) forward(p, start, sm, wait);
     } else if (rank == 1) {
       if (lane == 0) write_record(p, start, int(cluster_id_x()));
     } else {
       const uint32_t tmem = ld_volatile_shared(sm.tmem_slot());
-      if (warp == kPVIssuerWarp) pv_issuer<kBf16>(p, start, sm, tmem, wait);
-      else if (elect_one()) s_issuer<kBf16>(p, start, sm, tmem, wait);
+      if (elect_one()) {
+        if (warp == kPVIssuerWarp) pv_issuer<kBf16>(p, start, sm, tmem, wait);
+        else s_issuer<kBf16>(p, start, sm, tmem, wait);
+      }
     }
   }
   __syncwarp();

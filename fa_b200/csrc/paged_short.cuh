@@ -279,12 +279,15 @@ __device__ __forceinline__ void short_rows(const PagedParams& p, const PagedStar
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tile = sm + kSmRing + e * kTileBytes;
-      if (key0 + kPagedBlock > w.blocks.end_key) {
-        // Values behind the last key that any row sees may be anything, and
+      if (w.blocks.unseen(p, key0)) {
+        // Values at keys that no row of the item sees may be anything, and
         // 0 * NaN is no 0: this warp's rows of them are cleared.
-        const int from = max(wk0, w.blocks.end_key - key0);
-        for (int i = int(lane); i < (wk0 + kKeys - from) * 16; i += 32)
-          st_shared_v4(tile + row_of(from + (i >> 4)) + (i & 1) * half_bytes + uint32_t((i >> 1) & 7) * 16u, 0, 0, 0, 0);
+        for (int part = 0; part < 2; ++part) {
+          const int2 keys = w.blocks.unseen_keys(p, key0, part);
+          const int from = max(wk0, keys.x), to = min(wk0 + kKeys, keys.y);
+          for (int i = int(lane); i < (to - from) * 16; i += 32)
+            st_shared_v4(tile + row_of(from + (i >> 4)) + (i & 1) * half_bytes + uint32_t((i >> 1) & 7) * 16u, 0, 0, 0, 0);
+        }
         fence_proxy_async_smem();  // the next copy into this entry follows these writes
         __syncwarp();
       }

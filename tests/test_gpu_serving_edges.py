@@ -463,3 +463,48 @@ def test_dense_values_behind_the_last_row_may_be_anything(nq, nk, window, sinks)
     want = op(q, k, v, causal=True, window=window, sinks=sinks)
     k[:, :, nq:], v[:, :, nq:] = float("nan"), float("nan")
     assert torch.equal(op(q, k, v, causal=True, window=window, sinks=sinks), want)
+
+
+# --------------------------------------- values at keys that no row of an item sees
+def _plant(pages, table, r, keys, value):
+    ps = pages.shape[1]
+    pages[table[r].long()[keys // ps], keys % ps] = value
+
+
+@gpu
+@pytest.mark.parametrize("value", [float("nan"), float("inf")], ids=["nan", "inf"])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 4), (64, 0), (64, 130), (128, 4), (200, 1), (200, 129), (300, 20), (513, 300)])
+@pytest.mark.parametrize("hq,hkv,ps,dtype", [(12, 1, 16, F16), (8, 2, 64, BF16), (4, 4, 8, F16), (16, 1, 256, BF16)])
+@pytest.mark.parametrize("lens", [[(1, 1500), (1, 333), (3, 900), (1, 130)], [(300, 1500), (1, 700), (90, 640)]], ids=["short", "chunk"])
+def test_paged_values_outside_every_window_may_be_anything(lens, hq, hkv, ps, dtype, window, sinks, value):
+    from fa_b200.paged import PagedOperator
+
+    q, kp, vp, table, kv, cu = _cache(lens, hq, hkv, ps, dtype, 3)
+    op, longest = PagedOperator(), max(n for n, _ in lens)
+    want = op(q, kp, vp, table, kv, cu, max_q=longest, window=window, sinks=sinks)
+    for r, (n, total) in enumerate(lens):
+        hidden = torch.arange(sinks, max(sinks, total - n + 1 - window), device="cuda")
+        _plant(vp, table, r, hidden, value)
+        _plant(kp, table, r, hidden, float("nan"))
+    got = op(q, kp, vp, table, kv, cu, max_q=longest, window=window, sinks=sinks)
+    assert op.status("cuda")[0] == 0
+    assert torch.isfinite(want).all() and torch.equal(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("hq,hkv", [(12, 1), (6, 6)])
+def test_a_value_leaves_the_rows_behind_its_window_alone(hq, hkv):
+    """A key that an earlier tile of the same chunk sees, and later ones do not."""
+    from fa_b200.paged import PagedOperator
+
+    window, sinks, n = 70, 3, 1200
+    q, kp, vp, table, kv, cu = _cache([(n, n + 40)], hq, hkv, 16, F16, 4)
+    op = PagedOperator()
+    want = op(q, kp, vp, table, kv, cu, max_q=n, window=window, sinks=sinks)
+    for key in (17, 128, 255, 300, 511):
+        _plant(vp, table, 0, torch.tensor([key], device="cuda"), float("nan"))
+        got = op(q, kp, vp, table, kv, cu, max_q=n, window=window, sinks=sinks)
+        clean = key - 40 + window + 256  # a tile of 256 rows further on
+        assert torch.equal(got[max(0, clean):], want[max(0, clean):])
+        if key > 40:
+            assert torch.isnan(got[key - 40]).all()  # the row at the key itself does see it
