@@ -215,7 +215,8 @@ int b200fa_paged_fwd(const b200fa_paged_args* args, void* stream) {
   if (rc != B200FA_OK) return rc;
   if (!a.workspace || (reinterpret_cast<uintptr_t>(a.workspace) & 255u))
     return fail(B200FA_ERR_WORKSPACE, "workspace must be 256-byte aligned");
-  if (reinterpret_cast<uintptr_t>(a.status) & 3u) return fail(B200FA_ERR_ALIGNMENT, "status must be 4-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(a.status) | reinterpret_cast<uintptr_t>(a.tables_status)) & 3u)
+    return fail(B200FA_ERR_ALIGNMENT, "status and tables_status must be 4-byte aligned");
   if (a.requests == 0 || a.tokens == 0) return B200FA_OK;
   const PagedDevice* d = nullptr;
   if ((rc = paged_device(&d)) != B200FA_OK) return rc;
@@ -261,6 +262,7 @@ int b200fa_paged_fwd(const b200fa_paged_args* args, void* stream) {
   p.scale_log2 = float(double(a.scale) * 1.4426950408889634074);
   p.timeout_ns = uint64_t(a.timeout_us ? a.timeout_us : 2000000u) * 1000ull;
   p.flags = a.flags;
+  p.tables_status = a.tables_status;
   p.ws = static_cast<uint8_t*>(a.workspace);
   p.status = a.status ? a.status : static_cast<uint32_t*>(a.workspace);
   const bool bf16 = a.dtype == B200FA_DTYPE_BF16;

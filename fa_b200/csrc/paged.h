@@ -57,6 +57,7 @@ struct PagedParams {
   int32_t part_rows;        // rows of a partial result
   uint64_t timeout_ns;
   uint32_t flags;           // B200FA_PAGED_TEST_WITHHOLD_V
+  const int32_t* tables_status;  // other than 0: no row sees a key; may be NULL
   uint8_t* ws;
   uint32_t* status;
 };
@@ -77,6 +78,7 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedParams& p, int 
   b = b < a ? a : b > p.tokens ? p.tokens : b;
   const int64_t most = int64_t(p.width) << p.page_shift;
   int kv = p.kv_lens[r];
+  if (p.tables_status != nullptr && *p.tables_status != 0) kv = 0;
   kv = kv < 0 ? 0 : kv > most ? int(most) : kv;
   return PagedRequest{a, b - a, kv};
 }

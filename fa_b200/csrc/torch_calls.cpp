@@ -337,7 +337,7 @@ std::optional<Tensor> append(const Tensor& k, const Tensor& v, const Tensor& kp,
 
 Tensor paged(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& kv, const Tensor& cu,
              int64_t max_q, double scale, int64_t window, int64_t sinks, const std::optional<Tensor>& out_in, const Tensor& status,
-             uint32_t timeout_us, uint32_t flags) {
+             uint32_t timeout_us, uint32_t flags, const std::optional<Tensor>& tables_status) {
   constexpr int64_t kDim = 128;
   need_pages(kp, vp, kDim);
   need(q.dim() == 3, "q must be [T, Hq, 128]");
@@ -394,6 +394,10 @@ Tensor paged(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& 
   a.workspace = ws.data_ptr();
   a.ws_bytes = uint64_t(ws.numel());
   a.status = static_cast<uint32_t*>(status.data_ptr());
+  if (tables_status) {
+    need_int32("tables_status", *tables_status, 1, dev);
+    a.tables_status = ptr<int32_t>(*tables_status);
+  }
   check(g.paged_fwd(&a, stream_of(dev)), "b200fa_paged_fwd");
   if (out_in) written(out);
   return out;

@@ -76,7 +76,8 @@ class PagedArgs(C.Structure):
                 ("tokens", _i64), ("num_pages", _i64),
                 ("requests", _i32), ("width", _i32), ("page_size", _i32), ("heads_q", _i32), ("heads_kv", _i32),
                 ("max_q", _i32), ("scale", _f), ("window", _i32), ("sinks", _i32), ("timeout_us", _u32),
-                ("flags", _u32), ("workspace", C.c_void_p), ("ws_bytes", _u64), ("status", C.c_void_p)]
+                ("flags", _u32), ("workspace", C.c_void_p), ("ws_bytes", _u64), ("status", C.c_void_p),
+                ("tables_status", C.c_void_p)]
 
 
 Strides2, Strides3 = _i64 * 2, _i64 * 3

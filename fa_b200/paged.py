@@ -35,11 +35,13 @@ class StepTables:
     cu_q: torch.Tensor       # int32 [R + 1]
     kv_lens: torch.Tensor    # int32 [R]
     free_left: torch.Tensor  # int32 [1]
-    status: torch.Tensor     # int32 [1]
+    status: torch.Tensor     # int32 [1]; None: taken to be 0
 
     @staticmethod
     def empty(requests: int, num_tokens: int, device) -> "StepTables":
-        return StepTables(*calls.load().empty_tables(requests, num_tokens, torch.device(device)))
+        tables = StepTables(*calls.load().empty_tables(requests, num_tokens, torch.device(device)))
+        tables.status.zero_()
+        return tables
 
     def tensors(self) -> tuple:
         return (self.slots, self.positions, self.cu_q, self.kv_lens, self.free_left, self.status)
@@ -57,8 +59,9 @@ def build_tables(ctx_lens, new_lens, block_table, free_pages, free_count, *, pag
     token get slot -1 and position 0.
 
     ``status`` (on the GPU) is 0, or 1: too few free pages, 2: a request
-    outgrows its row of block_table or 2^31 - 1 tokens, 3: more new tokens than num_tokens; then
-    nothing is handed out, every slot is -1, kv_lens are ctx_lens and the table
+    outgrows its row of block_table or 2^31 - 1 tokens, 3: more new tokens than
+    num_tokens; then nothing is handed out, every slot is -1, kv_lens are ctx_lens (cu_q still
+    counts the new tokens; ``PagedOperator.step`` gives zeros) and the table
     is as it was.  The outputs must not overlap the inputs or one another: a
     loop alternates between two ``StepTables``.
     """
@@ -128,7 +131,8 @@ class PagedOperator:
         return ws
 
     def __call__(self, q, k_pages, v_pages, block_table, kv_lens, cu_q, *, max_q: int, scale: float | None = None,
-                 window: int = 0, sinks: int = 0, out: torch.Tensor | None = None, flags: int = 0) -> torch.Tensor:
+                 window: int = 0, sinks: int = 0, out: torch.Tensor | None = None, flags: int = 0,
+                 tables_status: torch.Tensor | None = None) -> torch.Tensor:
         """q [T, Hq, 128]; block_table int32 [R, width]; kv_lens int32 [R], the
         cached tokens of each request, its new ones included; cu_q int32
         [R + 1], the requests' rows of q.  Row i of request r stands at
@@ -142,24 +146,29 @@ class PagedOperator:
         any row of its work item sees is not read.  Where the table ends early
         or names a page outside the cache, zeros are read and
         ``status(device)`` says so.  A NaN or infinity in V at a key that some
-        row of a work item sees can reach all of that item's rows."""
+        row of a work item sees can reach all of that item's rows.
+
+        ``tables_status`` (int32 [1] on the GPU): the status of the step's
+        ``build_tables``.  Where it is not 0 the new tokens have no place in the
+        cache, and all their rows become zeros."""
         window, sinks = _window(window, sinks, True)
         return calls.load().paged(q, k_pages, v_pages, block_table, kv_lens, cu_q, max_q,
                                   HEAD_DIM ** -0.5 if scale is None else scale, window, sinks, out,
-                                  self.workspace(q.device), self.timeout_us, flags)
+                                  self.workspace(q.device), self.timeout_us, flags, tables_status)
 
     def step(self, q, k, v, k_pages, v_pages, block_table, tables: StepTables, *, max_q: int,
              rotary: Rotary | None = None, scale: float | None = None, window: int = 0, sinks: int = 0,
              out: torch.Tensor | None = None) -> torch.Tensor:
         """The attention of one layer in a step: appends k and v to the cache
         at ``tables``' slots, rotated when ``rotary`` is given, and returns
-        the attention of the (rotated) q over it."""
+        the attention of the (rotated) q over it.  After a step that could not
+        be met (``tables.status``) the cache is as it was and the rows are zeros."""
         if q.requires_grad:
             q = q.detach()  # the attention has no graph
         turned = append(k, v, k_pages, v_pages, tables.slots, q=q if rotary is not None else None,
                         positions=tables.positions if rotary is not None else None, rotary=rotary)
         return self(q if turned is None else turned, k_pages, v_pages, block_table, tables.kv_lens, tables.cu_q,
-                    max_q=max_q, scale=scale, window=window, sinks=sinks, out=out)
+                    max_q=max_q, scale=scale, window=window, sinks=sinks, out=out, tables_status=tables.status)
 
     def status(self, device) -> tuple[int, int, int, int]:
         """Synchronize the device and read the status words {status, site, block, 0}."""

@@ -410,6 +410,9 @@ typedef struct b200fa_paged_args {
                                    b200fa_reset_status); NULL: the first ones of
                                    the workspace.  A struct that ends before this
                                    field is accepted too.                        */
+    const int32_t* tables_status; /* b200fa_build_tables' status, or NULL: other
+                                   than 0, nothing was handed out for the new
+                                   tokens and all their rows become zeros        */
 } b200fa_paged_args;
 
 /* Test-only: no V block is loaded, so that the waits for it run out and the

@@ -508,3 +508,50 @@ def test_a_value_leaves_the_rows_behind_its_window_alone(hq, hkv):
         assert torch.equal(got[max(0, clean):], want[max(0, clean):])
         if key > 40:
             assert torch.isnan(got[key - 40]).all()  # the row at the key itself does see it
+
+
+# ------------------------------------------------- a step that could not be met
+@gpu
+@pytest.mark.parametrize("R,new,width,T,status", [(2, [5, 90], 8, 256, 1), (2, [5, 300], 8, 512, 2), (2, [5, 90], 8, 64, 3)])
+@pytest.mark.parametrize("max_q", [1, 90])
+def test_a_step_without_pages_gives_zeros_and_leaves_the_cache(R, new, width, T, status, max_q):
+    """Nothing was handed out, so the new tokens have no place: their rows must
+    not look like an answer, and the next step that can be met is right."""
+    from fa_b200.paged import PagedOperator, build_tables
+
+    ps, hq, hkv = 16, 4, 2
+    lens, free = i32([20, 30]), torch.arange(4, 8, device="cuda").int()
+    table = torch.full((R, width), -1, dtype=torch.int32, device="cuda")
+    table[0, :2], table[1, :2] = i32([0, 1]), i32([2, 3])
+    kp, vp = (torch.randn((8, ps, hkv, 128), device="cuda").half() for _ in range(2))
+    kc, vc = kp.clone(), vp.clone()
+    q, k, v = (torch.randn((T, h, 128), device="cuda").half() for h in (hq, hkv, hkv))
+    op = PagedOperator()
+    t = build_tables(lens, i32(new), table, free, i32([4]), page_size=ps, num_tokens=T)
+    assert t.status.tolist() == [status]
+    out = torch.full_like(q, 7.0)
+    op.step(q, k, v, kp, vp, table, t, max_q=max_q, out=out)
+    n = min(sum(new), T)
+    assert bool((out[:n] == 0).all()) and bool((out[n:] == 7.0).all())
+    assert op.status("cuda")[0] == 0 and torch.equal(kp, kc) and torch.equal(vp, vc)
+    t = build_tables(t.kv_lens, i32([5, 20]), table, free, t.free_left, page_size=ps, num_tokens=T)
+    assert t.status.tolist() == [0]
+    out = op.step(q, k, v, kp, vp, table, t, max_q=max_q)
+    O, A = ref.paged_attention(q, kp, vp, table, t.kv_lens, t.cu_q)
+    bound = A[:25] * (HALF[F16] + 3e-4 + 2.0 ** -16) + O[:25].abs() * HALF[F16] + 2.0 ** -24
+    assert bool(((out[:25].double() - O[:25]).abs() <= bound).all())
+
+
+@gpu
+def test_tables_filled_by_hand_need_no_status():
+    from fa_b200.paged import PagedOperator, StepTables
+
+    q, kp, vp, table, kv, cu = _cache([(2, 40), (1, 7)], 4, 2, 16, F16, 5)
+    op = PagedOperator()
+    want = op(q, kp, vp, table, kv, cu, max_q=2)
+    k, v = (torch.zeros((3, 2, 128), dtype=F16, device="cuda") for _ in range(2))
+    t = StepTables.empty(2, 3, "cuda")
+    t.slots.fill_(-1), t.positions.zero_(), t.cu_q.copy_(cu), t.kv_lens.copy_(kv)
+    assert torch.equal(op.step(q, k, v, kp, vp, table, t, max_q=2), want)
+    t.status = None
+    assert torch.equal(op.step(q, k, v, kp, vp, table, t, max_q=2), want)
