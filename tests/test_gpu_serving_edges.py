@@ -5,8 +5,10 @@ test_gpu_serving.py; most checks here are for equality."""
 
 import copy
 import pickle
+import re
 import threading
 import time
+from pathlib import Path
 
 import pytest
 import torch
@@ -15,6 +17,7 @@ from oracle import serving_ref as ref
 
 F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
 gpu = pytest.mark.gpu
+ROOT = Path(__file__).resolve().parents[1]
 HALF = {t: torch.finfo(t).eps / 2 for t in (F16, BF16, F32)}
 i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
 
@@ -555,3 +558,52 @@ def test_tables_filled_by_hand_need_no_status():
     assert torch.equal(op.step(q, k, v, kp, vp, table, t, max_q=2), want)
     t.status = None
     assert torch.equal(op.step(q, k, v, kp, vp, table, t, max_q=2), want)
+
+
+# ------------------------------------------------------------------ the README
+@gpu
+def test_the_readme_serving_loop_keeps_its_layers_apart():
+    """The loop as printed, for two layers and three steps, against attention of
+    each layer's own keys."""
+    text = (ROOT / "README.md").read_text()
+    block = next(b for b in re.findall(r"```python\n(.*?)```", text, re.S) if "build_tables" in b)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    results = []
+
+    class Layer:
+        def __init__(self, number):
+            self.number, self.rows = number, []
+
+        def qkv(self):
+            x = [torch.randn((scope["T"], h, 128), generator=g, device="cuda").half() for h in (12, 1, 1)]
+            self.rows.append(x)
+            return x
+
+        def take(self, o):
+            results.append((self.number, len(self.rows) - 1, o.clone()))
+
+    made = [Layer(0), Layer(1)]
+    steps = [i32([9, 3]), i32([1, 40]), i32([1, 1])]
+    scope = {"torch": torch, "R": 2, "layers": made, "steps": steps, "longest": 40}
+    exec(compile(block, "README.md", "exec"), scope)
+    assert len(results) == 6
+    from fa_b200.rotary import Rotary
+
+    rotary, counts = Rotary(128), [s.tolist() for s in steps]
+    for number, step, o in results:
+        layer = made[number]
+        for r in range(2):
+            ks, vs, had = [], [], 0
+            for s in range(step + 1):
+                a = sum(counts[s][:r])
+                ks.append(layer.rows[s][1][a:a + counts[s][r]])
+                vs.append(layer.rows[s][2][a:a + counts[s][r]])
+                had += counts[s][r]
+            n, a = counts[step][r], sum(counts[step][:r])
+            k = rotary(torch.cat(ks).contiguous(), torch.arange(had, device="cuda"))
+            q = rotary(layer.rows[step][0][a:a + n].contiguous(), torch.arange(had - n, had, device="cuda"))
+            see = ref.visible(torch.arange(had - n, had, device="cuda"), had)
+            for h in range(12):
+                O, A = ref.attend(q[:, h], k[:, 0], torch.cat(vs)[:, 0], see, 128 ** -0.5)
+                bound = A * (HALF[F16] + 3e-4 + 2.0 ** -16) + O.abs() * HALF[F16] + 2.0 ** -24
+                assert bool(((o[a:a + n, h].double() - O).abs() <= bound).all())
