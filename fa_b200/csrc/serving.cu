@@ -151,9 +151,9 @@ __global__ void __launch_bounds__(kTableThreads) b200_build_tables_kernel(const 
 // more heads at once per thread: slower still, occupancy fell.)
 //
 // The angle: position times frequency in turns as a 64-bit binary fraction,
-// reduced mod 1 by the integer product's wrap-around.  It is exact whatever
-// the position, where a 32-bit product of position and frequency is off by
-// position * 2^-24 radians (0.008 at 131072).
+// reduced mod 1 by the integer product's wrap-around.  The product is exact, so
+// the angle is off by position * 2^-65 turns, the frequency's rounding, where a
+// 32-bit product is off by position * 2^-24 radians (0.008 at 131072).
 struct Segment {  // a run of heads: rows [batch][n][heads][dim] -> the same, or the cache
   const uint4* src;
   uint4* dst;

@@ -11,8 +11,9 @@ position; ``scaling`` stretches them for contexts longer than trained on:
   number of turns.
 
 ``magnitude`` multiplies the rotated elements.  The kernel keeps each
-frequency as a 64-bit fraction of a turn, so the angle of any position is
-exact before its sine is taken.
+frequency as a 64-bit fraction of a turn, computed in decimal arithmetic and
+rounded once, and multiplies it by the position exactly (mod 1): before its sine
+is taken, the angle of position p is off by p * 2^-65 turns at most.
 """
 
 from __future__ import annotations
@@ -20,6 +21,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import threading
+from decimal import Decimal, localcontext
 
 import torch
 from torch.autograd import forward_ad
@@ -27,6 +29,8 @@ from torch.autograd import forward_ad
 from . import calls, lib
 
 LAYOUTS = {"half": 0, "interleaved": 1}
+
+_PI = Decimal("3.14159265358979323846264338327950288419716939937510")
 
 _first_use = threading.RLock()  # of a Rotary on a device
 
@@ -97,15 +101,21 @@ class Rotary:
         self.dim, self.rotary_dim, self.layout = dim, rotary_dim, layout
         self.magnitude = float(magnitude)
         self.frequencies = []  # angle per position of each pair
-        for i in range(rotary_dim // 2):
-            f = base ** (-2.0 * i / rotary_dim)
-            if scaling == "linear":
-                f /= factor
-            elif scaling == "banded":
-                turns = original_length * f / (2.0 * math.pi)
-                keep = min(1.0, max(0.0, (turns - low) / (high - low)))
-                f = f * keep + f / factor * (1.0 - keep)
-            self.frequencies.append(f)
+        self._turns = []       # the same in turns, mod 1, times 2^64
+        with localcontext() as ctx:
+            ctx.prec = 50
+            factor, low, high, original = (Decimal(float(x)) for x in (factor, low, high, original_length))
+            log_base = Decimal(float(base)).ln()
+            for i in range(rotary_dim // 2):
+                f = (log_base * (-2 * i) / rotary_dim).exp()
+                if scaling == "linear":
+                    f /= factor
+                elif scaling == "banded":
+                    turns = original * f / (2 * _PI)
+                    keep = min(Decimal(1), max(Decimal(0), (turns - low) / (high - low)))
+                    f = f * keep + f / factor * (1 - keep)
+                self.frequencies.append(float(f))
+                self._turns.append(int((f / (2 * _PI) * 2**64).to_integral_value()) % 2**64)
         self._tables = {}  # device -> int64 tensor of 0.64 fixed-point turns
         self._descs = {}   # (device, inverse) -> (RotaryDesc, its address, its table)
 
@@ -123,8 +133,7 @@ class Rotary:
             if t is None:
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("the first use of a Rotary on a device cannot be captured: call table(device) before")
-                turns = [round(f / (2.0 * math.pi) * 2.0**64) % 2**64 for f in self.frequencies]
-                t = torch.tensor([x - 2**64 if x >= 2**63 else x for x in turns], dtype=torch.int64).to(device)
+                t = torch.tensor([x - 2**64 if x >= 2**63 else x for x in self._turns], dtype=torch.int64).to(device)
                 self._tables[device] = t
         return t
 

@@ -336,7 +336,8 @@ int b200fa_build_tables(const int32_t* ctx_lens, const int32_t* new_lens, int32_
 
 /* Rotary positions.  freq[i] is pair i's angle per position in turns, as a
  * 64-bit binary fraction (0.64 fixed point); the angle of position p is
- * p * freq[i] mod 1, exact for any 63-bit p.  layout 0: pair (i, i + rot/2);
+ * p * freq[i] mod 1 (the product is exact; the frequency's own rounding,
+ * 2^-65 turns, counts p times).  layout 0: pair (i, i + rot/2);
  * 1: pair (2i, 2i + 1).  Elements rot.. of a head are copied.  magnitude
  * multiplies the rotated ones; inverse turns by the negative angle. */
 typedef struct b200fa_rotary_desc {

@@ -4,6 +4,7 @@ bounds of waits, ends of the number ranges.  Tolerances as in
 test_gpu_serving.py; most checks here are for equality."""
 
 import copy
+import math
 import pickle
 import re
 import threading
@@ -607,3 +608,38 @@ def test_the_readme_serving_loop_keeps_its_layers_apart():
                 O, A = ref.attend(q[:, h], k[:, 0], torch.cat(vs)[:, 0], see, 128 ** -0.5)
                 bound = A * (HALF[F16] + 3e-4 + 2.0 ** -16) + O.abs() * HALF[F16] + 2.0 ** -24
                 assert bool(((o[a:a + n, h].double() - O).abs() <= bound).all())
+
+
+# --------------------------------------------------------- ends of the number ranges
+@gpu
+@pytest.mark.parametrize("kw", [{}, {"scaling": "linear", "factor": 3.0}, {"base": 500000.0, "scaling": "banded", "factor": 8.0,
+                                                                       "original_length": 8192}], ids=["plain", "linear", "banded"])
+def test_angles_of_very_far_positions(kw):
+    """Against 60-digit arithmetic.  The angle of position p is off by at most
+    p * 2^-65 turns (the frequency's rounding) and 2^-25 turns (its 32-bit sine)."""
+    from decimal import Decimal, localcontext
+
+    from fa_b200.rotary import Rotary
+
+    rot = 64
+    x = torch.zeros((1, 1, 1, rot), device="cuda")
+    x[..., : rot // 2] = 1.0  # y = (cos, sin) of each pair
+    rotary = Rotary(rot, **kw)
+    for p in (3, 2**20 + 1, 2**31 - 1, 2**40 + 12345, 2**50 + 7):
+        y = rotary(x, torch.tensor([p], device="cuda"))[0, 0, 0].double().cpu()
+        with localcontext() as ctx:
+            ctx.prec = 60
+            pi = Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+            base, factor = Decimal(kw.get("base", 10000.0)), Decimal(kw.get("factor", 1.0))
+            for i in range(rot // 2):
+                f = (base.ln() * Decimal(-2 * i) / rot).exp()
+                if kw.get("scaling") == "linear":
+                    f /= factor
+                elif kw.get("scaling") == "banded":
+                    turns = kw["original_length"] * f / (2 * pi)
+                    keep = min(Decimal(1), max(Decimal(0), (turns - 1) / 3))
+                    f = f * keep + f / factor * (1 - keep)
+                turn = p * f / (2 * pi) % 1
+                a = float(turn * 2 * pi)
+                tol = 6e-7 * 2 + 2 * math.pi * p * 2.0 ** -65
+                assert abs(float(y[i]) - math.cos(a)) <= tol and abs(float(y[i + rot // 2]) - math.sin(a)) <= tol, (p, i)
