@@ -133,23 +133,21 @@ __device__ __forceinline__ PagedBlocks paged_blocks(const PagedParams& p, const 
   return b;
 }
 
-// sum over i < n of floor((a i + b) / m), a, b >= 0, by the Euclidean
-// reduction of (a, m) (the lattice points under a line).
-__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
-  int64_t sum = 0;
-  while (n > 0) {
-    sum += a / m * (n * (n - 1) / 2) + b / m * n;
-    a %= m;
-    b %= m;
-    const int64_t top = a * n + b;
-    if (top < m) break;
-    n = top / m;
-    b = top % m;
-    const int64_t t = m;
-    m = a;
-    a = t;
+// Sum over i < n of floor((k i + b) / 128), k > 0, b >= 0: the numerators' sum less
+// that of their residues mod 128.  With g the largest power of two (up to 128) in
+// k, the residues repeat after 128 / g terms, which take every value that is b mod
+// g once; what is left of a period is added up term by term (a few, mostly: a
+// request's tiles).
+__device__ __forceinline__ int64_t block_sum(int64_t n, int k, int64_t b) {
+  static_assert(kPagedBlock == 128, "residues mod 128");
+  const int log_g = __ffs(k) - 1 < 7 ? __ffs(k) - 1 : 7, g = 1 << log_g, period = 128 >> log_g;
+  int64_t residues = (n >> (7 - log_g)) * (int64_t(period) * (int(b) & (g - 1)) + 64 * (period - 1));
+  int r = int(b) & 127;
+  for (int i = int(n) & (period - 1); i > 0; --i) {
+    residues += r;
+    r = (r + k) & 127;
   }
-  return sum;
+  return (k * (n * (n - 1) / 2) + b * n - residues) >> 7;
 }
 
 // Key blocks of the request's first `tiles` tiles, for one key/value head: the
@@ -167,13 +165,13 @@ __device__ __forceinline__ int64_t blocks_before(const PagedParams& p, const Pag
   const int64_t full = tiles < last ? tiles : last;  // tiles that are not the request's last
   if (t1 > full) t1 = full;
   n += t1;
-  n += floor_sum(full - t1, kPagedBlock, k, c + k * t1 + k - 1) + (full - t1);
+  n += block_sum(full - t1, int(k), c + k * t1 + k - 1) + (full - t1);
   if (tiles > last) n += q.kv > 0 ? (q.kv - 1) / kPagedBlock + 1 : 1;
   if (p.window > 0) {
     const int64_t s = p.sinks / kPagedBlock + (p.sinks % kPagedBlock != 0);
     const int64_t b = c - (p.window - 1) - s * kPagedBlock;  // keys of tile 0 between its window and the sinks' blocks
     int64_t t2 = b < 0 ? (-b + k - 1) / k : 0;
-    if (t2 < tiles) n -= floor_sum(tiles - t2, kPagedBlock, k, b + k * t2);
+    if (t2 < tiles) n -= block_sum(tiles - t2, int(k), b + k * t2);
   }
   return n;
 }

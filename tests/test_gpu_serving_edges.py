@@ -643,3 +643,18 @@ def test_angles_of_very_far_positions(kw):
                 a = float(turn * 2 * pi)
                 tol = 6e-7 * 2 + 2 * math.pi * p * 2.0 ** -65
                 assert abs(float(y[i]) - math.cos(a)) <= tol and abs(float(y[i + rot // 2]) - math.sin(a)) <= tol, (p, i)
+
+
+@gpu
+@pytest.mark.parametrize("hq,hkv,tokens", [(12, 1, 1), (5, 1, 3), (3, 1, 5), (7, 7, 16), (9, 1, 1)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (90, 0), (260, 131)])
+def test_many_tiles_of_few_tokens_are_placed_right(hq, hkv, tokens, window, sinks):
+    """max_q = 1 for long requests: tiles of 1, 3, 5 or 16 tokens, hundreds of a request."""
+    from fa_b200.paged import PagedOperator
+
+    assert 16 // (hq // hkv) == tokens
+    q, kp, vp, table, kv, cu = _cache([(700, 900), (1, 40), (333, 1000), (129, 129)], hq, hkv, 16, F16, 14)
+    out = PagedOperator()(q, kp, vp, table, kv, cu, max_q=1, window=window, sinks=sinks)
+    O, A = ref.paged_attention(q, kp, vp, table, kv, cu, window, sinks)
+    bound = A * (HALF[F16] + 3e-4 + 2.0 ** -16) + O.abs() * HALF[F16] + 2.0 ** -24
+    assert bool(((out.double() - O).abs() <= bound).all())
