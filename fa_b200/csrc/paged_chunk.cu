@@ -1,8 +1,7 @@
 // paged_chunk.cu -- attention over a paged cache for many rows: chunks of
 // prompts.  Bound by the tensor cores (4 * 128 * rows flops per key), so the
-// products run as the dense attention kernel's do (fa_kernel.cuh, whose
-// pipeline, tensor memory layout and register split this kernel shares):
-// pairs of CTAs, tcgen05 cta_group::2, M = 256, S and PV issued by a thread
+// products run as the dense attention kernel's do (fa_kernel.cuh; what the two
+// share is in fa_pipeline.cuh): pairs of CTAs, tcgen05 cta_group::2, M = 256, S and PV issued by a thread
 // each, two softmax warpgroups on alternate key blocks, TMA rings for K and V.
 //
 // What differs:
@@ -23,16 +22,8 @@
 //   * an item that lies in the stretch is normalised and stored; one that a
 //     stretch's end cuts leaves FP32 partial results, joined by
 //     b200_paged_combine_kernel.
-#define B200FA_CAUSAL 1
-#define B200FA_WINDOW 1  // for bits_below
-#define s_issuer_role s_issuer_role_paged_unused
-#define pv_issuer_role pv_issuer_role_paged_unused
-#define watch_role watch_role_paged_unused
-#define forward_role forward_role_paged_unused
-#define load_role load_role_paged_unused
-#include "fa_kernel.cuh"
-
 #include "b200fa.h"
+#include "fa_pipeline.cuh"
 #include "paged.h"
 #include "paged_common.cuh"
 
