@@ -13,6 +13,7 @@ namespace b200fa {
 namespace {
 
 constexpr int64_t kInt32Max = (int64_t(1) << 31) - 1;
+constexpr int kSms = 148;  // of a B200: sizes grids only
 
 // ------------------------------------------------------------ page tables
 // Latency-bound: a few KB in, 12 bytes per token out.  Every block scans all
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(kTableThreads) b200_build_tables_kernel(const 
 // each, into shared memory while its first rows are on their way, and then turns
 // (or copies) sixteen elements -- eight pairs -- of a row per thread and step,
 // the next row's loads ahead of this one's stores.  16000 tokens of 48 heads,
-// half of them turned: 69 us, 5.7 TB/s; 2 x 12 x 32768 rows: 75 us, 5.4 TB/s.
+// half of them turned: 69 us, 5.7 TB/s; 2 x 12 x 32768 rows: 79 us, 5.1 TB/s.
 // (Angles in the threads' registers, anew for every eight heads: 100 and 102 us;
 // more heads at once per thread: slower still, occupancy fell.)
 //
@@ -213,7 +214,7 @@ __device__ __forceinline__ void from_float2(float2 x, __nv_bfloat162& o) { o = _
 template <typename T, int kLayout>
 __global__ void __launch_bounds__(256) b200_rotary_kernel(const RotaryParams p) {
   constexpr int kPer = Sixteen<T>::kPer, kPieces = Sixteen<T>::kPieces;
-  extern __shared__ float2 angles[];  // [token of the block][pair]: cos, sin
+  extern __shared__ __align__(16) float2 angles[];  // [token of the block][pair]: cos, sin; read two pairs at a time
   __shared__ int32_t tok_b[kMaxTokens], tok_n[kMaxTokens];
   __shared__ int64_t tok_slot[kMaxTokens];
   const int32_t token0 = int32_t(blockIdx.x) * p.tokens_per_block;
@@ -364,7 +365,7 @@ int launch_rotary(RotaryParams& p, const b200fa_rotary_desc* r, int32_t dim, int
   p.magnitude = r ? r->magnitude : 1.f;
   p.sign = r && r->inverse ? -1.f : 1.f;
   int64_t per = 1;
-  if (p.tokens > 4 * 148) {
+  if (p.tokens > 4 * kSms) {
     per = 288 / p.heads;
     const int64_t most = p.rot ? (16 << 10) / (p.rot * 4) : kMaxTokens;
     per = per < 1 ? 1 : per > kMaxTokens ? kMaxTokens : per;
@@ -388,6 +389,8 @@ int launch_rotary(RotaryParams& p, const b200fa_rotary_desc* r, int32_t dim, int
   return e == cudaSuccess ? B200FA_OK : cuda_fail(e, "rotary kernel launch");
 }
 
+// Powers of two: a slot's page and offset are a shift and a mask, and a page is
+// whole parts of a 128-key block, or whole blocks.
 int page_shift(int32_t page_size) {
   if (page_size < 8 || page_size > (1 << 20) || (page_size & (page_size - 1))) return -1;
   int s = 0;
@@ -421,7 +424,7 @@ int b200fa_build_tables(const int32_t* ctx_lens, const int32_t* new_lens, int32_
   TableParams p{ctx_lens, new_lens, block_table, table_stride, free_pages, free_count, slots, positions, cu_q, kv_lens,
                 free_left, status, num_tokens, free_capacity, requests, width, shift};
   int64_t blocks = (num_tokens + 4 * kTableThreads - 1) / (4 * kTableThreads);
-  blocks = blocks < 1 ? 1 : blocks > 296 ? 296 : blocks;
+  blocks = blocks < 1 ? 1 : blocks > 2 * kSms ? 2 * kSms : blocks;
   b200_build_tables_kernel<<<unsigned(blocks), kTableThreads, size_t(2 * (requests + 1)) * 4,
                              static_cast<cudaStream_t>(stream)>>>(p);
   const cudaError_t e = cudaGetLastError();
