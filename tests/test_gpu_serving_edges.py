@@ -658,3 +658,48 @@ def test_many_tiles_of_few_tokens_are_placed_right(hq, hkv, tokens, window, sink
     O, A = ref.paged_attention(q, kp, vp, table, kv, cu, window, sinks)
     bound = A * (HALF[F16] + 3e-4 + 2.0 ** -16) + O.abs() * HALF[F16] + 2.0 ** -24
     assert bool(((out.double() - O).abs() <= bound).all())
+
+
+@gpu
+def test_a_rotary_and_its_gradient_in_a_graph():
+    from fa_b200.rotary import Rotary
+
+    rotary, pos = Rotary(64), torch.arange(9, device="cuda") * 5
+    x, g = torch.randn((2, 3, 9, 64), device="cuda").requires_grad_(), torch.randn((2, 3, 9, 64), device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(rotary(x, pos), x, g)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = rotary(x, pos)
+        (grad,) = torch.autograd.grad(y, x, g)
+    for _ in range(2):
+        with torch.no_grad():
+            x.add_(1.0), g.mul_(0.5)
+        graph.replay()
+        assert torch.equal(y.detach(), rotary(x.detach(), pos)) and torch.equal(grad, rotary(g, pos, inverse=True))
+
+
+@gpu
+def test_steps_of_two_threads_on_streams_of_their_own():
+    from fa_b200.paged import PagedOperator
+    from fa_b200.rotary import Rotary
+
+    op, rotary = PagedOperator(), Rotary(128)
+    cases = [_cache([(1, 9000), (2, 500)], 12, 1, 16, F16, 30), _cache([(200, 4000)], 8, 2, 64, F16, 31)]
+    longest = [2, 200]
+    wants = [op(rotary(c[0], torch.zeros(c[0].shape[0], dtype=torch.int64, device="cuda")), *c[1:], max_q=n)
+             for c, n in zip(cases, longest)]
+    torch.cuda.synchronize()
+
+    def work(c, n):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            zero = torch.zeros(c[0].shape[0], dtype=torch.int64, device="cuda")
+            out = [op(rotary(c[0], zero), *c[1:], max_q=n) for _ in range(30)]
+            torch.cuda.current_stream().synchronize()
+            return out
+
+    for want, got in zip(wants, _in_two_threads(*[lambda c=c, n=n: work(c, n) for c, n in zip(cases, longest)])):
+        assert all(torch.equal(o, want) for o in got)
