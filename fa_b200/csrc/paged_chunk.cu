@@ -17,8 +17,8 @@
 //     last, the last of the sinks', the first of the window's -- V is loaded in
 //     smaller boxes, with zeros in those keys' places (load_seen_v).
 //   * scores are masked in tensor memory before the softmax loads them.
-//   * 4096 + 1024 tokens over 32768 + 20480 keys, 12 heads on 1: 826 us in short
-//     bursts, 935 under the power cap, 961 TFLOP/s of visible products.
+//   * 4096 + 1024 tokens over 32768 + 20480 keys, 12 heads on 1: 829 us in short
+//     bursts, 917 under the power cap, 979 TFLOP/s of visible products.
 //   * an item that lies in the stretch is normalised and stored; one that a
 //     stretch's end cuts leaves FP32 partial results, joined by
 //     b200_paged_combine_kernel.
@@ -288,8 +288,10 @@ __device__ __forceinline__ void load(const PagedParams& p, const PagedStart& sta
   __syncwarp();
 }
 
-// Exponentials of 64 keys of one row: P in the cache's type, four chains of
-// FP32 sums.  All through MUFU: with one pair of eight on the FMA pipe, as in
+// Exponentials of 64 keys of one row: P rounded to the cache's type, as the
+// tensor cores take it (errors against 64 bits are 2.3e-3 beside 1.7e-3 with P in
+// 32 bits in BF16, 3.0e-4 beside 2.1e-4 in FP16), and four chains of FP32 sums of
+// the unrounded values.  All through MUFU: with one pair of eight on the FMA pipe, as in
 // the dense kernel, chunks took 4 to 10 % longer here (4 x 512 tokens over 32768
 // keys, 12 heads on 1: 248 against 225 us) -- the pipe's turn comes while the
 // other group loads and reduces, and the loop is shorter without it.

@@ -6,9 +6,10 @@
 // nothing but keep five 32 KiB entries of K and V in flight (a page per
 // TMA box, in two halves of 64 columns, 128-byte swizzle), and eight warps that multiply with
 // mma.sync -- 16 rows are an eighth of a tcgen05 tile, and the products are far
-// from the limit (tensor pipe 17 % busy).  32 tokens over 4096..16384 keys, 32
-// heads on 8: 211 us, 6.5 TB/s of the cache's bytes; one token over 2048 keys,
-// 12 heads on 1: 11 us with the join, a chain of latencies.  A warp owns 16 rows and a share of
+// from the limit (tensor pipe 15 % busy).  32 tokens over 4096..16384 keys, 32
+// heads on 8: 222 us, 6.2 TB/s of the cache's bytes (212 us, 6.5 TB/s in short
+// bursts); one token over 2048 keys, 12 heads on 1: 11 us with the join, a chain
+// of latencies.  A warp owns 16 rows and a share of
 // each block's keys (all eight share the keys of a 16-row tile) with its own
 // running maximum, sum and output in registers; the shares are joined once,
 // at the item's end, through shared memory.
@@ -263,6 +264,9 @@ __device__ __forceinline__ void short_rows(const PagedParams& p, const PagedStar
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[i][0] *= fa, o[i][1] *= fa, o[i][2] *= fb, o[i][3] *= fb;
       }
+      // P is rounded to the cache's type, as the tensor cores take it: errors
+      // against 64 bits are 2.2e-3 beside 1.7e-3 with P in 32 bits (BF16), 2.5e-4
+      // beside 2.2e-4 (FP16).  Its sum is that of the unrounded values.
       uint32_t pf[kTiles][2];
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {

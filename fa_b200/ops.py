@@ -96,7 +96,7 @@ class Operator:
                  unit_range: tuple[int, int] | None = None, flags: int = 0,
                  capture: torch.Tensor | None = None, causal: bool = False, window: int = 0,
                  sinks: int = 0, rotary=None, positions: torch.Tensor | None = None) -> torch.Tensor:
-        """O = softmax(Q K^T * scale) V.  ``causal``: query row i attends keys
+        """O = softmax(Q K^T * scale) V, forward only.  ``causal``: query row i attends keys
         0..i only (top-left aligned, as torch's ``is_causal``; an addition,
         the reference's operator is non-causal).  ``window`` > 0 (with
         ``causal``): only keys i - window < j <= i of those, and the first

@@ -10,7 +10,8 @@ passed as ``pool.transpose(1, 2)``).  One step of a serving loop is
 
 or, the last two together, ``op.step(...)``.  ``t.kv_lens`` and ``t.free_left``
 are the next step's lengths and free count.  Nothing synchronizes, and lengths
-stay on the device, so a step can be captured into a CUDA graph.
+stay on the device, so a step can be captured into a CUDA graph; the operator and
+the rotary must live as long as it.
 """
 
 from __future__ import annotations

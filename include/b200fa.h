@@ -139,7 +139,8 @@ extern "C" {
 /* Sliding window with sinks, on top of B200FA_FLAG_CAUSAL (required): query
  * row i attends keys i - window < j <= i and the first `sinks` keys j <= i
  * (b200fa_options.window >= 1, .sinks >= 0).  A row that sees no key (Nq > Nk)
- * gets zeros.  Key blocks that no row of a work item sees are not read.
+ * gets zeros.  Key blocks that no row of a work item sees are not read, nor is
+ * V of any key that none of them sees.
  * Runs a separate kernel (b200_fa_window_kernel), the same for both variants:
  * softmax sums in FP32. */
 #define B200FA_FLAG_WINDOW        64u
