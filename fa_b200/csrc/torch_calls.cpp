@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <array>
+#include <atomic>
 #include <cmath>
 #include <optional>
 #include <string>
@@ -335,6 +336,18 @@ std::optional<Tensor> append(const Tensor& k, const Tensor& v, const Tensor& kp,
   return q_out;
 }
 
+// Bytes of a call's workspace: a constant of the (current) device, asked for once.
+int64_t workspace_bytes(c10::Device dev) {
+  static std::array<std::atomic<int64_t>, 64> known{};
+  auto& n = known.at(size_t(dev.index()));
+  if (n.load(std::memory_order_relaxed) == 0) {
+    const int64_t bytes = g.paged_workspace_size();
+    check(int(bytes < 0 ? bytes : 0), "b200fa_paged_workspace_size");
+    n.store(bytes, std::memory_order_relaxed);
+  }
+  return n.load(std::memory_order_relaxed);
+}
+
 Tensor paged(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& kv, const Tensor& cu,
              int64_t max_q, double scale, int64_t window, int64_t sinks, const std::optional<Tensor>& out_in, const Tensor& status,
              uint32_t timeout_us, uint32_t flags, const std::optional<Tensor>& tables_status) {
@@ -362,9 +375,7 @@ Tensor paged(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& 
   // Partial results live for this call: a block of torch's allocator belongs to
   // the call's stream, or to the graph that is being captured, so calls that
   // overlap never share one (the join finds its rows by what is written there).
-  const int64_t bytes = g.paged_workspace_size();
-  check(int(bytes < 0 ? bytes : 0), "b200fa_paged_workspace_size");
-  const Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  const Tensor ws = at::empty({workspace_bytes(dev)}, q.options().dtype(at::kByte));
   b200fa_paged_args a = {};
   a.struct_size = sizeof(a);
   a.dtype = dtype_of(q.scalar_type());

@@ -61,10 +61,10 @@ def build_tables(ctx_lens, new_lens, block_table, free_pages, free_count, *, pag
 
     ``status`` (on the GPU) is 0, or 1: too few free pages, 2: a request
     outgrows its row of block_table or 2^31 - 1 tokens, 3: more new tokens than
-    num_tokens; then nothing is handed out, every slot is -1, kv_lens are ctx_lens (cu_q still
-    counts the new tokens; ``PagedOperator.step`` gives zeros) and the table
-    is as it was.  The outputs must not overlap the inputs or one another: a
-    loop alternates between two ``StepTables``.
+    num_tokens; then nothing is handed out, every slot is -1, kv_lens are
+    ctx_lens (cu_q still counts the new tokens; ``PagedOperator.step`` gives
+    zeros) and the table is as it was.  The outputs must not overlap the inputs
+    or one another: a loop alternates between two ``StepTables``.
     """
     r = calls.load().build_tables(ctx_lens, new_lens, block_table, free_pages, free_count, page_size, num_tokens,
                                   None if out is None else out.tensors())
@@ -101,8 +101,9 @@ class PagedOperator:
 
     The operator owns the status words of each device, made by its first call
     there, which cannot be captured.  Everything else lives for one call, so
-    calls may overlap: on any streams, in any graphs.  Keep the operator as long
-    as a graph that captured a call of it."""
+    calls may overlap: on any streams, in any graphs (which, as ever, must not
+    share a memory pool if they are replayed at the same time).  Keep the
+    operator as long as a graph that captured a call of it."""
 
     def __init__(self, *, timeout_us: int = 0):
         self.timeout_us = int(timeout_us)
